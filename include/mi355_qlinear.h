@@ -698,6 +698,99 @@ MI355Q_API mi355q_status mi355q_kv_cache_read(mi355q_context* ctx, void* stream,
                                               uint32_t out_row_stride, uint32_t first_position,
                                               uint32_t sequence_length);
 
+/* ------------------------------------------------------------------------------------------
+ * 8-bit block KV cache: append, read back, attention, eviction.  No counterpart in the reference, whose quantized
+ * cache keeps a scale per token and group (mi355q_kv_cache_write above).
+ * ---------------------------------------------------------------------------------------- */
+#define MI355Q_KV_BLOCK_TOKENS 64
+/* One layer's cache: `block_count` blocks of 64 tokens for each of `kv_head_count` heads, shared by all sequences.
+ * codes_dev: int8 [block_count][kv_head_count][2][64 * head_dimension], keys then values, 16-byte aligned, codes in
+ *   [-127, 127].  A key code (token t, dimension d) lies at byte
+ *   (((t / 16) * (head_dimension / 64) + d / 64) * 4 + d / 16 % 4) * 256 + t % 16 * 16 + d % 16, a value code at byte
+ *   (d / 16 * 4 + t / 4 % 4) * 256 + d % 16 * 16 + t / 32 * 8 + t / 16 % 2 * 4 + t % 4: the orders in which the matrix
+ *   cores take their operands, so that the attention kernels read whole cache lines and never transpose.
+ * scales_dev: fp32 [block_count][kv_head_count][2], one scale for the block's keys and one for its values; a number is
+ *   code * scale.
+ * weight_sums_dev: fp32 [block_count][kv_head_count][64], the attention weight each cached token has received (needed
+ *   by mi355q_kv_block_evict and by attention with accumulate_weights; may be NULL otherwise).
+ * head_dimension is 64, 128 or 256. */
+typedef struct mi355q_kv_block_cache {
+    uint32_t kv_head_count, head_dimension, block_count, reserved0;
+    void* codes_dev;
+    float* scales_dev;
+    float* weight_sums_dev;
+} mi355q_kv_block_cache;
+/* The sequences of one call, all tables in device memory (a captured graph may be replayed with other contents).
+ * block_table_dev: int32 [sequence_count][block_table_stride], the cache block of tokens [64 j, 64 j + 64) of a sequence.
+ * lengths_dev: int32 [sequence_count], tokens of each sequence in the cache, those of this call among them.
+ * row_starts_dev: int32 [sequence_count + 1]: rows [row_starts[b], row_starts[b + 1]) of the call's row tensors are the
+ *   LAST tokens of sequence b, so row i of n stands at position length - n + i.
+ * row_count, maximum_rows, maximum_length: bounds of row_starts[sequence_count], of the rows of a sequence and of its
+ *   length, known on the host: launches are sized by them.
+ * The tables are read on the device only and are not errors there: lengths are cut to [0, maximum_length] and to the
+ * table's width, rows to [0, row_count] and to maximum_rows, and a token whose block id lies outside [0, block_count) is
+ * absent: nothing is written for it, it reads as zeros, and attention does not see it. */
+typedef struct mi355q_kv_sequences {
+    uint32_t sequence_count, block_table_stride;
+    const int32_t* block_table_dev;
+    const int32_t* lengths_dev;
+    const int32_t* row_starts_dev;
+    uint32_t row_count, maximum_rows, maximum_length, reserved0;
+} mi355q_kv_sequences;
+/* Writes the rows of k and v ([row_count, row_stride >= kv_head_count * head_dimension], head h at columns
+ * [h * head_dimension, ...); 0 = dense rows; f16, bf16 or fp32) into the blocks of their tokens.  A block's scale is
+ * amax / 127.49 over the finite values ever written to it while it held earlier tokens of the sequence: it never shrinks,
+ * and where new rows make it grow the block's earlier codes are brought to the new scale (rint(code * old / new)).
+ * A number becomes rint(x / scale), half to even, cut to [-127, 127]; a NaN becomes 0.  Weight sums of the written tokens
+ * become 0.  Blocks written by one call must be distinct (no block shared by two sequences). */
+MI355Q_API mi355q_status mi355q_kv_block_append(mi355q_context* ctx, void* stream, const mi355q_kv_block_cache* cache,
+                                                const mi355q_kv_sequences* sequences, const void* k_dev, const void* v_dev,
+                                                mi355q_dtype dtype, uint32_t row_stride);
+/* The reverse: the last tokens of each sequence as numbers (code * scale, rounded once to `dtype`). */
+MI355Q_API mi355q_status mi355q_kv_block_read(mi355q_context* ctx, void* stream, const mi355q_kv_block_cache* cache,
+                                              const mi355q_kv_sequences* sequences, void* k_dev, void* v_dev,
+                                              mi355q_dtype dtype, uint32_t row_stride);
+/* Attention of every row's `head_count` query heads (a multiple of kv_head_count; consecutive heads share a KV head) over
+ * the cached tokens at positions up to the row's own, and, with window > 0, only over the `window` last of them:
+ *   out[row, head] = sum_t softmax_t(scale * q[row, head] . k_t) v_t
+ * q and out are [row_count, stride >= head_count * head_dimension] (0 = dense), f16 or bf16 both, each its own type.
+ * lse_dev (or NULL): fp32 [row_count, head_count], log sum_t exp(scale * q . k_t).  A row that sees no token gets zeros
+ * and -inf.  With accumulate_weights the softmax weights every token received from the call's rows and heads are added to
+ * the cache's weight sums, in a fixed order (the same inputs give the same bits).  Products with the 8-bit codes are
+ * exact, sums, maxima and weights fp32; the weights are rounded to f16 in front of the product with the values.
+ * Partial results and scores live in the context's scratch. */
+MI355Q_API mi355q_status mi355q_kv_block_attention(mi355q_context* ctx, void* stream, const mi355q_kv_block_cache* cache,
+                                                   const mi355q_kv_sequences* sequences, const void* q_dev,
+                                                   mi355q_dtype q_dtype, uint32_t q_row_stride, uint32_t head_count,
+                                                   float scale, uint32_t window, void* out_dev, mi355q_dtype out_dtype,
+                                                   uint32_t out_row_stride, float* lse_dev, int accumulate_weights);
+/* Reduces every sequence to at most `budget` tokens: for each KV head the first `sinks` and the last `recent` tokens and
+ * those of the others that received most attention weight (cache->weight_sums_dev; equal sums: the lowest position; a
+ * NaN sum counts as less than any).  What is kept goes, in order, to the blocks of new_block_table_dev ([sequence_count]
+ * [new_block_table_stride], at least ceil(budget / 64) entries a row, none of them a block that a sequence of the call
+ * holds), with the weight sums; a new block takes the largest scale of its tokens' old blocks, and codes from blocks of
+ * smaller scale are rounded once more.  Codes, sums and scales behind the kept tokens are cleared.  new_lengths_dev gets
+ * min(length, budget); positions_dev (or NULL), int32 [sequence_count][kv_head_count][budget], the old position of every
+ * kept token (the entries behind the last are left alone).  sequences->row_starts_dev and the row bounds are not read. */
+MI355Q_API mi355q_status mi355q_kv_block_evict(mi355q_context* ctx, void* stream, const mi355q_kv_block_cache* cache,
+                                               const mi355q_kv_sequences* sequences, uint32_t budget, uint32_t recent,
+                                               uint32_t sinks, const int32_t* new_block_table_dev,
+                                               uint32_t new_block_table_stride, int32_t* new_lengths_dev,
+                                               int32_t* positions_dev);
+
+/* What a served token is reported with, from rows of logits ([row_count, row_stride >= vocabulary_size], 0 = dense):
+ * log softmax(logits)[token_ids[row]], the entropy of the softmax in nats, and the `top_count` (0 to 32) likeliest tokens
+ * in order with their log probabilities ([row_count, top_count]; equal logits: the lowest index first).  A NaN logit
+ * counts as -inf (a masked token), +inf as the largest finite number.  Masked tokens are no alternatives: places that
+ * nothing fills hold -1 and -inf.  A row that is masked throughout has entropy 0 and log probability -inf; so has a token
+ * id outside the vocabulary.  token_ids_dev and logprob_dev go together and may be NULL both, entropy_dev may be NULL.
+ * Partial results live in the context's scratch. */
+MI355Q_API mi355q_status mi355q_token_logprobs(mi355q_context* ctx, void* stream, const void* logits_dev,
+                                               mi355q_dtype dtype, uint32_t row_count, uint32_t vocabulary_size,
+                                               uint32_t row_stride, const int32_t* token_ids_dev, float* logprob_dev,
+                                               float* entropy_dev, uint32_t top_count, int32_t* top_ids_dev,
+                                               float* top_logprobs_dev);
+
 #ifdef __cplusplus
 }
 #endif

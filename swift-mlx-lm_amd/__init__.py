@@ -101,6 +101,18 @@ class _KvLayout(C.Structure):
                 ("maximum_sequence_length", C.c_uint32), ("head_slot_bytes", C.c_uint32)]
 
 
+class _KvBlockCache(C.Structure):
+    _fields_ = [("kv_head_count", C.c_uint32), ("head_dimension", C.c_uint32), ("block_count", C.c_uint32),
+                ("reserved0", C.c_uint32), ("codes_dev", C.c_void_p), ("scales_dev", C.c_void_p),
+                ("weight_sums_dev", C.c_void_p)]
+
+
+class _KvSequences(C.Structure):
+    _fields_ = [("sequence_count", C.c_uint32), ("block_table_stride", C.c_uint32), ("block_table_dev", C.c_void_p),
+                ("lengths_dev", C.c_void_p), ("row_starts_dev", C.c_void_p), ("row_count", C.c_uint32),
+                ("maximum_rows", C.c_uint32), ("maximum_length", C.c_uint32), ("reserved0", C.c_uint32)]
+
+
 class _DeviceInfo(C.Structure):
     _fields_ = [("name", C.c_char * 64), ("arch", C.c_char * 32), ("compute_units", C.c_int32),
                 ("wavefront_size", C.c_int32), ("lds_bytes_per_workgroup", C.c_int32), ("reserved0", C.c_int32),
@@ -210,6 +222,12 @@ def library() -> C.CDLL:
         "mi355q_kv_bytes_per_head_slot": (u32, [u8, u32]),
         "mi355q_kv_cache_write": (i32, [vp, vp, P(_KvLayout), vp, vp, C.c_int, u32, u32, u32]),
         "mi355q_kv_cache_read": (i32, [vp, vp, P(_KvLayout), vp, vp, C.c_int, u32, u32, u32]),
+        "mi355q_kv_block_append": (i32, [vp, vp, P(_KvBlockCache), P(_KvSequences), vp, vp, C.c_int, u32]),
+        "mi355q_kv_block_read": (i32, [vp, vp, P(_KvBlockCache), P(_KvSequences), vp, vp, C.c_int, u32]),
+        "mi355q_kv_block_attention": (i32, [vp, vp, P(_KvBlockCache), P(_KvSequences), vp, C.c_int, u32, u32, C.c_float, u32,
+                                            vp, C.c_int, u32, vp, C.c_int]),
+        "mi355q_kv_block_evict": (i32, [vp, vp, P(_KvBlockCache), P(_KvSequences), u32, u32, u32, vp, u32, vp, vp]),
+        "mi355q_token_logprobs": (i32, [vp, vp, vp, C.c_int, u32, u32, u32, vp, vp, vp, u32, vp, vp]),
         "mi355q_staf_open": (i32, [C.c_char_p, P(vp)]),
         "mi355q_staf_close": (None, [vp]),
         "mi355q_staf_format_version": (u32, [vp]),
@@ -699,6 +717,43 @@ class KVCacheSpecification:
                          self.maximum_sequence_length, self.bytes_per_head_slot)
 
 
+KV_BLOCK_TOKENS = 64
+
+
+class KVBlockCache:
+    """One layer's 8-bit block cache: int8 codes [block][head][key, value][64 x head_dimension], fp32 scales
+    [block][head][key, value] and, for eviction, the weight sums [block][head][64], all in device memory of the caller."""
+
+    def __init__(self, kv_head_count: int, head_dimension: int, block_count: int, codes, scales, weight_sums=None):
+        self.kv_head_count, self.head_dimension, self.block_count = kv_head_count, head_dimension, block_count
+        self._keepalive = (codes, scales, weight_sums)
+        self._c = _KvBlockCache(kv_head_count, head_dimension, block_count, 0, Context._ptr(codes), Context._ptr(scales),
+                                Context._ptr(weight_sums))
+
+    @staticmethod
+    def codes_bytes(kv_head_count: int, head_dimension: int, block_count: int) -> int:
+        return block_count * kv_head_count * 2 * KV_BLOCK_TOKENS * head_dimension
+
+    @staticmethod
+    def scales_bytes(kv_head_count: int, block_count: int) -> int:
+        return block_count * kv_head_count * 2 * 4
+
+    @staticmethod
+    def weight_sums_bytes(kv_head_count: int, block_count: int) -> int:
+        return block_count * kv_head_count * KV_BLOCK_TOKENS * 4
+
+
+class KVSequences:
+    """The sequences of one call over a block cache: block table, lengths and row starts (int32, device memory) and the
+    bounds of the rows and lengths that the host knows."""
+
+    def __init__(self, sequence_count: int, block_table, block_table_stride: int, lengths, row_starts, row_count: int,
+                 maximum_rows: int, maximum_length: int):
+        self._keepalive = (block_table, lengths, row_starts)
+        self._c = _KvSequences(sequence_count, block_table_stride, Context._ptr(block_table), Context._ptr(lengths),
+                               Context._ptr(row_starts), row_count, maximum_rows, maximum_length, 0)
+
+
 def shape_family(output_dimension: int, input_dimension: int):
     """DecodeProjectionShapeFamily.resolve -> (family, preferredSimdgroups, tileElements, kernelBaseName)."""
     fam, sg, tile = C.c_int32(), C.c_uint32(), C.c_uint32()
@@ -917,3 +972,35 @@ class Context:
         """The same head through the entry point that allocates nothing (its partial keys live in the library image)."""
         _check(library().mi355q_lmhead_argmax_static(self.handle, stream, w.handle, self._ptr(x), x_dtype,
                                                      self._ptr(logits_f32), self._ptr(token_out), flags))
+
+    # ---- 8-bit block cache
+    def kv_block_append(self, cache: KVBlockCache, sequences: KVSequences, k, v, dtype, row_stride=0, stream=0):
+        """The rows of k and v become the last tokens of their sequences."""
+        _check(library().mi355q_kv_block_append(self.handle, stream, cache._c, sequences._c, self._ptr(k), self._ptr(v),
+                                                dtype, row_stride))
+
+    def kv_block_read(self, cache: KVBlockCache, sequences: KVSequences, k, v, dtype, row_stride=0, stream=0):
+        """The last tokens of each sequence as rows of numbers."""
+        _check(library().mi355q_kv_block_read(self.handle, stream, cache._c, sequences._c, self._ptr(k), self._ptr(v),
+                                              dtype, row_stride))
+
+    def kv_block_attention(self, cache: KVBlockCache, sequences: KVSequences, q, q_dtype, head_count, out, out_dtype, scale,
+                           window=0, lse=None, accumulate_weights=False, q_row_stride=0, out_row_stride=0, stream=0):
+        """Causal attention of the rows over the cached tokens of their sequences."""
+        _check(library().mi355q_kv_block_attention(self.handle, stream, cache._c, sequences._c, self._ptr(q), q_dtype,
+                                                   q_row_stride, head_count, scale, window, self._ptr(out), out_dtype,
+                                                   out_row_stride, self._ptr(lse), 1 if accumulate_weights else 0))
+
+    def kv_block_evict(self, cache: KVBlockCache, sequences: KVSequences, budget, new_block_table, new_block_table_stride,
+                       new_lengths, recent=0, sinks=0, positions=None, stream=0):
+        """Keeps the tokens of every sequence and KV head that received most attention weight, in new blocks."""
+        _check(library().mi355q_kv_block_evict(self.handle, stream, cache._c, sequences._c, budget, recent, sinks,
+                                               self._ptr(new_block_table), new_block_table_stride,
+                                               self._ptr(new_lengths), self._ptr(positions)))
+
+    def token_logprobs(self, logits, dtype, row_count, vocabulary_size, token_ids=None, top_count=0, logprob=None,
+                       entropy=None, top_ids=None, top_logprobs=None, row_stride=0, stream=0):
+        """Log probability of a token of each row, the row's entropy and its likeliest tokens."""
+        _check(library().mi355q_token_logprobs(self.handle, stream, self._ptr(logits), dtype, row_count, vocabulary_size,
+                                               row_stride, self._ptr(token_ids), self._ptr(logprob), self._ptr(entropy),
+                                               top_count, self._ptr(top_ids), self._ptr(top_logprobs)))

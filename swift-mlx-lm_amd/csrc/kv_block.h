@@ -1,0 +1,92 @@
+// The 8-bit block KV cache as its kernels see it (kv_block_cache.hip, kv_block_attention.hip).
+#pragma once
+
+#include "device_utils.h"
+
+namespace mi355q {
+
+constexpr uint32_t kKvTokens = MI355Q_KV_BLOCK_TOKENS;
+
+// The tables of a call and the cache.  Everything read from the tables is cut to what the host knows before it becomes
+// an address, so no content of theirs leads outside the caller's buffers.
+struct KvBlockArgs {
+    int8_t* codes;
+    float* scales;
+    float* sums;
+    const int32_t* table;
+    const int32_t* lengths;
+    const int32_t* starts;
+    uint32_t kv_heads, block_count, sequences, table_stride, row_count, max_rows, max_length;
+};
+
+// Sequence b of a call: `rows` rows from `row0` on, the last of its `length` tokens.  Rows may be more than tokens: then
+// the first of them stand at negative positions.
+struct KvSequence {
+    int32_t row0, rows, length;
+    const int32_t* table;
+    __device__ int32_t first() const { return length - rows; }      // position of row 0
+};
+
+__device__ __forceinline__ int32_t kv_length(const KvBlockArgs& a, uint32_t b) {
+    const int64_t most = min((int64_t)a.max_length, (int64_t)a.table_stride * kKvTokens);
+    const int64_t l = a.lengths[b];
+    return (int32_t)(l < 0 ? 0 : l < most ? l : most);
+}
+
+__device__ __forceinline__ KvSequence kv_sequence(const KvBlockArgs& a, uint32_t b) {
+    KvSequence s;
+    const int32_t r0 = a.starts[b], r1 = a.starts[b + 1];
+    s.length = kv_length(a, b);
+    s.table = a.table + (size_t)b * a.table_stride;
+    s.row0 = r0;
+    const bool sane = r0 >= 0 && r1 > r0 && (uint32_t)r1 <= a.row_count && (uint32_t)(r1 - r0) <= a.max_rows;
+    s.rows = sane ? r1 - r0 : 0;
+    return s;
+}
+
+// Cache block of tokens [64 j, 64 j + 64), -1 if absent (the caller keeps j inside the length).
+__device__ __forceinline__ int32_t kv_block_id(const KvBlockArgs& a, const int32_t* table, int32_t j) {
+    const int32_t id = table[j];
+    return (uint32_t)id < a.block_count ? id : -1;
+}
+
+template <int HD>
+__device__ __forceinline__ int8_t* kv_codes(const KvBlockArgs& a, int32_t block, uint32_t head, uint32_t part) {
+    return a.codes + (((size_t)block * a.kv_heads + head) * 2 + part) * (kKvTokens * HD);
+}
+__device__ __forceinline__ float* kv_scale(const KvBlockArgs& a, int32_t block, uint32_t head, uint32_t part) {
+    return a.scales + ((size_t)block * a.kv_heads + head) * 2 + part;
+}
+__device__ __forceinline__ float* kv_sums(const KvBlockArgs& a, int32_t block, uint32_t head) {
+    return a.sums + ((size_t)block * a.kv_heads + head) * kKvTokens;
+}
+
+// Byte of a code inside its 64 x HD codes.  Both orders are made of 16-byte pieces.  Keys: a piece is 16 dimensions of a
+// token, sixteen tokens of a tile side by side, the four pieces of 64 dimensions behind one another: 64 lanes of a
+// matrix operand (token = lane % 16, dimensions by lane / 16) are 1 KiB in a row.  Values: a piece is a dimension's codes
+// of the sixteen tokens whose scores lane group c = t / 4 % 4 of the score tile holds, so weights become an operand
+// without leaving their registers.
+template <int HD>
+__device__ __forceinline__ uint32_t kv_key_byte(uint32_t t, uint32_t d) {
+    return (((t >> 4) * (HD / 64) + (d >> 6)) * 4 + ((d >> 4) & 3)) * 256 + (t & 15) * 16 + (d & 15);
+}
+template <int HD>
+__device__ __forceinline__ uint32_t kv_value_byte(uint32_t t, uint32_t d) {
+    return ((d >> 4) * 4 + ((t >> 2) & 3)) * 256 + (d & 15) * 16 + (t >> 5) * 8 + ((t >> 4) & 1) * 4 + (t & 3);
+}
+
+// Checks shared by the entry points; fills the kernel arguments (kv_block_cache.hip).  `rows`: the call reads row tables.
+mi355q_status kv_block_prepare(const mi355q_context* ctx, const mi355q_kv_block_cache* cache,
+                               const mi355q_kv_sequences* sequences, bool rows, KvBlockArgs* out);
+
+// f(integral_constant<int, head dimension>)
+template <typename F>
+mi355q_status kv_with_head_dimension(uint32_t hd, F&& f) {
+    switch (hd) {
+    case 64: return f(std::integral_constant<int, 64>{});
+    case 128: return f(std::integral_constant<int, 128>{});
+    default: return f(std::integral_constant<int, 256>{});
+    }
+}
+
+}  // namespace mi355q

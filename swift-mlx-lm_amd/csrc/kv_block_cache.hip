@@ -1,0 +1,555 @@
+// 8-bit block KV cache: append (quantise rows into blocks), read back, eviction by attention weight.
+//
+// A block is 64 tokens of one KV head; its keys and its values have one fp32 scale each.  All kernels here are HBM-bound
+// (a few operations a byte) and mostly small: a workgroup owns the keys or the values of one block, holds their 64 x HD
+// codes in LDS in cache order and moves them to and from memory 16 bytes a lane.
+#include "kv_block.h"
+
+namespace mi355q {
+
+// The divisor is a little under 127.5, so the largest magnitude still becomes 127, the step is as fine as it can be, and
+// the 8-bit mantissas of bf16 rows do not fall on the middle between two codes (with 127 every x = amax / 2 would: 63.5,
+// decided by the last bit of the scale).
+constexpr float kInverseSteps = (float)(1.0 / 127.49);
+
+// x / scale to the nearest code, half to even.  fmin and fmax drop a NaN, so it is sorted out first.
+__device__ __forceinline__ int kv_code(float x, float scale) {
+    const float q = rintf(__fdiv_rn(x, scale));
+    return x != x ? 0 : (int)fminf(fmaxf(q, -127.0f), 127.0f);
+}
+
+// four codes of a word times `ratio` (at most one), each to the nearest code
+__device__ __forceinline__ uint32_t kv_rescale4(uint32_t w, float ratio) {
+    uint32_t out = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) out |= ((uint32_t)(int)rintf((float)(int8_t)(w >> (8 * i)) * ratio) & 0xFFu) << (8 * i);
+    return out;
+}
+
+// Pieces of a block in LDS: one 16-byte gap behind every sixteen, so that the lanes of a wavefront, which write four
+// bytes into pieces 64 or 256 bytes apart, spread over the banks.
+__device__ __forceinline__ uint32_t lds_piece(uint32_t byte) { return byte + ((byte >> 8) << 4); }
+template <int HD>
+constexpr uint32_t kKvLdsBytes = kKvTokens * HD + kKvTokens * HD / 16;
+
+// Eight consecutive elements of a row, from element i on (`vec`: 16-byte aligned).
+template <int D>
+__device__ __forceinline__ void load8(const void* p, size_t i, bool vec, float (&x)[8]) {
+    if (vec) {
+        if constexpr (D == MI355Q_F32) {
+            const float4 lo = *(const float4*)((const float*)p + i), hi = *(const float4*)((const float*)p + i + 4);
+            x[0] = lo.x; x[1] = lo.y; x[2] = lo.z; x[3] = lo.w; x[4] = hi.x; x[5] = hi.y; x[6] = hi.z; x[7] = hi.w;
+        } else {
+            const uint4 w = *(const uint4*)((const uint16_t*)p + i);
+            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const uint16_t h = (uint16_t)(ws[e >> 1] >> (16 * (e & 1)));
+                x[e] = D == MI355Q_BF16 ? bf16_to_f32(h) : f16_to_f32(h);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = load_act<D>(p, i + e);
+    }
+}
+
+template <int D>
+__device__ __forceinline__ void store8(void* p, size_t i, bool vec, const float (&x)[8]) {
+    if (vec && D != MI355Q_F32) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const uint16_t lo = D == MI355Q_BF16 ? f32_to_bf16_rne(x[2 * e]) : f32_to_f16_rne(x[2 * e]);
+            const uint16_t hi = D == MI355Q_BF16 ? f32_to_bf16_rne(x[2 * e + 1]) : f32_to_f16_rne(x[2 * e + 1]);
+            w[e] = (uint32_t)lo | ((uint32_t)hi << 16);
+        }
+        *(uint4*)((uint16_t*)p + i) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else if (vec) {
+        *(float4*)((float*)p + i) = make_float4(x[0], x[1], x[2], x[3]);
+        *(float4*)((float*)p + i + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) store_out<D>(p, i + e, x[e]);
+    }
+}
+
+// Keys (part 0) or values (part 1) of one touched block and head: 2 HD threads, each four consecutive tokens (a quad) of
+// eight dimensions, which is four 8-byte runs of keys or eight words of values.
+template <int HD, int D>
+__global__ __launch_bounds__(2 * HD) void kv_block_append_kernel(KvBlockArgs a, const void* k, const void* v,
+                                                                 uint32_t row_stride, bool vec) {
+    __shared__ __align__(16) uint8_t lds[kKvLdsBytes<HD>];
+    __shared__ float wave_top[2 * HD / 64];
+    const KvSequence s = kv_sequence(a, blockIdx.z);
+    const uint32_t head = blockIdx.y >> 1, part = blockIdx.y & 1;
+    const int32_t first = max(s.first(), 0), j = first / (int32_t)kKvTokens + (int32_t)blockIdx.x;
+    if (s.rows <= 0 || j * (int32_t)kKvTokens >= s.length) return;
+    const int32_t block = kv_block_id(a, s.table, j);
+    if (block < 0) return;
+    const int32_t base = j * (int32_t)kKvTokens;
+    const uint32_t lo = (uint32_t)max(first - base, 0), hi = (uint32_t)min(s.length - base, (int32_t)kKvTokens);
+    const uint32_t tid = threadIdx.x, d8 = tid % (HD / 8), quad = tid / (HD / 8);
+    float x[4][8];
+    float top = 0.0f;
+    const void* src = part ? v : k;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t t = quad * 4 + i;
+        if (t >= lo && t < hi) {
+            const size_t row = (size_t)(s.row0 + (base + (int32_t)t - s.first()));
+            load8<D>(src, row * row_stride + (size_t)head * HD + d8 * 8, vec, x[i]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[i][e]) <= 3.402823466e38f ? fabsf(x[i][e]) : 0.0f);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[i][e] = 0.0f;
+        }
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    if ((tid & 63) == 0) wave_top[tid >> 6] = top;
+    float* const scale_at = kv_scale(a, block, head, part);
+    const float old = lo ? *scale_at : 0.0f;
+    __syncthreads();
+    for (int w = 0; w < 2 * HD / 64; w++) top = fmaxf(top, wave_top[w]);
+    const float scale = fmaxf(old, top * kInverseSteps);
+    int8_t* const codes = kv_codes<HD>(a, block, head, part);
+    const float divisor = scale > 0.0f ? scale : 1.0f;
+    uint32_t c[4][2];                                      // codes of token i: dimensions 0..3, 4..7
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            c[i][h] = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) c[i][h] |= ((uint32_t)kv_code(x[i][4 * h + e], divisor) & 0xFFu) << (8 * e);
+        }
+    if (part == 0 && a.sums && tid < kKvTokens && tid >= lo && tid < hi) kv_sums(a, block, head)[tid] = 0.0f;
+    if (tid == 0) *scale_at = scale;
+    if (lo && scale == old) {                              // earlier tokens stay as they are: only the new codes are written
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t t = quad * 4 + i;
+            if (t < lo || t >= hi) continue;
+            if (part == 0) {
+                *(uint2*)(codes + kv_key_byte<HD>(t, d8 * 8)) = make_uint2(c[i][0], c[i][1]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) codes[kv_value_byte<HD>(t, d8 * 8 + e)] = (int8_t)(c[i][e >> 2] >> (8 * (e & 3)));
+            }
+        }
+        return;
+    }
+    if (lo) {                                              // the block's codes to the new scale
+        const float ratio = __fdiv_rn(old, divisor);
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            const uint32_t byte = (r * 2 * HD + tid) * 16;
+            uint4 w = *(const uint4*)(codes + byte);
+            w.x = kv_rescale4(w.x, ratio); w.y = kv_rescale4(w.y, ratio);
+            w.z = kv_rescale4(w.z, ratio); w.w = kv_rescale4(w.w, ratio);
+            *(uint4*)(lds + lds_piece(byte)) = w;
+        }
+        __syncthreads();
+    }
+    const bool whole = quad * 4 >= lo;                     // (tokens behind the new ones get zeros)
+    if (part == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t t = quad * 4 + i;
+            if (t >= lo) *(uint2*)(lds + lds_piece(kv_key_byte<HD>(t, d8 * 8))) = make_uint2(c[i][0], c[i][1]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const uint32_t at = lds_piece(kv_value_byte<HD>(quad * 4, d8 * 8 + e));
+            uint32_t w = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) w |= ((c[i][e >> 2] >> (8 * (e & 3))) & 0xFFu) << (8 * i);
+            if (whole) {
+                *(uint32_t*)(lds + at) = w;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (quad * 4 + i >= lo) lds[at + i] = (uint8_t)(w >> (8 * i));
+            }
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        const uint32_t byte = (r * 2 * HD + tid) * 16;
+        *(uint4*)(codes + byte) = *(const uint4*)(lds + lds_piece(byte));
+    }
+}
+
+// The reverse, the same thread layout.
+template <int HD, int D>
+__global__ __launch_bounds__(2 * HD) void kv_block_read_kernel(KvBlockArgs a, void* k, void* v, uint32_t row_stride, bool vec) {
+    __shared__ __align__(16) uint8_t lds[kKvLdsBytes<HD>];
+    const KvSequence s = kv_sequence(a, blockIdx.z);
+    const uint32_t head = blockIdx.y >> 1, part = blockIdx.y & 1;
+    // rows in front of the first token (more rows than tokens) read as zeros: block -1, -2, ... holds them
+    const int32_t first = s.first(), j = (first >= 0 ? first : first - (int32_t)kKvTokens + 1) / (int32_t)kKvTokens + (int32_t)blockIdx.x;
+    const int32_t base = j * (int32_t)kKvTokens;
+    if (s.rows <= 0 || base >= s.length) return;
+    const int32_t block = j >= 0 ? kv_block_id(a, s.table, j) : -1;
+    const uint32_t tid = threadIdx.x, d8 = tid % (HD / 8), quad = tid / (HD / 8);
+    float scale = 0.0f;
+    if (block >= 0) {
+        const int8_t* const codes = kv_codes<HD>(a, block, head, part);
+        scale = *kv_scale(a, block, head, part);
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            const uint32_t byte = (r * 2 * HD + tid) * 16;
+            *(uint4*)(lds + lds_piece(byte)) = *(const uint4*)(codes + byte);
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < 2; r++) *(uint4*)(lds + lds_piece((r * 2 * HD + tid) * 16)) = make_uint4(0, 0, 0, 0);
+    }
+    __syncthreads();
+    uint32_t c[4][2];
+    if (part == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint2 w = *(const uint2*)(lds + lds_piece(kv_key_byte<HD>(quad * 4 + i, d8 * 8)));
+            c[i][0] = w.x; c[i][1] = w.y;
+        }
+    } else {
+        uint32_t w[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) w[e] = *(const uint32_t*)(lds + lds_piece(kv_value_byte<HD>(quad * 4, d8 * 8 + e)));
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                c[i][h] = 0;
+#pragma unroll
+                for (int e = 0; e < 4; e++) c[i][h] |= ((w[4 * h + e] >> (8 * i)) & 0xFFu) << (8 * e);
+            }
+    }
+    void* const dst = part ? v : k;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int32_t p = base + (int32_t)(quad * 4 + i);
+        if (p < first || p >= s.length) continue;
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = (float)(int8_t)(c[i][e >> 2] >> (8 * (e & 3))) * scale;
+        store8<D>(dst, (size_t)(s.row0 + (p - first)) * row_stride + (size_t)head * HD + d8 * 8, vec, x);
+    }
+}
+
+// ---- eviction ----------------------------------------------------------------------------------------------------------
+
+struct EvictArgs {
+    uint32_t budget, recent, sinks, new_stride;
+    const int32_t* new_table;
+    int32_t* new_lengths;
+    int32_t* positions;       // [sequence][head][budget], ascending
+};
+
+// Weight sums in the order of their value, as unsigned numbers (-0 like 0, a NaN under all).
+__device__ __forceinline__ uint32_t sum_key(float v) {
+    if (v != v) return 0;
+    const uint32_t u = __float_as_uint(v + 0.0f);
+    return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+
+constexpr uint32_t kSelectThreads = 1024;
+
+// One workgroup per sequence and head: the key of the last token kept is found digit by digit (four histograms of 256),
+// then the positions are written in order, ties with that key from the lowest position on.
+__global__ __launch_bounds__(kSelectThreads) void kv_block_select_kernel(KvBlockArgs a, EvictArgs e) {
+    __shared__ uint32_t bins[256];
+    __shared__ uint32_t digit, wanted;
+    __shared__ uint32_t wave_above[kSelectThreads / 64], wave_ties[kSelectThreads / 64];
+    const uint32_t head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t length = (uint32_t)kv_length(a, b);
+    const int32_t* const table = a.table + (size_t)b * a.table_stride;
+    int32_t* const out = e.positions + ((size_t)b * a.kv_heads + head) * e.budget;
+    if (head == 0 && tid == 0) e.new_lengths[b] = (int32_t)min(length, e.budget);
+    if (length <= e.budget) {
+        for (uint32_t t = tid; t < length; t += kSelectThreads) out[t] = (int32_t)t;
+        return;
+    }
+    // budget >= sinks + recent and length > budget: the tokens between the two are more than those wanted of them
+    const uint32_t low = e.sinks, high = length - e.recent;
+    auto key_of = [&](uint32_t t) {
+        const int32_t block = kv_block_id(a, table, (int32_t)(t / kKvTokens));
+        return block < 0 ? sum_key(0.0f) : sum_key(kv_sums(a, block, head)[t % kKvTokens]);
+    };
+    uint32_t prefix = 0, need = e.budget - e.sinks - e.recent;     // tokens wanted among those whose key starts with prefix
+    const bool any = need > 0;
+    for (int shift = 24; any && shift >= 0; shift -= 8) {
+        if (tid < 256) bins[tid] = 0;
+        __syncthreads();
+        for (uint32_t t = low + tid; t < high; t += kSelectThreads) {
+            const uint32_t key = key_of(t);
+            if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&bins[(key >> shift) & 255u], 1u);
+        }
+        __syncthreads();
+        if (tid == 0) {
+            uint32_t left = need, d = 255;
+            while (d > 0 && bins[d] < left) left -= bins[d--];
+            digit = d; wanted = left;
+        }
+        __syncthreads();
+        prefix |= digit << shift;
+        need = wanted;
+    }
+    // `need` tokens with exactly this key, the first of them, and all with a larger one
+    uint32_t written = 0, ties = 0;
+    for (uint32_t start = 0; start < length; start += kSelectThreads) {
+        const uint32_t t = start + tid;
+        bool keep = t < length && (t < low || t >= high), tie = false;
+        if (any && t >= low && t < high) {
+            const uint32_t key = key_of(t);
+            keep = key > prefix;
+            tie = key == prefix;
+        }
+        const uint64_t tie_mask = __ballot(tie);
+        if (lane == 0) wave_ties[wave] = (uint32_t)__popcll(tie_mask);
+        __syncthreads();
+        uint32_t before = ties, all_ties = ties;
+        for (uint32_t w = 0; w < kSelectThreads / 64; w++) {
+            if (w < wave) before += wave_ties[w];
+            all_ties += wave_ties[w];
+        }
+        keep |= tie && before + (uint32_t)__popcll(tie_mask & ((1ull << lane) - 1)) < need;
+        const uint64_t mask = __ballot(keep);
+        if (lane == 0) wave_above[wave] = (uint32_t)__popcll(mask);
+        __syncthreads();
+        uint32_t at = written, all = written;
+        for (uint32_t w = 0; w < kSelectThreads / 64; w++) {
+            if (w < wave) at += wave_above[w];
+            all += wave_above[w];
+        }
+        at += (uint32_t)__popcll(mask & ((1ull << lane) - 1));
+        if (keep && at < e.budget) out[at] = (int32_t)t;
+        written = all;
+        ties = all_ties;
+        __syncthreads();
+    }
+}
+
+// One workgroup per new block, head and sequence: keys and values of its 64 kept tokens, gathered piece by piece (keys)
+// and code by code (values, whose pieces hold sixteen tokens), brought to the largest of their scales.
+template <int HD>
+__global__ __launch_bounds__(2 * HD) void kv_block_gather_kernel(KvBlockArgs a, EvictArgs e) {
+    __shared__ int32_t block_of[kKvTokens];               // source block of each kept token, -1: none
+    __shared__ uint32_t token_of[kKvTokens];
+    __shared__ float ratio[2][kKvTokens];
+    const uint32_t j = blockIdx.x, head = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+    const uint32_t length = (uint32_t)kv_length(a, b), kept = min(length, e.budget);
+    const int32_t target = e.new_table[(size_t)b * e.new_stride + j];
+    if ((uint32_t)target >= a.block_count) return;
+    const int32_t* const table = a.table + (size_t)b * a.table_stride;
+    if (tid < kKvTokens) {                                // the first wavefront
+        const uint32_t at = j * kKvTokens + tid;
+        int32_t source = -1;
+        uint32_t token = 0;
+        float scale[2] = {0.0f, 0.0f}, sum = 0.0f;
+        if (at < kept) {
+            // written by the launch before this one; always inside the length
+            const uint32_t p = (uint32_t)e.positions[((size_t)b * a.kv_heads + head) * e.budget + at];
+            source = kv_block_id(a, table, (int32_t)(p / kKvTokens));
+            token = p % kKvTokens;
+            if (source >= 0) {
+                scale[0] = *kv_scale(a, source, head, 0);
+                scale[1] = *kv_scale(a, source, head, 1);
+                sum = kv_sums(a, source, head)[token];
+            }
+        }
+        block_of[tid] = source;
+        token_of[tid] = token;
+#pragma unroll
+        for (int part = 0; part < 2; part++) {
+            float top = scale[part];
+#pragma unroll
+            for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+            ratio[part][tid] = __fdiv_rn(scale[part], top > 0.0f ? top : 1.0f);
+            if (tid == 0) *kv_scale(a, target, head, (uint32_t)part) = top;
+        }
+        kv_sums(a, target, head)[tid] = sum;
+    }
+    __syncthreads();
+    int8_t* const keys = kv_codes<HD>(a, target, head, 0);
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        const uint32_t piece = r * 2 * HD + tid;
+        const uint32_t t = (piece / (4 * (HD / 64) * 16)) * 16 + piece % 16, within = piece / 16 % (4 * (HD / 64));
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (block_of[t] >= 0) {
+            const uint32_t u = token_of[t];
+            w = *(const uint4*)(kv_codes<HD>(a, block_of[t], head, 0) + ((u >> 4) * (HD / 64) * 4 + within) * 256 + (u & 15) * 16);
+            const float f = ratio[0][t];
+            w.x = kv_rescale4(w.x, f); w.y = kv_rescale4(w.y, f); w.z = kv_rescale4(w.z, f); w.w = kv_rescale4(w.w, f);
+        }
+        *(uint4*)(keys + piece * 16) = w;
+    }
+    int8_t* const values = kv_codes<HD>(a, target, head, 1);
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        const uint32_t piece = r * 2 * HD + tid;           // dimension piece / 64 * 16 + piece % 16, lane group piece / 16 % 4
+        const uint32_t d = piece / 64 * 16 + piece % 16, c = piece / 16 % 4;
+        uint32_t w[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            w[q] = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t t = (uint32_t)q * 16 + c * 4 + i;
+                if (block_of[t] < 0) continue;
+                const float code = (float)kv_codes<HD>(a, block_of[t], head, 1)[kv_value_byte<HD>(token_of[t], d)];
+                w[q] |= ((uint32_t)(int)rintf(code * ratio[1][t]) & 0xFFu) << (8 * i);
+            }
+        }
+        *(uint4*)(values + piece * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// ---- host --------------------------------------------------------------------------------------------------------------
+
+mi355q_status kv_block_prepare(const mi355q_context* ctx, const mi355q_kv_block_cache* cache,
+                               const mi355q_kv_sequences* sequences, bool rows, KvBlockArgs* out) {
+    if (!ctx) return fail(MI355Q_ERR_NULL_HANDLE, "context is null");
+    if (!cache || !sequences) return fail(MI355Q_ERR_INVALID_ARGUMENT, "null cache or sequences");
+    if (cache->head_dimension != 64 && cache->head_dimension != 128 && cache->head_dimension != 256)
+        return fail(MI355Q_ERR_UNSUPPORTED_FORMAT, "the block cache holds heads of 64, 128 or 256 dimensions (got %u)", cache->head_dimension);
+    if (!cache->kv_head_count || !cache->block_count) return fail(MI355Q_ERR_SHAPE, "a block cache needs heads and blocks");
+    if (cache->kv_head_count > 32767) return fail(MI355Q_ERR_SHAPE, "%u KV heads: at most 32767", cache->kv_head_count);
+    if (cache->block_count > 0x7FFFFFFFu) return fail(MI355Q_ERR_SHAPE, "block ids are int32: %u blocks", cache->block_count);
+    if (!cache->codes_dev || !cache->scales_dev) return fail(MI355Q_ERR_INVALID_ARGUMENT, "null codes or scales");
+    if ((uintptr_t)cache->codes_dev % 16 || (uintptr_t)cache->scales_dev % 4 || (uintptr_t)cache->weight_sums_dev % 4)
+        return fail(MI355Q_ERR_INVALID_ARGUMENT, "misaligned cache: codes to 16 bytes, scales and weight sums to 4");
+    if (!sequences->sequence_count || !sequences->block_table_stride) return fail(MI355Q_ERR_SHAPE, "no sequences or an empty block table");
+    if (sequences->sequence_count > 65535) return fail(MI355Q_ERR_SHAPE, "%u sequences in one call: at most 65535", sequences->sequence_count);
+    if (!sequences->block_table_dev || !sequences->lengths_dev || (rows && !sequences->row_starts_dev))
+        return fail(MI355Q_ERR_INVALID_ARGUMENT, "null block table, lengths or row starts");
+    if ((uintptr_t)sequences->block_table_dev % 4 || (uintptr_t)sequences->lengths_dev % 4 || (uintptr_t)sequences->row_starts_dev % 4)
+        return fail(MI355Q_ERR_INVALID_ARGUMENT, "misaligned block table, lengths or row starts");
+    if (!sequences->maximum_length || sequences->maximum_length > (1u << 30))
+        return fail(MI355Q_ERR_SHAPE, "maximum length %u: 1 to 2^30", sequences->maximum_length);
+    if (rows && (!sequences->row_count || !sequences->maximum_rows || sequences->maximum_rows > sequences->row_count ||
+                 sequences->row_count > (1u << 30)))
+        return fail(MI355Q_ERR_SHAPE, "row bounds: 1 <= maximum_rows (%u) <= row_count (%u) <= 2^30", sequences->maximum_rows,
+                    sequences->row_count);
+    out->codes = (int8_t*)cache->codes_dev;
+    out->scales = cache->scales_dev;
+    out->sums = cache->weight_sums_dev;
+    out->table = sequences->block_table_dev;
+    out->lengths = sequences->lengths_dev;
+    out->starts = sequences->row_starts_dev;
+    out->kv_heads = cache->kv_head_count;
+    out->block_count = cache->block_count;
+    out->sequences = sequences->sequence_count;
+    out->table_stride = sequences->block_table_stride;
+    out->row_count = sequences->row_count;
+    out->max_rows = sequences->maximum_rows;
+    out->max_length = sequences->maximum_length;
+    return MI355Q_OK;
+}
+
+namespace {
+
+// Rows of the append and read entry points: strides, alignment; `vec`: whole 16-byte accesses.
+mi355q_status check_rows(const KvBlockArgs& a, uint32_t hd, const void* k, const void* v, int dtype, uint32_t* row_stride, bool* vec) {
+    if (!k || !v) return fail(MI355Q_ERR_INVALID_ARGUMENT, "null rows");
+    if (dtype != MI355Q_F16 && dtype != MI355Q_BF16 && dtype != MI355Q_F32)
+        return fail(MI355Q_ERR_INVALID_ARGUMENT, "unknown element type %d", dtype);
+    const uint64_t width = (uint64_t)a.kv_heads * hd;
+    if (*row_stride == 0) *row_stride = (uint32_t)width;
+    if (*row_stride < width) return fail(MI355Q_ERR_SHAPE, "row stride %u is shorter than heads x head dimension = %llu", *row_stride, (unsigned long long)width);
+    const size_t size = dtype == MI355Q_F32 ? 4 : 2;
+    if ((uintptr_t)k % size || (uintptr_t)v % size) return fail(MI355Q_ERR_INVALID_ARGUMENT, "misaligned rows");
+    *vec = (uintptr_t)k % 16 == 0 && (uintptr_t)v % 16 == 0 && *row_stride * size % 16 == 0;
+    return MI355Q_OK;
+}
+
+}  // namespace
+}  // namespace mi355q
+
+using namespace mi355q;
+
+extern "C" {
+
+mi355q_status mi355q_kv_block_append(mi355q_context* ctx, void* stream, const mi355q_kv_block_cache* cache,
+                                     const mi355q_kv_sequences* sequences, const void* k_dev, const void* v_dev,
+                                     mi355q_dtype dtype, uint32_t row_stride) {
+    KvBlockArgs a;
+    bool vec;
+    if (mi355q_status st = kv_block_prepare(ctx, cache, sequences, true, &a)) return st;
+    if (mi355q_status st = check_rows(a, cache->head_dimension, k_dev, v_dev, (int)dtype, &row_stride, &vec)) return st;
+    MI355Q_HIP(hipSetDevice(ctx->device));
+    // blocks that `rows` consecutive tokens can touch: one more than they fill, if they start behind a block's first
+    const uint32_t rows = a.max_rows < a.max_length ? a.max_rows : a.max_length;
+    const dim3 grid((rows + kKvTokens - 2) / kKvTokens + 1, 2 * a.kv_heads, a.sequences);
+    return kv_with_head_dimension(cache->head_dimension, [&](auto hd) -> mi355q_status {
+        constexpr int HD = decltype(hd)::value;
+        const hipStream_t s = (hipStream_t)stream;
+        if (dtype == MI355Q_F32) kv_block_append_kernel<HD, MI355Q_F32><<<grid, 2 * HD, 0, s>>>(a, k_dev, v_dev, row_stride, vec);
+        else if (dtype == MI355Q_BF16) kv_block_append_kernel<HD, MI355Q_BF16><<<grid, 2 * HD, 0, s>>>(a, k_dev, v_dev, row_stride, vec);
+        else kv_block_append_kernel<HD, MI355Q_F16><<<grid, 2 * HD, 0, s>>>(a, k_dev, v_dev, row_stride, vec);
+        MI355Q_HIP(hipGetLastError());
+        return MI355Q_OK;
+    });
+}
+
+mi355q_status mi355q_kv_block_read(mi355q_context* ctx, void* stream, const mi355q_kv_block_cache* cache,
+                                   const mi355q_kv_sequences* sequences, void* k_dev, void* v_dev, mi355q_dtype dtype,
+                                   uint32_t row_stride) {
+    KvBlockArgs a;
+    bool vec;
+    if (mi355q_status st = kv_block_prepare(ctx, cache, sequences, true, &a)) return st;
+    if (mi355q_status st = check_rows(a, cache->head_dimension, k_dev, v_dev, (int)dtype, &row_stride, &vec)) return st;
+    MI355Q_HIP(hipSetDevice(ctx->device));
+    const dim3 grid((a.max_rows + kKvTokens - 2) / kKvTokens + 1, 2 * a.kv_heads, a.sequences);
+    return kv_with_head_dimension(cache->head_dimension, [&](auto hd) -> mi355q_status {
+        constexpr int HD = decltype(hd)::value;
+        const hipStream_t s = (hipStream_t)stream;
+        if (dtype == MI355Q_F32) kv_block_read_kernel<HD, MI355Q_F32><<<grid, 2 * HD, 0, s>>>(a, k_dev, v_dev, row_stride, vec);
+        else if (dtype == MI355Q_BF16) kv_block_read_kernel<HD, MI355Q_BF16><<<grid, 2 * HD, 0, s>>>(a, k_dev, v_dev, row_stride, vec);
+        else kv_block_read_kernel<HD, MI355Q_F16><<<grid, 2 * HD, 0, s>>>(a, k_dev, v_dev, row_stride, vec);
+        MI355Q_HIP(hipGetLastError());
+        return MI355Q_OK;
+    });
+}
+
+mi355q_status mi355q_kv_block_evict(mi355q_context* ctx, void* stream, const mi355q_kv_block_cache* cache,
+                                    const mi355q_kv_sequences* sequences, uint32_t budget, uint32_t recent, uint32_t sinks,
+                                    const int32_t* new_block_table_dev, uint32_t new_block_table_stride,
+                                    int32_t* new_lengths_dev, int32_t* positions_dev) {
+    KvBlockArgs a;
+    if (mi355q_status st = kv_block_prepare(ctx, cache, sequences, false, &a)) return st;
+    if (!a.sums) return fail(MI355Q_ERR_INVALID_ARGUMENT, "eviction needs the cache's weight sums");
+    if (!new_block_table_dev || !new_lengths_dev) return fail(MI355Q_ERR_INVALID_ARGUMENT, "null new block table or lengths");
+    if ((uintptr_t)new_block_table_dev % 4 || (uintptr_t)new_lengths_dev % 4 || (uintptr_t)positions_dev % 4)
+        return fail(MI355Q_ERR_INVALID_ARGUMENT, "misaligned new block table, lengths or positions");
+    if (!budget || budget > (1u << 30)) return fail(MI355Q_ERR_SHAPE, "budget %u: 1 to 2^30 tokens", budget);
+    if ((uint64_t)recent + sinks > budget)
+        return fail(MI355Q_ERR_SHAPE, "%u recent and %u first tokens do not fit a budget of %u", recent, sinks, budget);
+    const uint32_t blocks = (budget + kKvTokens - 1) / kKvTokens;
+    if (new_block_table_stride < blocks)
+        return fail(MI355Q_ERR_SHAPE, "a budget of %u tokens needs %u blocks a sequence, the new table has %u", budget, blocks, new_block_table_stride);
+    MI355Q_HIP(hipSetDevice(ctx->device));
+    ScratchGuard guard(ctx, (hipStream_t)stream);
+    if (guard.status) return guard.status;
+    EvictArgs e{budget, recent, sinks, new_block_table_stride, new_block_table_dev, new_lengths_dev, positions_dev};
+    if (!e.positions) {
+        if (mi355q_status st = ensure_workspace(ctx, (size_t)a.sequences * a.kv_heads * budget * 4)) return st;
+        e.positions = (int32_t*)ctx->workspace;
+    }
+    kv_block_select_kernel<<<dim3(a.kv_heads, a.sequences), kSelectThreads, 0, (hipStream_t)stream>>>(a, e);
+    MI355Q_HIP(hipGetLastError());
+    return kv_with_head_dimension(cache->head_dimension, [&](auto hd) -> mi355q_status {
+        constexpr int HD = decltype(hd)::value;
+        kv_block_gather_kernel<HD><<<dim3(blocks, a.kv_heads, a.sequences), 2 * HD, 0, (hipStream_t)stream>>>(a, e);
+        MI355Q_HIP(hipGetLastError());
+        return MI355Q_OK;
+    });
+}
+
+}  // extern "C"
