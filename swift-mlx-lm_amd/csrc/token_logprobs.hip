@@ -5,10 +5,10 @@
 // is log l - t / l.  HBM-bound: a logit is read once; about ten vector instructions each, one of them an exponential.
 //
 // Alternatives: logits are ordered by 64-bit keys (ordered value, ~index), all distinct, so equal logits need no rule of
-// their own.  A wavefront keeps a threshold that at least top_count of the logits it has seen reach; keys above it are
-// collected in LDS and cut back to the top_count largest when the room runs out and at the end.  The first threshold is
-// the top_count-th largest of the 64 lanes' maxima, so that of the first 1024 logits a few dozen are collected and of
-// later ones only those that still belong to the largest.
+// their own.  The pass itself only notes, for every lane, the largest logit of each of its steps of sixteen (one LDS
+// store).  At the end a wavefront takes the top_count-th largest of its 64 lanes' maxima as a limit that top_count logits
+// reach, and only the steps whose maximum reaches it -- some two dozen of the slice's hundreds or thousands -- are read
+// again, from the cache, and their keys collected in LDS and cut to the largest.
 #include "device_utils.h"
 
 namespace mi355q {
@@ -17,6 +17,7 @@ constexpr uint32_t kTopMost = 32;                    // alternatives a row
 constexpr uint32_t kTopRoom = 256;                   // keys a wavefront collects
 constexpr uint32_t kLogprobLane = 16;                // logits of a lane per step
 constexpr uint32_t kLogprobStep = 256 * kLogprobLane;
+constexpr uint32_t kSliceSteps = 16;                 // steps of a slice at most
 constexpr float kMasked = -INFINITY, kLargest = 3.402823466e38f;
 
 struct LogprobArgs {
@@ -42,6 +43,12 @@ __device__ __forceinline__ float key_logit(unsigned long long key) {
 }
 constexpr unsigned long long kMaskedKey = ((unsigned long long)0x007FFFFFu << 32) | 0xFFFFFFFFu;   // no -inf is above it
 
+// the bf16 number at or above x, its bits (a maximum: no NaN)
+__device__ __forceinline__ uint16_t bf16_above(float x) {
+    const uint32_t u = __float_as_uint(x), cut = u >> 16;
+    return (uint16_t)((u & 0x80000000u) || !(u & 0xFFFFu) ? cut : cut + 1u);
+}
+
 // orders a wavefront's own accesses to its part of LDS
 __device__ __forceinline__ void wave_lds_order() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -54,31 +61,57 @@ struct TopKeys {
     unsigned long long threshold;
     uint32_t count, top, lane;
 
-    // Cuts the collection back to its `top` largest keys, in order: every lane counts the keys above its own.
-    __device__ void cut() {
-        wave_lds_order();
-        unsigned long long own[kTopRoom / 64];
-        uint32_t rank[kTopRoom / 64];
+    // Cuts the collection back to its `top` largest keys, in order: every lane counts the keys above each of its own.
+    template <uint32_t N>
+    __device__ void cut_from() {
+        unsigned long long own[N];
+        uint32_t rank[N];
 #pragma unroll
-        for (uint32_t i = 0; i < kTopRoom / 64; i++) {
+        for (uint32_t i = 0; i < N; i++) {
             own[i] = i * 64 + lane < count ? room[i * 64 + lane] : 0;
             rank[i] = 0;
         }
+#pragma unroll 4
         for (uint32_t k = 0; k < count; k++) {
             const unsigned long long other = room[k];
 #pragma unroll
-            for (uint32_t i = 0; i < kTopRoom / 64; i++) rank[i] += other > own[i] ? 1u : 0u;
+            for (uint32_t i = 0; i < N; i++) rank[i] += other > own[i] ? 1u : 0u;
         }
         wave_lds_order();
 #pragma unroll
-        for (uint32_t i = 0; i < kTopRoom / 64; i++)
+        for (uint32_t i = 0; i < N; i++)
             if (i * 64 + lane < count && rank[i] < top) room[rank[i]] = own[i];
+    }
+    __device__ void cut() {
+        wave_lds_order();
+        if (count <= 64) cut_from<1>();
+        else if (count <= 128) cut_from<2>();
+        else cut_from<kTopRoom / 64>();
         wave_lds_order();
         if (count >= top) {
             count = top;
             const unsigned long long last = room[top - 1];
             threshold = last > threshold ? last : threshold;
         }
+    }
+    // A number that the lanes' values reach `top` times: the top-th largest of them, its last six bits cut off (they are
+    // the lanes' numbers meanwhile, which makes the 64 values distinct).
+    __device__ float limit_of(float value) {
+        uint32_t* const own = (uint32_t*)room;       // (no keys yet)
+        const uint32_t u = __float_as_uint(value + 0.0f);
+        const uint32_t mine = (((u & 0x80000000u) ? ~u : u | 0x80000000u) & ~63u) | (63u - lane);
+        own[lane] = mine;
+        wave_lds_order();
+        uint32_t above = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < 64; k += 4) {
+            const u32x4 o = *(const u32x4*)(own + k);
+            above += (o.x > mine ? 1u : 0u) + (o.y > mine ? 1u : 0u) + (o.z > mine ? 1u : 0u) + (o.w > mine ? 1u : 0u);
+        }
+        wave_lds_order();
+        const uint32_t found = (uint32_t)__shfl((int)mine, (int)__builtin_ctzll(__ballot(above == top - 1))) & ~63u;
+        if (found < 0x00800000u) return kMasked;     // -inf with its last bits cut off
+        return __uint_as_float((found & 0x80000000u) ? found ^ 0x80000000u : ~found);
     }
     // one key of each lane (0: none)
     __device__ void push(unsigned long long key) {
@@ -127,25 +160,31 @@ __device__ void write_row(const LogprobArgs& a, uint32_t row, const LogSum& s, c
     }
 }
 
+// Logit `at` (counted from the 16-byte boundary `lead` elements in front of the row) as fp32, -inf outside the row.
+template <int D>
+__device__ __forceinline__ float logit_at(const LogprobArgs& a, size_t row_at, uint32_t lead, uint32_t at) {
+    return at >= lead && at < a.vocabulary + lead ? load_act<D>(a.logits, row_at + (at - lead)) : kMasked;
+}
+
 // One workgroup per slice of a row; its wavefronts take steps of 1024 logits in turn.
 template <int D>
 __global__ __launch_bounds__(256) void token_logprobs_kernel(LogprobArgs a) {
     __shared__ unsigned long long room[4][kTopRoom];
-    __shared__ float maxima[4][64];
+    __shared__ uint16_t maxima[4][kSliceSteps][64];  // of each step, each lane: the bf16 number at or above it
     __shared__ LogSum sums[4];
     __shared__ uint32_t counts[4];
     constexpr uint32_t VE = D == MI355Q_F32 ? 4 : 8;             // logits of a 16-byte load
     const uint32_t row = blockIdx.x / a.slices, slice = blockIdx.x - row * a.slices;
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t lane = threadIdx.x & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t size = D == MI355Q_F32 ? 4 : 2;
     const size_t row_at = (size_t)row * a.row_stride;
     // steps start at 16-byte boundaries: `lead` elements in front of the row are skipped in its first one
     const uint32_t lead = (uint32_t)(((uintptr_t)a.logits + row_at * size) % 16) / size;
-    const uint32_t begin = slice * a.slice_length, end = min(begin + a.slice_length, a.vocabulary + lead);
-    TopKeys keys{room[wave], kMaskedKey, 0, a.top, lane};
+    const uint32_t begin = slice * a.slice_length + wave * (64 * kLogprobLane);
+    const uint32_t end = min((slice + 1) * a.slice_length, a.vocabulary + lead);
     LogSum s{kMasked, 0.0f, 0.0f};
-    bool first = true;
-    for (uint32_t at = begin + wave * (64 * kLogprobLane); at < end; at += kLogprobStep) {
+    uint32_t steps = 0;
+    for (uint32_t at = begin; at < end; at += kLogprobStep, steps++) {
         float x[kLogprobLane];
         if (at >= lead && at + 64 * kLogprobLane <= a.vocabulary + lead) {
 #pragma unroll
@@ -166,10 +205,7 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(LogprobArgs a) {
             }
         } else {
 #pragma unroll
-            for (uint32_t i = 0; i < kLogprobLane; i++) {
-                const uint32_t p = at + i / VE * (64 * VE) + lane * VE + i % VE;
-                x[i] = p >= lead && p < a.vocabulary + lead ? load_act<D>(a.logits, row_at + (p - lead)) : kMasked;
-            }
+            for (uint32_t i = 0; i < kLogprobLane; i++) x[i] = logit_at<D>(a, row_at, lead, at + i / VE * (64 * VE) + lane * VE + i % VE);
         }
         // a NaN is dropped by every maximum: by this one, by the clamp of z below (e^z = 0) and by `x > kMasked` of the keys
         float top = kMasked;
@@ -186,36 +222,46 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(LogprobArgs a) {
         for (uint32_t i = 0; i < kLogprobLane; i++) {
             const float z = fmaxf(x[i] - safe, -1e4f), e = __expf(z);
             l += e;
-            t += e * z;
+            t = fmaf(e, z, t);
         }
         const float d = fmaxf(s.m - safe, -1e4f), f = __expf(d);
         s.t = f * (s.t + d * s.l) + t;
         s.l = f * s.l + l;
         s.m = m;
-        if (a.top) {
-            if (first) {                             // the top-th largest of the lanes' maxima
-                maxima[wave][lane] = top;
-                wave_lds_order();
-                uint32_t above = 0;
-                for (uint32_t k = 0; k < 64; k++) {
-                    const float other = maxima[wave][k];
-                    above += other > top || (other == top && k < lane) ? 1u : 0u;
-                }
-                const uint64_t last = __ballot(above == a.top - 1);
-                const float limit = __shfl(top, (int)__builtin_ctzll(last));
-                const unsigned long long key = logit_key(limit, 0xFFFFFFFFu);
-                keys.threshold = key > kMaskedKey ? key : kMaskedKey;
-                first = false;
-            }
-            const float limit = key_logit(keys.threshold);
-            if (__ballot(top >= limit && top > kMasked)) {
+        if (a.top) maxima[wave][steps][lane] = bf16_above(top);
+    }
+    TopKeys keys{room[wave], kMaskedKey, 0, a.top, lane};
+    if (a.top && steps) {
+        const float limit = keys.limit_of(s.m);
+        const unsigned long long key = logit_key(limit, 0xFFFFFFFFu);
+        keys.threshold = key > kMaskedKey ? key : kMaskedKey;
+        // the steps of sixteen that reach the limit, as step * 64 + lane, over the maxima that have been looked at
+        uint16_t* const list = maxima[wave][0];
+        uint32_t listed = 0;
+        for (uint32_t i = 0; i < steps; i++) {
+            const float top = bf16_to_f32(maxima[wave][i][lane]);
+            const bool reaches = top >= limit && top > kMasked;
+            const uint64_t mask = __ballot(reaches);
+            wave_lds_order();
+            if (reaches) list[listed + (uint32_t)__popcll(mask & ((1ull << lane) - 1))] = (uint16_t)(i * 64 + lane);
+            listed += (uint32_t)__popcll(mask);
+        }
+        wave_lds_order();
+        const uint32_t e = lane & 15;
+        for (uint32_t i = 0; i < listed; i += 16) {  // four of them a key of each lane, four loads in flight
+            float x[4];
+            uint32_t at[4];
 #pragma unroll
-                for (uint32_t i = 0; i < kLogprobLane; i++)
-                    keys.push(x[i] > kMasked ? logit_key(x[i], at - lead + i / VE * (64 * VE) + lane * VE + i % VE) : 0);
+            for (uint32_t r = 0; r < 4; r++) {
+                const uint32_t which = i + r * 4 + lane / 16, entry = which < listed ? list[which] : 0u;
+                at[r] = begin + (entry >> 6) * kLogprobStep + e / VE * (64 * VE) + (entry & 63) * VE + e % VE;
+                x[r] = which < listed ? logit_at<D>(a, row_at, lead, at[r]) : kMasked;
             }
+#pragma unroll
+            for (uint32_t r = 0; r < 4; r++)
+                if (i + r * 4 < listed) keys.push(x[r] > kMasked ? logit_key(fminf(x[r], kLargest), at[r] - lead) : 0);
         }
     }
-    if (a.top) keys.cut();
     // lanes, then wavefronts
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) {
@@ -230,7 +276,8 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(LogprobArgs a) {
     if (wave) return;
     for (uint32_t w = 1; w < 4; w++) s.join(sums[w].m, sums[w].l, sums[w].t);
     if (a.top) {
-        for (uint32_t w = 1; w < 4; w++) keys.push(lane < counts[w] ? room[w][lane] : 0);
+        for (uint32_t w = 1; w < 4; w++)
+            for (uint32_t i = 0; i < counts[w]; i += 64) keys.push(i + lane < counts[w] ? room[w][i + lane] : 0);
         keys.cut();
         if (lane >= keys.count && lane < a.top) room[0][lane] = 0;
         wave_lds_order();
@@ -262,6 +309,21 @@ __global__ __launch_bounds__(64) void token_logprobs_join_kernel(LogprobArgs a) 
         TopKeys keys{room, kMaskedKey, 0, a.top, lane};
         const size_t base = (size_t)row * a.slices * a.top;
         const uint32_t all = a.slices * a.top;
+        if (all > kTopRoom) {
+            // a limit that `top` keys reach: the slices' keys are in order, so if n of their q-th keys reach it, n q do
+            const uint32_t lists = a.slices < 64 ? a.slices : 64, q = (a.top + lists - 1) / lists, n = (a.top + q - 1) / q;
+            const unsigned long long own = lane < lists ? a.part_keys[base + (size_t)lane * a.top + q - 1] : 0;
+            room[lane] = own;
+            wave_lds_order();
+            uint32_t above = 0;
+#pragma unroll 8
+            for (uint32_t k = 0; k < 64; k++) above += room[k] > own || (room[k] == own && k < lane) ? 1u : 0u;
+            const int holder = (int)__builtin_ctzll(__ballot(above == n - 1));
+            const unsigned long long limit = ((unsigned long long)(uint32_t)__shfl((int)(own >> 32), holder) << 32) |
+                                             (uint32_t)__shfl((int)(uint32_t)own, holder);
+            wave_lds_order();
+            if (limit > keys.threshold) keys.threshold = limit - 1;
+        }
         for (uint32_t i = 0; i < all; i += 64) keys.push(i + lane < all ? a.part_keys[base + i + lane] : 0);
         keys.cut();
         if (lane >= keys.count && lane < a.top) room[lane] = 0;
@@ -277,8 +339,9 @@ namespace {
 void logprob_slices(LogprobArgs* a) {
     const uint32_t span = a->vocabulary + 8, steps = (span + kLogprobStep - 1) / kLogprobStep;
     uint64_t slices = (2048 + a->rows - 1) / a->rows;
+    const uint32_t least = (steps + kSliceSteps - 1) / kSliceSteps;
+    if (slices < least) slices = least;
     if (slices > steps) slices = steps;
-    if (slices > 64) slices = 64;
     const uint32_t each = (uint32_t)((steps + slices - 1) / slices);
     a->slice_length = each * kLogprobStep;
     a->slices = (steps + each - 1) / each;
