@@ -12,6 +12,8 @@
 //  - The score tile S^T = K Q^T leaves lane (n, c) = (lane % 16, lane / 16) with tokens 4c .. 4c + 3 of each sixteen for
 //    query row n, which is the operand layout of out^T = V^T P^T given the order in which the cache stores values:
 //    weights never leave their registers.
+#include <algorithm>
+
 #include "kv_block.h"
 
 namespace mi355q {
@@ -19,6 +21,7 @@ namespace mi355q {
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
 
 struct AttentionArgs {
     KvBlockArgs kv;
@@ -26,6 +29,7 @@ struct AttentionArgs {
     void* out;
     float* lse;               // may be null
     uint32_t q_stride, out_stride, heads, group, window, q_dtype, out_dtype;
+    uint32_t q_aligned;       // rows can be read 16 bytes at a time
     float scale_log2;         // scale * log2(e)
     // partial results (parts > 1) of row slot ((sequence * kv_heads + head) * tiles + tile) * parts + part, 16 RT rows each
     uint32_t tiles, parts, part_blocks;
@@ -39,6 +43,7 @@ struct AttentionArgs {
 };
 
 constexpr float kLowest = -3.402823466e38f;
+constexpr uint32_t kMostParts = 128;                  // parts that the visible blocks of a row tile are split into
 constexpr float kRaise = 8.0f, kHeadroom = 6.0f;      // log2: how far scores may pass m, and p = 2^6 at the maximum
 
 // ---- the rows of a call ------------------------------------------------------------------------------------------------
@@ -66,6 +71,25 @@ __device__ __forceinline__ int32_t row_low(const AttentionArgs& a, int32_t posit
     return a.window && (int64_t)position >= (int64_t)a.window ? position - (int32_t)a.window + 1 : 0;
 }
 
+// Block ids and scales are the same for a whole wavefront and are not written while the kernel runs: loads from the constant
+// address space go through the scalar unit and never wait behind the vector loads in flight.
+template <typename T>
+__device__ __forceinline__ T scalar_load(const T* p) {
+    return *(const __attribute__((address_space(4))) T*)p;
+}
+__device__ __forceinline__ int32_t scalar_block_id(const KvBlockArgs& a, const int32_t* table, int32_t j) {
+    const int32_t id = scalar_load(table + j);
+    return (uint32_t)id < a.block_count ? id : -1;
+}
+// keys' and values' scale of a block
+struct BlockScales {
+    float key, value;
+};
+__device__ __forceinline__ BlockScales scalar_scales(const KvBlockArgs& a, int32_t block, uint32_t head) {
+    const float* const p = kv_scale(a, block < 0 ? 0 : block, head, 0);
+    return BlockScales{scalar_load(p), scalar_load(p + 1)};
+}
+
 // ---- operands ----------------------------------------------------------------------------------------------------------
 // Eight codes (already biased to c + 128) as f16: 0x64 in front of a byte is 1024 + byte.
 __device__ __forceinline__ half8 codes_f16(uint32_t w0, uint32_t w1) {
@@ -79,25 +103,31 @@ __device__ __forceinline__ half8 codes_f16(uint32_t w0, uint32_t w1) {
 }
 __device__ __forceinline__ u32x4 biased(u32x4 w) { return w ^ 0x80808080u; }
 
-// Elements [d0, d0 + 16) of a query row as fp32 (zeros for a row that is not there).
-__device__ __forceinline__ void load_query16(const AttentionArgs& a, bool there, size_t at, float (&x)[16]) {
-    if (!there) {
-#pragma unroll
-        for (int e = 0; e < 16; e++) x[e] = 0.0f;
-        return;
-    }
+// Sixteen elements of a query row, as they are stored (two to a word) and as fp32, zeros for a row that is not there (whose
+// address is any row's).
+struct Query16 {
+    u32x4 lo, hi;
+};
+__device__ __forceinline__ Query16 load_query16(const AttentionArgs& a, size_t at) {
     const uint16_t* const p = (const uint16_t*)a.q + at;
-    uint32_t w[8];
-    if (((uintptr_t)p & 15) == 0) {
-        const u32x4 lo = *(const u32x4*)p, hi = *(const u32x4*)(p + 8);
-        w[0] = lo.x; w[1] = lo.y; w[2] = lo.z; w[3] = lo.w; w[4] = hi.x; w[5] = hi.y; w[6] = hi.z; w[7] = hi.w;
+    Query16 w;
+    if (a.q_aligned) {
+        w.lo = *(const u32x4*)p;
+        w.hi = *(const u32x4*)(p + 8);
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; e++) w[e] = (uint32_t)p[2 * e] | ((uint32_t)p[2 * e + 1] << 16);
+        for (int e = 0; e < 4; e++) {
+            w.lo[e] = (uint32_t)p[2 * e] | ((uint32_t)p[2 * e + 1] << 16);
+            w.hi[e] = (uint32_t)p[2 * e + 8] | ((uint32_t)p[2 * e + 9] << 16);
+        }
     }
+    return w;
+}
+__device__ __forceinline__ void widen_query16(const AttentionArgs& a, bool there, const Query16& w, float (&x)[16]) {
 #pragma unroll
     for (int e = 0; e < 16; e++) {
-        const uint16_t h = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+        const uint32_t word = there ? (e < 8 ? w.lo[e >> 1] : w.hi[(e >> 1) - 4]) : 0u;
+        const uint16_t h = (uint16_t)(word >> (16 * (e & 1)));
         x[e] = a.q_dtype == MI355Q_BF16 ? bf16_to_f32(h) : f16_to_f32(h);
     }
 }
@@ -148,36 +178,68 @@ __device__ __forceinline__ void store_row4(const AttentionArgs& a, size_t at, co
 // A workgroup takes one KV head, 16 RT rows and one part of the visible blocks; its four wavefronts take blocks in turn,
 // each with accumulators of its own, which are added at the end.  HBM-bound.
 template <int HD, int RT>
-__global__ __launch_bounds__(256, 2) void kv_block_attention_rows_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void kv_block_attention_rows_kernel(AttentionArgs a) {
     constexpr int S = HD / 64, DT = HD / 16;
     __shared__ __align__(16) float lds_out[2][16 * RT * HD];
     __shared__ float2 lds_ml[4][16 * RT];
     const uint32_t lane = threadIdx.x & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t n = lane & 15, c = lane >> 4;
-    const uint32_t head = blockIdx.x % a.kv.kv_heads, part = blockIdx.x / a.kv.kv_heads, tile = blockIdx.y, b = blockIdx.z;
+    const uint32_t head = blockIdx.x % a.kv.kv_heads, part = blockIdx.x / a.kv.kv_heads, b = blockIdx.z;
     const KvSequence s = kv_sequence(a.kv, b);
-    const uint32_t rows = (uint32_t)s.rows * a.group, r0 = tile * 16 * RT;
-    if (r0 >= rows) return;
-    const uint32_t r1 = min(r0 + 16 * RT, rows);
-    const RowRange g = row_range(a, s, r0, r1);
+    const uint32_t rows = (uint32_t)s.rows * a.group;      // at most 16 RT
+    if (!rows) return;
+    const RowRange g = row_range(a, s, 0, rows);
     const uint32_t parts = part_count(a, g);
     if (part >= parts) return;
 
+    // the rows are asked for first, then the first block, so that both are under way while the rows are converted
+    Query16 raw[RT][S];
+    int32_t position[RT], low[RT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        const uint32_t r = t * 16 + n < rows ? t * 16 + n : 0, token = r / a.group, h = head * a.group + r % a.group;
+        position[t] = s.first() + (int32_t)token;
+        low[t] = row_low(a, position[t]);
+#pragma unroll
+        for (int i = 0; i < S; i++) raw[t][i] = load_query16(a, (size_t)(s.row0 + (int32_t)token) * a.q_stride + (size_t)h * HD + i * 64 + c * 16);
+    }
+
+    // The loop is a pipeline of its own: a block's keys are loaded while the values of the one before are multiplied, its
+    // values while its keys are, into the registers that were just read.
+    const int32_t end = min(g.first + (int32_t)((part + 1) * a.part_blocks), g.last);
+    u32x4 kw[4][S], vw[DT];
+    auto address = [&](int32_t id) { return kv_codes<HD>(a.kv, id < 0 ? 0 : id, head, 0); };      // (an absent block loads block 0 and is masked)
+    auto load_keys = [&](int32_t id) {
+        const u32x4* const p = (const u32x4*)address(id) + lane;
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int i = 0; i < S; i++) kw[k][i] = __builtin_nontemporal_load(p + (k * S + i) * 64);
+    };
+    auto load_values = [&](int32_t id) {
+        const u32x4* const p = (const u32x4*)(address(id) + kKvTokens * HD) + lane;
+#pragma unroll
+        for (int d = 0; d < DT; d++) vw[d] = __builtin_nontemporal_load(p + d * 64);
+    };
+    int32_t j = g.first + (int32_t)(part * a.part_blocks + wave);
+    int32_t block = -1, next = -1;
+    BlockScales scales{0.0f, 0.0f};
+    if (j < end) {
+        block = scalar_block_id(a.kv, s.table, j);
+        load_keys(block);
+        load_values(block);
+        scales = scalar_scales(a.kv, block, head);
+        if (j + 4 < end) next = scalar_block_id(a.kv, s.table, j + 4);
+    }
     half8 q[RT][S][2];
     float factor[RT], m[RT], l[RT];
-    int32_t position[RT], low[RT];
     floatx4 o[RT][DT];
 #pragma unroll
     for (int t = 0; t < RT; t++) {
-        const uint32_t r = r0 + t * 16 + n;
-        const bool there = r < r1;
-        const uint32_t token = r / a.group, h = head * a.group + r % a.group;
-        position[t] = s.first() + (int32_t)token;
-        low[t] = row_low(a, position[t]);
         float x[S][16], top = 0.0f;
 #pragma unroll
         for (int i = 0; i < S; i++) {
-            load_query16(a, there, (size_t)(s.row0 + (int32_t)token) * a.q_stride + (size_t)h * HD + i * 64 + c * 16, x[i]);
+            widen_query16(a, t * 16 + n < rows, raw[t][i], x[i]);
 #pragma unroll
             for (int e = 0; e < 16; e++) top = fmaxf(top, fabsf(x[i][e]));
         }
@@ -193,34 +255,10 @@ __global__ __launch_bounds__(256, 2) void kv_block_attention_rows_kernel(Attenti
 #pragma unroll
         for (int d = 0; d < DT; d++) o[t][d] = floatx4{0, 0, 0, 0};
     }
-
-    const int32_t end = min(g.first + (int32_t)((part + 1) * a.part_blocks), g.last);
-    for (int32_t j = g.first + (int32_t)(part * a.part_blocks + wave); j < end; j += 4) {
-        const int32_t block = kv_block_id(a.kv, s.table, j);
-        const int32_t base = j * (int32_t)kKvTokens;
-        if (block < 0) {
-            if (a.scores) {
-#pragma unroll
-                for (int t = 0; t < RT; t++)
-                    if (r0 + t * 16 + n < r1)
-#pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            *(floatx4*)(a.scores + ((size_t)(b * a.kv.kv_heads + head) * a.score_rows + r0 + t * 16 + n) * a.score_stride +
-                                        base + k * 16 + c * 4) = floatx4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            }
-            continue;
-        }
-        const u32x4* const kp = (const u32x4*)kv_codes<HD>(a.kv, block, head, 0) + lane;
-        const u32x4* const vp = (const u32x4*)kv_codes<HD>(a.kv, block, head, 1) + lane;
-        u32x4 kw[4][S], vw[DT];
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-#pragma unroll
-            for (int i = 0; i < S; i++) kw[k][i] = kp[(k * S + i) * 64];
-#pragma unroll
-        for (int d = 0; d < DT; d++) vw[d] = vp[d * 64];
-        const float ks = *kv_scale(a.kv, block, head, 0), vs = *kv_scale(a.kv, block, head, 1);
-        const float vlog = vs > 0.0f ? log2f(vs) : 0.0f, vinv = vs > 0.0f ? exp2f(-vlog) : 1.0f;
+    for (; j < end; j += 4) {
+        const int32_t base = j * (int32_t)kKvTokens, id = block;
+        const bool more = j + 4 < end;
+        const float ks = scales.key, vlog = scales.value > 0.0f ? log2f(scales.value) : 0.0f;
         floatx4 x[RT][4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
@@ -237,27 +275,34 @@ __global__ __launch_bounds__(256, 2) void kv_block_attention_rows_kernel(Attenti
                 }
             }
         }
+        if (more) {
+            block = next;
+            load_keys(block);
+            scales = scalar_scales(a.kv, block, head);
+            if (j + 8 < end) next = scalar_block_id(a.kv, s.table, j + 8);
+        }
         // every row sees the whole block?
-        const bool whole = base + 63 <= g.low && (!a.window || base >= row_low(a, g.high));
+        const bool whole = id >= 0 && base + 63 <= g.low && (!a.window || base >= row_low(a, g.high));
         half8 p[RT][2];
 #pragma unroll
         for (int t = 0; t < RT; t++) {
             const float f = factor[t] * ks;
             float top = kLowest;
 #pragma unroll
+            for (int k = 0; k < 4; k++) x[t][k] *= f;
+            if (!whole) {
+                const int32_t first = low[t] - base - (int32_t)c * 4, last = id >= 0 ? position[t] - base - (int32_t)c * 4 : -1000000;
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[t][k][i] = k * 16 + i >= first && k * 16 + i <= last ? x[t][k][i] : -INFINITY;
+            }
+#pragma unroll
             for (int k = 0; k < 4; k++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    float v = x[t][k][i] * f;
-                    if (!whole) {
-                        const int32_t at = base + k * 16 + (int32_t)c * 4 + i;
-                        v = at >= low[t] && at <= position[t] ? v : -INFINITY;
-                    }
-                    x[t][k][i] = v;
-                    top = fmaxf(top, v);
-                }
-            if (a.scores && r0 + t * 16 + n < r1) {
-                float* const at = a.scores + ((size_t)(b * a.kv.kv_heads + head) * a.score_rows + r0 + t * 16 + n) * a.score_stride + base + c * 4;
+                for (int i = 0; i < 4; i++) top = fmaxf(top, x[t][k][i]);
+            if (a.scores && t * 16 + n < rows) {
+                float* const at = a.scores + ((size_t)(b * a.kv.kv_heads + head) * a.score_rows + t * 16 + n) * a.score_stride + base + c * 4;
 #pragma unroll
                 for (int k = 0; k < 4; k++) *(floatx4*)(at + k * 16) = x[t][k];
             }
@@ -270,7 +315,7 @@ __global__ __launch_bounds__(256, 2) void kv_block_attention_rows_kernel(Attenti
                 for (int d = 0; d < DT; d++) o[t][d] *= shrink;
                 m[t] = raised;
             }
-            const float shift = vlog - m[t];
+            const float shift = vlog - m[t], vinv = exp2f(-vlog);
             float sum = 0.0f;
 #pragma unroll
             for (int k = 0; k < 4; k++)
@@ -292,6 +337,7 @@ __global__ __launch_bounds__(256, 2) void kv_block_attention_rows_kernel(Attenti
                 o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, p[t][1], o[t][d], 0, 0, 0);
             }
         }
+        if (more) load_values(block);
     }
 
     // the four wavefronts' results: to a common maximum, then added pairwise through LDS in a fixed order
@@ -335,10 +381,10 @@ __global__ __launch_bounds__(256, 2) void kv_block_attention_rows_kernel(Attenti
     if (wave) return;
 #pragma unroll
     for (int t = 0; t < RT; t++) {
-        const uint32_t r = r0 + t * 16 + n;
-        if (r >= r1) continue;
+        const uint32_t r = t * 16 + n;
+        if (r >= rows) continue;
         if (parts > 1) {
-            const size_t slot = ((((size_t)b * a.kv.kv_heads + head) * a.tiles + tile) * a.parts + part) * (16 * RT) + t * 16 + n;
+            const size_t slot = (((size_t)b * a.kv.kv_heads + head) * a.parts + part) * (16 * RT) + t * 16 + n;
 #pragma unroll
             for (int d = 0; d < DT; d++) *(floatx4*)(a.part_out + slot * HD + d * 16 + c * 4) = o[t][d];
             if (c == 0) a.part_ml[slot] = make_float2(m[t], l[t]);
@@ -357,11 +403,332 @@ __global__ __launch_bounds__(256, 2) void kv_block_attention_rows_kernel(Attenti
     }
 }
 
-// Joins the parts of a row: one wavefront per row.
+// ---- many rows: prompts and prompt chunks ------------------------------------------------------------------------------
+// A workgroup takes 32 WAVES rows of one KV head, 32 a wavefront, and walks the visible blocks (or one part of them).  A
+// block's codes are read once per workgroup, 16 bytes a lane, become f16 on the way into LDS, and lie there as the
+// fragments of 32 x 32 x 16 products, so that an operand is one conflict-free 16-byte read a lane: the loads of block
+// j + 2 and the conversion of block j + 1 overlap the products of block j.
+template <int HD, int WAVES>
+struct TileLds {
+    u32x4 key[2 * (HD / 16) * 64];      // fragment (32-token half, sixteen dimensions)
+    u32x4 value[(HD / 32) * 4 * 64];    // fragment (32 dimensions, sixteen tokens)
+};
+
+template <int HD, int WAVES>
+struct TileLoader {
+    static constexpr int PIECES = 4 * HD / (64 * WAVES);      // 16-byte pieces of a thread, keys and values each
+    u32x4 key[PIECES], value[PIECES];
+    __device__ __forceinline__ void load(const AttentionArgs& a, int32_t block, uint32_t head, uint32_t tid) {
+        const u32x4* const kp = (const u32x4*)kv_codes<HD>(a.kv, block, head, 0) + tid;
+        const u32x4* const vp = (const u32x4*)kv_codes<HD>(a.kv, block, head, 1) + tid;
+#pragma unroll
+        for (int i = 0; i < PIECES; i++) key[i] = kp[i * 64 * WAVES];
+#pragma unroll
+        for (int i = 0; i < PIECES; i++) value[i] = vp[i * 64 * WAVES];
+    }
+    __device__ __forceinline__ void store(TileLds<HD, WAVES>& lds, uint32_t tid) const {
+        constexpr uint32_t S = HD / 64;
+#pragma unroll
+        for (int i = 0; i < PIECES; i++) {
+            const uint32_t p = i * 64 * WAVES + tid, t = p & 15, kq = (p >> 4) & 3, seg = (p >> 6) % S, tile = (p >> 6) / S;
+            const uint32_t fragment = (tile >> 1) * (HD / 16) + seg * 4 + (kq >> 1) * 2, slot = (kq & 1) * 32 + (tile & 1) * 16 + t;
+            const u32x4 w = biased(key[i]);
+            lds.key[fragment * 64 + slot] = __builtin_bit_cast(u32x4, codes_f16(w.x, w.y));
+            lds.key[(fragment + 1) * 64 + slot] = __builtin_bit_cast(u32x4, codes_f16(w.z, w.w));
+        }
+#pragma unroll
+        for (int i = 0; i < PIECES; i++) {
+            const uint32_t p = i * 64 * WAVES + tid, d = p & 15, kq = (p >> 4) & 3, tile = p >> 6;
+            const uint32_t fragment = (tile >> 1) * 4 + (kq >> 1), slot = (kq & 1) * 32 + (tile & 1) * 16 + d;
+            const u32x4 w = biased(value[i]);
+            lds.value[fragment * 64 + slot] = __builtin_bit_cast(u32x4, codes_f16(w.x, w.y));
+            lds.value[(fragment + 2) * 64 + slot] = __builtin_bit_cast(u32x4, codes_f16(w.z, w.w));
+        }
+    }
+};
+
+// Query row r as the operand of 32 x 32 x 16 products: lane (n, h) = (lane % 32, lane / 32) holds dimensions
+// 64 i + 32 k + 16 h .. + 16 of row n.  Returns the factor that takes sums of products with codes to log2 units (without
+// the keys' scale).
 template <int HD>
-__global__ __launch_bounds__(64) void kv_block_attention_join_kernel(AttentionArgs a, uint32_t tile_rows) {
-    constexpr int E = HD / 64;
-    const uint32_t lane = threadIdx.x, head = blockIdx.y, b = blockIdx.z, r = blockIdx.x;
+__device__ __forceinline__ float load_query_tile(const AttentionArgs& a, bool there, size_t at, uint32_t h, half8 (&q)[HD / 64][2][2]) {
+    Query16 raw[HD / 32];
+    float x[HD / 32][16], top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < HD / 32; i++) raw[i] = load_query16(a, at + i * 32 + h * 16);
+#pragma unroll
+    for (int i = 0; i < HD / 32; i++) {
+        widen_query16(a, there, raw[i], x[i]);
+#pragma unroll
+        for (int e = 0; e < 16; e++) top = fmaxf(top, fabsf(x[i][e]));
+    }
+    float up, down;
+    row_power(fmaxf(top, lane_xor<32>(top)), up, down);
+#pragma unroll
+    for (int i = 0; i < HD / 32; i++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) q[i >> 1][i & 1][e >> 3][e & 7] = (_Float16)(x[i][e] * up);
+    return a.scale_log2 * down;
+}
+
+template <int HD, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, HD == 256 ? 1 : 2) void kv_block_attention_tiles_kernel(AttentionArgs a) {
+    constexpr int S = HD / 64, DT = HD / 32;
+    constexpr uint32_t ROWS = 32 * WAVES;
+    extern __shared__ __align__(16) uint8_t lds_raw[];
+    TileLds<HD, WAVES>* const lds = (TileLds<HD, WAVES>*)lds_raw;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+    const uint32_t n = lane & 31, h = lane >> 5;
+    // the last rows of a prompt see most: they start first
+    const uint32_t head = blockIdx.x % a.kv.kv_heads, part = blockIdx.x / a.kv.kv_heads, tile = gridDim.y - 1 - blockIdx.y, b = blockIdx.z;
+    const KvSequence s = kv_sequence(a.kv, b);
+    const uint32_t rows = (uint32_t)s.rows * a.group, r0 = tile * ROWS;
+    if (r0 >= rows) return;
+    const uint32_t r1 = min(r0 + ROWS, rows);
+    const RowRange g = row_range(a, s, r0, r1);
+    const uint32_t parts = part_count(a, g);
+    if (part >= parts) return;
+    const int32_t begin = g.first + (int32_t)(part * a.part_blocks), end = min(begin + (int32_t)a.part_blocks, g.last);
+
+    const uint32_t w0 = r0 + wave * 32, r = w0 + n, token = r / a.group, out_head = head * a.group + r % a.group;
+    const bool working = w0 < r1;                          // a wavefront without rows only moves blocks
+    const int32_t position = s.first() + (int32_t)token, low = row_low(a, position);
+    const RowRange own = row_range(a, s, w0, working ? min(w0 + 32, r1) : w0 + 1);
+    half8 q[S][2][2];
+    const float factor = load_query_tile<HD>(a, r < r1, r < r1 ? (size_t)(s.row0 + (int32_t)token) * a.q_stride + (size_t)out_head * HD : 0, h, q);
+    float m = kLowest, l = 0.0f;
+    floatx16 o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+
+    TileLoader<HD, WAVES> raw;
+    BlockScales scales[2] = {};
+    int32_t id[2] = {-1, -1};
+    auto fetch = [&](int32_t j, int slot) {                // (a block that is absent loads block 0 and is masked)
+        id[slot] = scalar_block_id(a.kv, s.table, j);
+        raw.load(a, id[slot] < 0 ? 0 : id[slot], head, tid);
+        scales[slot] = scalar_scales(a.kv, id[slot], head);
+    };
+    if (begin < end) {
+        fetch(begin, 0);
+        raw.store(lds[0], tid);
+        if (begin + 1 < end) fetch(begin + 1, 1);
+    }
+    __syncthreads();
+    auto step = [&](int32_t j, auto slot_) {
+        constexpr int slot = decltype(slot_)::value;
+        const TileLds<HD, WAVES>& cur = lds[slot];
+        const BlockScales now = scales[slot];
+        const int32_t id_now = id[slot];
+        const int32_t base = j * (int32_t)kKvTokens;
+        const bool visible = working && id_now >= 0 && j >= own.first && j < own.last;
+        floatx16 x[2];
+        if (visible) {
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) x[t][i] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < HD / 16; k++)
+                    x[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, cur.key[(t * (HD / 16) + k) * 64 + lane]),
+                                                                  q[k >> 2][(k >> 1) & 1][k & 1], x[t], 0, 0, 0);
+            }
+        }
+        if (j + 1 < end) raw.store(lds[slot ^ 1], tid);
+        if (j + 2 < end) fetch(j + 2, slot);
+        if (visible) {
+            const float f = fmaxf(factor * now.key, 1e-37f);      // (a masked score times it stays -inf)
+            const float vlog = now.value > 0.0f ? log2f(now.value) : 0.0f, vinv = exp2f(-vlog);
+            if (!(base + 63 <= own.low && (!a.window || base >= row_low(a, own.high)))) {
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const int32_t at = base + t * 32 + (i >> 2) * 8 + (int32_t)h * 4 + (i & 3);
+                        x[t][i] = at >= low && at <= position ? x[t][i] : -INFINITY;
+                    }
+            }
+            float top = fmaxf(x[0][0], x[1][0]);
+#pragma unroll
+            for (int i = 1; i < 16; i++) top = fmaxf(top, fmaxf(x[0][i], x[1][i]));
+            top = top * f + (vlog - kHeadroom);
+            if (__ballot(top > m + kRaise)) {
+                const float raised = fmaxf(m, fmaxf(top, lane_xor<32>(top)));
+                const float shrink = exp2f(m - raised);
+                l *= shrink;
+#pragma unroll
+                for (int d = 0; d < DT; d++) o[d] *= shrink;
+                m = raised;
+            }
+            const float shift = vlog - m;
+            float sum = 0.0f;
+            half8 p[2][2];
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float w = __builtin_amdgcn_exp2f(fmaf(x[t][i], f, shift));
+                    sum += w;
+                    p[t][(i >> 2) & 1][(i >> 3) * 4 + (i & 3)] = (_Float16)w;
+                }
+            l += sum * vinv;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, cur.value[(d * 4 + k) * 64 + lane]),
+                                                                  p[k >> 1][k & 1], o[d], 0, 0, 0);
+        }
+        __syncthreads();
+    };
+    for (int32_t j = begin; j < end; j += 2) {
+        step(j, std::integral_constant<int, 0>{});
+        if (j + 1 < end) step(j + 1, std::integral_constant<int, 1>{});
+    }
+
+    l += lane_xor<32>(l);
+    if (r >= r1) return;
+    if (parts > 1) {
+        const size_t slot = ((((size_t)b * a.kv.kv_heads + head) * a.tiles + tile) * a.parts + part) * ROWS + (r - r0);
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                *(floatx4*)(a.part_out + slot * HD + d * 32 + i * 8 + h * 4) = floatx4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+        if (h == 0) a.part_ml[slot] = make_float2(m, l);
+        return;
+    }
+    const size_t row = (size_t)(s.row0 + (int32_t)token);
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            store_row4(a, row * a.out_stride + (size_t)out_head * HD + d * 32 + i * 8 + h * 4,
+                       floatx4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]}, f);
+    if (h == 0) {
+        const float lse2 = l == 0.0f ? -INFINITY : m + log2f(l);
+        if (a.lse) a.lse[row * a.heads + out_head] = lse2 * 0.6931471805599453f;
+        if (a.lse2) a.lse2[((size_t)b * a.kv.kv_heads + head) * a.score_rows + r] = lse2;
+    }
+}
+
+// Weight sums of many rows: the scores are computed again, tokens against all rows that see them.  A wavefront holds the
+// keys of 32 tokens as operands and adds up 2^(x - lse2) over the rows, which pass through LDS 32 at a time; the sums of
+// its lanes, which hold different rows, are added at the end, so every sum is made in one fixed order.
+template <int HD>
+__global__ __launch_bounds__(256, 2) void kv_block_weights_tiles_kernel(AttentionArgs a) {
+    constexpr int S = HD / 64;
+    __shared__ u32x4 lds_q[2][(HD / 16) * 64];
+    __shared__ float lds_factor[2][32], lds_lse[2][32];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+    const uint32_t n = lane & 31, h = lane >> 5;
+    const uint32_t head = blockIdx.x % a.kv.kv_heads, chunk = blockIdx.x / a.kv.kv_heads, b = blockIdx.z;
+    const KvSequence s = kv_sequence(a.kv, b);
+    const int32_t start = (int32_t)chunk * 128, base = start + (int32_t)wave * 32;      // the workgroup's first token, the wavefront's
+    if (start >= s.length || s.rows <= 0) return;
+    const uint32_t rows = (uint32_t)s.rows * a.group;
+    // rows that see any of the workgroup's tokens: positions start .. start + 127 + window - 1
+    const uint32_t r_first = (uint32_t)max(start - s.first(), 0) * a.group;
+    const int64_t behind = a.window ? (int64_t)start + 127 + a.window - s.first() : (int64_t)s.rows;      // the first token past them
+    const uint32_t r_last = (uint32_t)max((int64_t)0, min((int64_t)s.rows, behind)) * a.group;
+    const int32_t id = base < s.length ? kv_block_id(a.kv, s.table, base / (int32_t)kKvTokens) : -1;
+    const int32_t block = id < 0 ? 0 : id;
+    const uint32_t half = (uint32_t)(base / 32) & 1;
+    half8 k[HD / 16];
+    {
+        const u32x4* const kp = (const u32x4*)kv_codes<HD>(a.kv, block, head, 0);
+#pragma unroll
+        for (int i = 0; i < S; i++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                const u32x4 w = biased(kp[((half * 2 + (n >> 4)) * S + i) * 64 + (c * 2 + h) * 16 + (n & 15)]);
+                k[i * 4 + c * 2] = codes_f16(w.x, w.y);
+                k[i * 4 + c * 2 + 1] = codes_f16(w.z, w.w);
+            }
+    }
+    const float ks = *kv_scale(a.kv, block, head, 0);
+    float sum[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) sum[i] = 0.0f;
+    // a thread stages 16 dimensions of a row at a time: HD / 16 threads a row
+    constexpr uint32_t PER_ROW = HD / 16, AT_ONCE = 256 / PER_ROW;
+    auto stage = [&](uint32_t first, int slot) {
+#pragma unroll
+        for (uint32_t pass = 0; pass < 32 / (AT_ONCE < 32 ? AT_ONCE : 32); pass++) {
+            const uint32_t row = pass * AT_ONCE + tid / PER_ROW, piece = tid % PER_ROW;
+            if (row >= 32) continue;
+            const uint32_t r = first + row, token = r / a.group, q_head = head * a.group + r % a.group;
+            const bool there = r < rows;
+            float x[16], top = 0.0f;
+            widen_query16(a, there, load_query16(a, (there ? (size_t)(s.row0 + (int32_t)token) * a.q_stride + (size_t)q_head * HD : 0) + piece * 16), x);
+#pragma unroll
+            for (int e = 0; e < 16; e++) top = fmaxf(top, fabsf(x[e]));
+#pragma unroll
+            for (uint32_t o = 1; o < PER_ROW; o *= 2) top = fmaxf(top, __shfl_xor(top, (int)o));
+            float up, down;
+            row_power(top, up, down);
+            half8 v[2];
+#pragma unroll
+            for (int e = 0; e < 16; e++) v[e >> 3][e & 7] = (_Float16)(x[e] * up);
+            // dimensions 64 i + 16 (2 c + h) .. : fragments 4 i + 2 c and the next, slot 32 h + row
+            const uint32_t fragment = (piece >> 2) * 4 + ((piece >> 1) & 1) * 2, place = (piece & 1) * 32 + row;
+            lds_q[slot][fragment * 64 + place] = __builtin_bit_cast(u32x4, v[0]);
+            lds_q[slot][(fragment + 1) * 64 + place] = __builtin_bit_cast(u32x4, v[1]);
+            if (piece == 0) {
+                lds_factor[slot][row] = a.scale_log2 * down;
+                // a row that is not there, or saw nothing, gives weights of 2^-inf
+                const float lse2 = there ? a.lse2[((size_t)b * a.kv.kv_heads + head) * a.score_rows + r] : INFINITY;
+                lds_lse[slot][row] = lse2 == -INFINITY ? INFINITY : lse2;
+            }
+        }
+    };
+    int slot = 0;
+    if (r_first < r_last) stage(r_first, 0);
+    __syncthreads();
+    for (uint32_t first = r_first; first < r_last; first += 32, slot ^= 1) {
+        if (first + 32 < r_last) stage(first + 32, slot ^ 1);
+        const int32_t position = s.first() + (int32_t)((first + n) / a.group), low = row_low(a, position);
+        const int32_t p_low = s.first() + (int32_t)(first / a.group), p_high = s.first() + (int32_t)((first + 31) / a.group);
+        if (id >= 0 && p_high >= base && base + 31 >= row_low(a, p_low)) {
+            floatx16 x;
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[i] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < HD / 16; i++)
+                x = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i], __builtin_bit_cast(half8, lds_q[slot][i * 64 + lane]), x, 0, 0, 0);
+            const float f = fmaxf(lds_factor[slot][n] * ks, 1e-37f), lse2 = lds_lse[slot][n];
+            if (!(base + 31 <= p_low && base >= row_low(a, p_high))) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int32_t at = base + (i >> 2) * 8 + (int32_t)h * 4 + (i & 3);
+                    x[i] = at >= low && at <= position ? x[i] : -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i++) sum[i] += __builtin_amdgcn_exp2f(fmaf(x[i], f, -lse2));
+        }
+        __syncthreads();
+    }
+    if (id < 0) return;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        float v = sum[i];
+        v += lane_xor<1>(v); v += lane_xor<2>(v); v += lane_xor<4>(v); v += lane_xor<8>(v); v += lane_xor<16>(v);
+        const int32_t at = base + (i >> 2) * 8 + (int32_t)h * 4 + (i & 3);
+        if (n == 0 && at < s.length) kv_sums(a.kv, block, head)[at % (int32_t)kKvTokens] += v;
+    }
+}
+
+// Joins the parts of a row: one workgroup per row, 1024 / HD parts at a time, added in a fixed order.
+template <int HD>
+__global__ __launch_bounds__(256) void kv_block_attention_join_kernel(AttentionArgs a, uint32_t tile_rows) {
+    constexpr uint32_t LANES = HD / 4, AT_ONCE = 256 / LANES;     // a thread holds four dimensions of every AT_ONCE-th part
+    __shared__ floatx4 lds_out[256];
+    __shared__ float lds_f[kMostParts];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, head = blockIdx.y, b = blockIdx.z, r = blockIdx.x;
     const KvSequence s = kv_sequence(a.kv, b);
     const uint32_t rows = (uint32_t)s.rows * a.group;
     if (r >= rows) return;
@@ -369,52 +736,72 @@ __global__ __launch_bounds__(64) void kv_block_attention_join_kernel(AttentionAr
     const uint32_t parts = part_count(a, row_range(a, s, r0, min(r0 + tile_rows, rows)));
     if (parts == 1) return;
     const size_t slot = (((size_t)b * a.kv.kv_heads + head) * a.tiles + tile) * a.parts * tile_rows + (r - r0);
+    // every wavefront: the common maximum and the sum
+    float2 ml[kMostParts / 64];
     float top = kLowest;
-    for (uint32_t p = 0; p < parts; p++) top = fmaxf(top, a.part_ml[slot + (size_t)p * tile_rows].x);
-    float l = 0.0f, o[E];
 #pragma unroll
-    for (int e = 0; e < E; e++) o[e] = 0.0f;
-    for (uint32_t p = 0; p < parts; p++) {
-        const size_t at = slot + (size_t)p * tile_rows;
-        const float2 ml = a.part_ml[at];
-        const float f = exp2f(ml.x - top);
-        l += ml.y * f;
-#pragma unroll
-        for (int e = 0; e < E; e++) o[e] += a.part_out[at * HD + e * 64 + lane] * f;
+    for (uint32_t i = 0; i < kMostParts / 64; i++) {
+        ml[i] = i * 64 + lane < parts ? a.part_ml[slot + (size_t)(i * 64 + lane) * tile_rows] : make_float2(kLowest, 0.0f);
+        top = fmaxf(top, ml[i].x);
     }
+    top = max_across(top, lane);
+    top = fmaxf(top, lane_xor<1>(top)); top = fmaxf(top, lane_xor<2>(top)); top = fmaxf(top, lane_xor<4>(top)); top = fmaxf(top, lane_xor<8>(top));
+    float l = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < kMostParts / 64; i++) {
+        const float f = exp2f(ml[i].x - top);
+        l += ml[i].y * f;
+        if (tid < 64) lds_f[i * 64 + lane] = f;
+    }
+    l = wave_reduce_sum(l);
+    __syncthreads();
+    floatx4 o = {0, 0, 0, 0};
+    const uint32_t d = tid % LANES * 4;
+#pragma unroll 4
+    for (uint32_t p = tid / LANES; p < parts; p += AT_ONCE)
+        o += *(const floatx4*)(a.part_out + (slot + (size_t)p * tile_rows) * HD + d) * lds_f[p];
+    lds_out[tid] = o;
+    __syncthreads();
+    if (tid >= LANES) return;
+#pragma unroll
+    for (uint32_t i = 1; i < AT_ONCE; i++) o += lds_out[i * LANES + tid];
     const uint32_t token = r / a.group, h = head * a.group + r % a.group;
     const size_t row = (size_t)(s.row0 + (int32_t)token);
-    const float f = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        const size_t at = row * a.out_stride + (size_t)h * HD + e * 64 + lane;
-        if (a.out_dtype == MI355Q_BF16) ((uint16_t*)a.out)[at] = f32_to_bf16_rne(o[e] * f);
-        else ((uint16_t*)a.out)[at] = f32_to_f16_rne(o[e] * f);
-    }
-    if (lane == 0) {
+    store_row4(a, row * a.out_stride + (size_t)h * HD + d, o, l == 0.0f ? 0.0f : 1.0f / l);
+    if (tid == 0) {
         const float lse2 = l == 0.0f ? -INFINITY : top + log2f(l);
         if (a.lse) a.lse[row * a.heads + h] = lse2 * 0.6931471805599453f;
-        if (a.scores) a.lse2[((size_t)b * a.kv.kv_heads + head) * a.score_rows + r] = lse2;
+        if (a.lse2) a.lse2[((size_t)b * a.kv.kv_heads + head) * a.score_rows + r] = lse2;
     }
 }
 
-// Weight sums from the stored scores: a thread per token, over the rows of its KV head that see it.
+// Weight sums from the stored scores: four tokens a thread, over the rows of its KV head.  Scores that a row does not see
+// were stored as -inf.
 __global__ __launch_bounds__(256) void kv_block_weights_kernel(AttentionArgs a) {
-    const uint32_t head = blockIdx.y, b = blockIdx.z;
+    const uint32_t head = blockIdx.x % a.kv.kv_heads, chunk = blockIdx.x / a.kv.kv_heads, b = blockIdx.z;
     const KvSequence s = kv_sequence(a.kv, b);
-    const int32_t t = (int32_t)(blockIdx.x * 256 + threadIdx.x);
-    if (t >= s.length || s.rows <= 0) return;
-    const int32_t block = kv_block_id(a.kv, s.table, t / (int32_t)kKvTokens);
-    if (block < 0) return;
     const uint32_t rows = (uint32_t)s.rows * a.group;
+    if (!rows) return;
+    const RowRange g = row_range(a, s, 0, rows);
+    const int32_t t = (int32_t)(chunk * 1024 + threadIdx.x * 4), j = t / (int32_t)kKvTokens;
+    if (j < g.first || j >= g.last) return;
+    const int32_t block = kv_block_id(a.kv, s.table, j);
     const size_t slot = ((size_t)b * a.kv.kv_heads + head) * a.score_rows;
-    float sum = 0.0f;
+    const floatx4* const scores = (const floatx4*)(a.scores + slot * a.score_stride + t);
+    floatx4 sum = {0, 0, 0, 0};
+#pragma unroll 4
     for (uint32_t r = 0; r < rows; r++) {
-        const int32_t position = s.first() + (int32_t)(r / a.group);
-        if (t > position || t < row_low(a, position)) continue;
-        sum += exp2f(a.scores[(slot + r) * a.score_stride + t] - a.lse2[slot + r]);
+        const floatx4 x = scores[(size_t)r * (a.score_stride / 4)];
+        float lse2 = scalar_load(a.lse2 + slot + r);
+        lse2 = lse2 == -INFINITY ? INFINITY : lse2;      // a row that sees nothing
+#pragma unroll
+        for (int i = 0; i < 4; i++) sum[i] += __builtin_amdgcn_exp2f(x[i] - lse2);
     }
-    kv_sums(a.kv, block, head)[t % (int32_t)kKvTokens] += sum;
+    if (block < 0) return;
+    float* const at = kv_sums(a.kv, block, head) + t % (int32_t)kKvTokens;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (t + i < s.length) at[i] += sum[i];
 }
 
 namespace {
@@ -430,21 +817,61 @@ struct Buffers {
     }
 };
 
+// Blocks that the rows of a tile can see, and the parts they are split into so that the launch has about `wanted`
+// workgroups; a part is a multiple of `unit` blocks.
+uint64_t visible_blocks(const AttentionArgs& a, uint32_t tile_rows) {
+    const uint64_t blocks = (a.kv.max_length + kKvTokens - 1) / kKvTokens;
+    if (!a.window) return blocks;
+    const uint64_t tokens = (uint64_t)a.window + tile_rows / a.group + 1;      // from the first row's first to the last row
+    return std::min(blocks, (tokens + kKvTokens - 2) / kKvTokens + 1);
+}
+void choose_parts(AttentionArgs* a, uint64_t blocks, uint64_t groups, uint32_t wanted, uint32_t unit) {
+    uint64_t parts = (wanted + groups - 1) / groups;
+    parts = std::min(parts, (blocks + unit - 1) / unit);
+    parts = std::max<uint64_t>(1, std::min<uint64_t>(parts, kMostParts));
+    a->part_blocks = (uint32_t)(((blocks + parts - 1) / parts + unit - 1) / unit * unit);
+    a->parts = (uint32_t)((blocks + a->part_blocks - 1) / a->part_blocks);
+}
+
+template <int HD, int WAVES>
+mi355q_status launch_tiles(mi355q_context* ctx, hipStream_t s, AttentionArgs a, bool weights) {
+    constexpr uint32_t ROWS = 32 * WAVES;
+    const uint32_t rows = a.kv.max_rows * a.group;
+    a.tiles = (rows + ROWS - 1) / ROWS;
+    const uint64_t groups = (uint64_t)a.kv.kv_heads * a.tiles * a.kv.sequences;
+    choose_parts(&a, visible_blocks(a, ROWS), groups, 512, 4);
+    a.score_rows = rows;
+    for (int pass = 0; pass < 2; pass++) {
+        Buffers buf{pass ? (char*)ctx->workspace : nullptr, 0};
+        if (a.parts > 1) {
+            a.part_out = buf.take<float>(groups * a.parts * ROWS * HD);
+            a.part_ml = buf.take<float2>(groups * a.parts * ROWS);
+        }
+        if (weights) a.lse2 = buf.take<float>((size_t)a.kv.sequences * a.kv.kv_heads * rows);
+        if (!pass && buf.used)
+            if (mi355q_status st = ensure_workspace(ctx, buf.used)) return st;
+    }
+    constexpr size_t lds = 2 * sizeof(TileLds<HD, WAVES>);
+    if (mi355q_status st = raise_lds_limit((const void*)kv_block_attention_tiles_kernel<HD, WAVES>, lds)) return st;
+    kv_block_attention_tiles_kernel<HD, WAVES><<<dim3(a.kv.kv_heads * a.parts, a.tiles, a.kv.sequences), 64 * WAVES, lds, s>>>(a);
+    MI355Q_HIP(hipGetLastError());
+    if (a.parts > 1) {
+        kv_block_attention_join_kernel<HD><<<dim3(rows, a.kv.kv_heads, a.kv.sequences), 256, 0, s>>>(a, ROWS);
+        MI355Q_HIP(hipGetLastError());
+    }
+    if (weights) {
+        kv_block_weights_tiles_kernel<HD><<<dim3((a.kv.max_length + 127) / 128 * a.kv.kv_heads, 1, a.kv.sequences), 256, 0, s>>>(a);
+        MI355Q_HIP(hipGetLastError());
+    }
+    return MI355Q_OK;
+}
+
 template <int HD, int RT>
 mi355q_status launch_rows(mi355q_context* ctx, hipStream_t s, AttentionArgs a, bool weights) {
     const uint32_t rows = a.kv.max_rows * a.group;
-    a.tiles = (rows + 16 * RT - 1) / (16 * RT);
-    uint64_t blocks = (a.kv.max_length + kKvTokens - 1) / kKvTokens;
-    if (a.window) {
-        const uint64_t reach = ((uint64_t)a.window + 16 * RT / a.group + 1 + kKvTokens - 2) / kKvTokens + 1;
-        if (reach < blocks) blocks = reach;
-    }
-    const uint64_t groups = (uint64_t)a.kv.kv_heads * a.tiles * a.kv.sequences;
-    uint64_t parts = (1536 + groups - 1) / groups;
-    if (parts > (blocks + 3) / 4) parts = (blocks + 3) / 4;
-    if (parts > 64) parts = 64;
-    a.part_blocks = (uint32_t)(((blocks + parts - 1) / parts + 3) / 4 * 4);
-    a.parts = (uint32_t)((blocks + a.part_blocks - 1) / a.part_blocks);
+    a.tiles = 1;
+    const uint64_t groups = (uint64_t)a.kv.kv_heads * a.kv.sequences;
+    choose_parts(&a, visible_blocks(a, 16 * RT), groups, 1024, 4);
     a.score_rows = rows;
     a.score_stride = (uint32_t)((a.kv.max_length + kKvTokens - 1) / kKvTokens * kKvTokens);
     for (int pass = 0; pass < 2; pass++) {
@@ -460,14 +887,14 @@ mi355q_status launch_rows(mi355q_context* ctx, hipStream_t s, AttentionArgs a, b
         if (!pass && buf.used)
             if (mi355q_status st = ensure_workspace(ctx, buf.used)) return st;
     }
-    kv_block_attention_rows_kernel<HD, RT><<<dim3(a.kv.kv_heads * a.parts, a.tiles, a.kv.sequences), 256, 0, s>>>(a);
+    kv_block_attention_rows_kernel<HD, RT><<<dim3(a.kv.kv_heads * a.parts, 1, a.kv.sequences), 256, 0, s>>>(a);
     MI355Q_HIP(hipGetLastError());
     if (a.parts > 1) {
-        kv_block_attention_join_kernel<HD><<<dim3(rows, a.kv.kv_heads, a.kv.sequences), 64, 0, s>>>(a, 16 * RT);
+        kv_block_attention_join_kernel<HD><<<dim3(rows, a.kv.kv_heads, a.kv.sequences), 256, 0, s>>>(a, 16 * RT);
         MI355Q_HIP(hipGetLastError());
     }
     if (weights) {
-        kv_block_weights_kernel<<<dim3((a.kv.max_length + 255) / 256, a.kv.kv_heads, a.kv.sequences), 256, 0, s>>>(a);
+        kv_block_weights_kernel<<<dim3((a.kv.max_length + 1023) / 1024 * a.kv.kv_heads, 1, a.kv.sequences), 256, 0, s>>>(a);
         MI355Q_HIP(hipGetLastError());
     }
     return MI355Q_OK;
@@ -491,6 +918,8 @@ extern "C" mi355q_status mi355q_kv_block_attention(mi355q_context* ctx, void* st
     if (!head_count || head_count % a.kv.kv_heads)
         return fail(MI355Q_ERR_SHAPE, "%u query heads do not share %u KV heads evenly", head_count, a.kv.kv_heads);
     if (head_count > 32767) return fail(MI355Q_ERR_SHAPE, "%u query heads: at most 32767", head_count);
+    if ((uint64_t)a.kv.max_rows * (head_count / a.kv.kv_heads) > (1u << 22))
+        return fail(MI355Q_ERR_SHAPE, "%u rows of %u heads share a KV head: at most 2^22 together", a.kv.max_rows, head_count / a.kv.kv_heads);
     const uint64_t width = (uint64_t)head_count * cache->head_dimension;
     if (q_row_stride == 0) q_row_stride = (uint32_t)width;
     if (out_row_stride == 0) out_row_stride = (uint32_t)width;
@@ -504,10 +933,14 @@ extern "C" mi355q_status mi355q_kv_block_attention(mi355q_context* ctx, void* st
     if (guard.status) return guard.status;
     a.q = q_dev; a.out = out_dev; a.lse = lse_dev;
     a.q_stride = q_row_stride; a.out_stride = out_row_stride;
+    a.q_aligned = (uintptr_t)q_dev % 16 == 0 && q_row_stride % 8 == 0;
     a.heads = head_count; a.group = head_count / a.kv.kv_heads; a.window = window;
     a.q_dtype = (uint32_t)q_dtype; a.out_dtype = (uint32_t)out_dtype; a.scale_log2 = scale * 1.4426950408889634f;
     return kv_with_head_dimension(cache->head_dimension, [&](auto hd) -> mi355q_status {
         constexpr int HD = decltype(hd)::value;
-        return launch_rows<HD, 1>(ctx, (hipStream_t)stream, a, accumulate_weights != 0);
+        const uint32_t rows = a.kv.max_rows * a.group;
+        if (rows <= 16) return launch_rows<HD, 1>(ctx, (hipStream_t)stream, a, accumulate_weights != 0);
+        if (HD < 256 && rows <= 32) return launch_rows<HD < 256 ? HD : 64, 2>(ctx, (hipStream_t)stream, a, accumulate_weights != 0);
+        return launch_tiles<HD, 4>(ctx, (hipStream_t)stream, a, accumulate_weights != 0);
     });
 }

@@ -338,7 +338,7 @@ namespace {
 // every CU has several.
 void logprob_slices(LogprobArgs* a) {
     const uint32_t span = a->vocabulary + 8, steps = (span + kLogprobStep - 1) / kLogprobStep;
-    uint64_t slices = (2048 + a->rows - 1) / a->rows;
+    uint64_t slices = (1024 + a->rows - 1) / a->rows;
     const uint32_t least = (steps + kSliceSteps - 1) / kSliceSteps;
     if (slices < least) slices = least;
     if (slices > steps) slices = steps;
