@@ -50,6 +50,17 @@ __device__ __forceinline__ int32_t kv_block_id(const KvBlockArgs& a, const int32
     return (uint32_t)id < a.block_count ? id : -1;
 }
 
+// Block ids and scales are the same for a whole wavefront and are not written while the kernel runs: loads from the constant
+// address space go through the scalar unit and never wait behind the vector loads in flight.
+template <typename T>
+__device__ __forceinline__ T scalar_load(const T* p) {
+    return *(const __attribute__((address_space(4))) T*)p;
+}
+__device__ __forceinline__ int32_t scalar_block_id(const KvBlockArgs& a, const int32_t* table, int32_t j) {
+    const int32_t id = scalar_load(table + j);
+    return (uint32_t)id < a.block_count ? id : -1;
+}
+
 template <int HD>
 __device__ __forceinline__ int8_t* kv_codes(const KvBlockArgs& a, int32_t block, uint32_t head, uint32_t part) {
     return a.codes + (((size_t)block * a.kv_heads + head) * 2 + part) * (kKvTokens * HD);

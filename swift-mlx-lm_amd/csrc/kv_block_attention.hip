@@ -71,16 +71,6 @@ __device__ __forceinline__ int32_t row_low(const AttentionArgs& a, int32_t posit
     return a.window && (int64_t)position >= (int64_t)a.window ? position - (int32_t)a.window + 1 : 0;
 }
 
-// Block ids and scales are the same for a whole wavefront and are not written while the kernel runs: loads from the constant
-// address space go through the scalar unit and never wait behind the vector loads in flight.
-template <typename T>
-__device__ __forceinline__ T scalar_load(const T* p) {
-    return *(const __attribute__((address_space(4))) T*)p;
-}
-__device__ __forceinline__ int32_t scalar_block_id(const KvBlockArgs& a, const int32_t* table, int32_t j) {
-    const int32_t id = scalar_load(table + j);
-    return (uint32_t)id < a.block_count ? id : -1;
-}
 // keys' and values' scale of a block
 struct BlockScales {
     float key, value;

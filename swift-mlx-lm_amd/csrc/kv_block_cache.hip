@@ -258,15 +258,48 @@ __device__ __forceinline__ uint32_t sum_key(float v) {
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-constexpr uint32_t kSelectThreads = 1024;
+constexpr uint32_t kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
+constexpr uint32_t kSelectBins = 2048;
+constexpr uint32_t kSelectKeys = 32768;              // keys that fit LDS; a longer sequence's others are read again
+constexpr uint32_t kSelectGroup = 8;                 // blocks of a wavefront in flight
 
-// One workgroup per sequence and head: the key of the last token kept is found digit by digit (four histograms of 256),
-// then the positions are written in order, ties with that key from the lowest position on.
-__global__ __launch_bounds__(kSelectThreads) void kv_block_select_kernel(KvBlockArgs a, EvictArgs e) {
-    __shared__ uint32_t bins[256];
-    __shared__ uint32_t digit, wanted;
-    __shared__ uint32_t wave_above[kSelectThreads / 64], wave_ties[kSelectThreads / 64];
-    const uint32_t head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// Exclusive sums of two counts over the workgroup's threads; `totals` is LDS for one pair a wavefront.
+__device__ __forceinline__ uint2 scan_counts(uint2 own, uint2* totals, uint32_t lane, uint32_t wave, uint2* all) {
+    uint2 sum = own;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+        const uint32_t x = (uint32_t)__shfl_up((int)sum.x, o), y = (uint32_t)__shfl_up((int)sum.y, o);
+        sum.x += lane >= (uint32_t)o ? x : 0;
+        sum.y += lane >= (uint32_t)o ? y : 0;
+    }
+    __syncthreads();
+    if (lane == 63) totals[wave] = sum;
+    __syncthreads();
+    uint2 before = make_uint2(sum.x - own.x, sum.y - own.y), every = make_uint2(0, 0);
+#pragma unroll
+    for (uint32_t w = 0; w < kSelectWaves; w++) {
+        const uint2 v = totals[w];
+        if (w < wave) { before.x += v.x; before.y += v.y; }
+        every.x += v.x;
+        every.y += v.y;
+    }
+    *all = every;
+    return before;
+}
+
+// One workgroup per sequence and head, a wavefront per block of 64 tokens at a time.  Latency-bound (a workgroup has one
+// sequence's few hundred kilobytes): the sums are read once, eight blocks of a wavefront in flight, and their keys held in
+// LDS; the key of the last token kept is found in three digits of 11, 11 and 10 bits from histograms; then every block's
+// kept tokens and ties become bit masks, whose counts give each block its place in the list.  Ties with the last key are
+// kept from the lowest position on.
+__global__ __launch_bounds__(kSelectThreads) void kv_block_select_kernel(KvBlockArgs a, EvictArgs e, uint32_t room) {
+    extern __shared__ uint32_t lds_keys[];
+    __shared__ uint32_t bins[kSelectBins];
+    __shared__ uint64_t keep_masks[kSelectThreads], tie_masks[kSelectThreads];
+    __shared__ uint2 totals[kSelectWaves];
+    __shared__ uint32_t found, left;
+    const uint32_t head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
     const uint32_t length = (uint32_t)kv_length(a, b);
     const int32_t* const table = a.table + (size_t)b * a.table_stride;
     int32_t* const out = e.positions + ((size_t)b * a.kv_heads + head) * e.budget;
@@ -275,63 +308,102 @@ __global__ __launch_bounds__(kSelectThreads) void kv_block_select_kernel(KvBlock
         for (uint32_t t = tid; t < length; t += kSelectThreads) out[t] = (int32_t)t;
         return;
     }
-    // budget >= sinks + recent and length > budget: the tokens between the two are more than those wanted of them
-    const uint32_t low = e.sinks, high = length - e.recent;
-    auto key_of = [&](uint32_t t) {
-        const int32_t block = kv_block_id(a, table, (int32_t)(t / kKvTokens));
-        return block < 0 ? sum_key(0.0f) : sum_key(kv_sums(a, block, head)[t % kKvTokens]);
+    // budget >= sinks + recent and length > budget: the tokens [low, high) between the two are more than those wanted
+    const uint32_t low = e.sinks, high = length - e.recent, blocks = (length + kKvTokens - 1) / kKvTokens;
+    uint32_t need = e.budget - e.sinks - e.recent;
+    const bool some = need > 0;
+    // f(block, key of the lane's token, whether it is one of [low, high)) for the blocks of a wavefront in [first, last)
+    auto each = [&](uint32_t first, uint32_t last, bool fresh, auto&& f) {
+        for (uint32_t j0 = first + wave; j0 < last; j0 += kSelectWaves * kSelectGroup) {
+            uint32_t key[kSelectGroup];
+#pragma unroll
+            for (uint32_t g = 0; g < kSelectGroup; g++) {
+                const uint32_t j = j0 + g * kSelectWaves, t = j * kKvTokens + lane;
+                key[g] = 0;
+                if (j >= last) continue;
+                if (!fresh && j < room / kKvTokens) {
+                    key[g] = lds_keys[t];
+                } else {
+                    const int32_t block = scalar_block_id(a, table, (int32_t)j);
+                    key[g] = __float_as_uint(block < 0 ? 0.0f : kv_sums(a, block, head)[lane]);
+                }
+            }
+#pragma unroll
+            for (uint32_t g = 0; g < kSelectGroup; g++) {
+                const uint32_t j = j0 + g * kSelectWaves, t = j * kKvTokens + lane;
+                if (j >= last) continue;
+                if (fresh || j >= room / kKvTokens) key[g] = sum_key(__uint_as_float(key[g]));
+                f(j, key[g], t >= low && t < high);
+            }
+        }
     };
-    uint32_t prefix = 0, need = e.budget - e.sinks - e.recent;     // tokens wanted among those whose key starts with prefix
-    const bool any = need > 0;
-    for (int shift = 24; any && shift >= 0; shift -= 8) {
-        if (tid < 256) bins[tid] = 0;
-        __syncthreads();
-        for (uint32_t t = low + tid; t < high; t += kSelectThreads) {
-            const uint32_t key = key_of(t);
-            if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&bins[(key >> shift) & 255u], 1u);
+    uint32_t prefix = 0;
+    if (some) {
+#pragma unroll
+        for (int digit = 0; digit < 3; digit++) {
+            constexpr uint32_t shifts[3] = {21, 10, 0}, widths[3] = {11, 11, 10};
+            const uint32_t shift = shifts[digit];
+            for (uint32_t i = tid; i < kSelectBins; i += kSelectThreads) bins[i] = 0;
+            __syncthreads();
+            each(0, blocks, digit == 0, [&](uint32_t j, uint32_t key, bool there) {
+                if (digit == 0 && j < room / kKvTokens) lds_keys[j * kKvTokens + lane] = key;
+                if (there && (digit == 0 || key >> (shift + widths[digit]) == prefix >> (shift + widths[digit])))
+                    atomicAdd(&bins[(key >> shift) & ((1u << widths[digit]) - 1)], 1u);
+            });
+            __syncthreads();
+            // counts from the highest bin down, two bins a thread: the one in which the need is met
+            const uint32_t bin = kSelectBins - 1 - 2 * tid, upper = bins[bin], pair = upper + bins[bin - 1];
+            uint2 all;
+            const uint32_t before = scan_counts(make_uint2(pair, 0), totals, lane, wave, &all).x;
+            if (before < need && need <= before + pair) {
+                const bool first = need <= before + upper;
+                found = first ? bin : bin - 1;
+                left = need - before - (first ? 0 : upper);
+            }
+            __syncthreads();
+            prefix |= found << shift;
+            need = left;
         }
-        __syncthreads();
-        if (tid == 0) {
-            uint32_t left = need, d = 255;
-            while (d > 0 && bins[d] < left) left -= bins[d--];
-            digit = d; wanted = left;
-        }
-        __syncthreads();
-        prefix |= digit << shift;
-        need = wanted;
     }
-    // `need` tokens with exactly this key, the first of them, and all with a larger one
+    // `need` tokens with exactly this key, the first of them, and all with a larger one, 1024 blocks at a time
     uint32_t written = 0, ties = 0;
-    for (uint32_t start = 0; start < length; start += kSelectThreads) {
-        const uint32_t t = start + tid;
-        bool keep = t < length && (t < low || t >= high), tie = false;
-        if (any && t >= low && t < high) {
-            const uint32_t key = key_of(t);
-            keep = key > prefix;
-            tie = key == prefix;
-        }
-        const uint64_t tie_mask = __ballot(tie);
-        if (lane == 0) wave_ties[wave] = (uint32_t)__popcll(tie_mask);
+    for (uint32_t first = 0; first < blocks; first += kSelectThreads) {
+        const uint32_t last = min(first + kSelectThreads, blocks);
         __syncthreads();
-        uint32_t before = ties, all_ties = ties;
-        for (uint32_t w = 0; w < kSelectThreads / 64; w++) {
-            if (w < wave) before += wave_ties[w];
-            all_ties += wave_ties[w];
-        }
-        keep |= tie && before + (uint32_t)__popcll(tie_mask & ((1ull << lane) - 1)) < need;
-        const uint64_t mask = __ballot(keep);
-        if (lane == 0) wave_above[wave] = (uint32_t)__popcll(mask);
+        each(first, last, false, [&](uint32_t j, uint32_t key, bool there) {
+            const uint32_t t = j * kKvTokens + lane;
+            const uint64_t keep = __ballot(there ? some && key > prefix : t < length), tie = __ballot(there && some && key == prefix);
+            if (lane == 0) { keep_masks[j - first] = keep; tie_masks[j - first] = tie; }
+        });
         __syncthreads();
-        uint32_t at = written, all = written;
-        for (uint32_t w = 0; w < kSelectThreads / 64; w++) {
-            if (w < wave) at += wave_above[w];
-            all += wave_above[w];
+        const bool mine = first + tid < last;
+        uint64_t keep = mine ? keep_masks[tid] : 0, tie = mine ? tie_masks[tid] : 0;
+        uint2 all;
+        const uint2 before = scan_counts(make_uint2((uint32_t)__popcll(keep), (uint32_t)__popcll(tie)), totals, lane, wave, &all);
+        const uint32_t ties_before = ties + before.y;
+        const uint32_t place = written + before.x + min(ties_before, need) - min(ties, need);
+        // the block's ties that are kept are its first: drop the last set bits until they fit
+        uint32_t fit = ties_before < need ? need - ties_before : 0;
+        if ((uint32_t)__popcll(tie) > fit) {
+            uint64_t chosen = 0;
+            for (; fit; fit--) {
+                chosen |= tie & -tie;
+                tie &= tie - 1;
+            }
+            tie = chosen;
         }
-        at += (uint32_t)__popcll(mask & ((1ull << lane) - 1));
-        if (keep && at < e.budget) out[at] = (int32_t)t;
-        written = all;
-        ties = all_ties;
-        __syncthreads();
+        keep |= tie;
+        // (a thread's masks pass from its lane to the whole wavefront)
+        for (uint32_t k = 0; k < 64; k++) {
+            const uint32_t j = first + wave * 64 + k;
+            if (j >= last) break;
+            const uint64_t mask = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(keep >> 32), (int)k) << 32) |
+                                  (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)keep, (int)k);
+            const uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)place, (int)k) + (uint32_t)__popcll(mask & ((1ull << lane) - 1));
+            if ((mask >> lane) & 1) out[at] = (int32_t)(j * kKvTokens + lane);
+        }
+        written += all.x + min(ties + all.y, need) - min(ties, need);
+        ties += all.y;
     }
 }
 
@@ -542,7 +614,9 @@ mi355q_status mi355q_kv_block_evict(mi355q_context* ctx, void* stream, const mi3
         if (mi355q_status st = ensure_workspace(ctx, (size_t)a.sequences * a.kv_heads * budget * 4)) return st;
         e.positions = (int32_t*)ctx->workspace;
     }
-    kv_block_select_kernel<<<dim3(a.kv_heads, a.sequences), kSelectThreads, 0, (hipStream_t)stream>>>(a, e);
+    const uint32_t tokens = (a.max_length + kKvTokens - 1) / kKvTokens * kKvTokens, room = tokens < kSelectKeys ? tokens : kSelectKeys;
+    if (mi355q_status st = raise_lds_limit((const void*)kv_block_select_kernel, (size_t)kSelectKeys * 4)) return st;
+    kv_block_select_kernel<<<dim3(a.kv_heads, a.sequences), kSelectThreads, (size_t)room * 4, (hipStream_t)stream>>>(a, e, room);
     MI355Q_HIP(hipGetLastError());
     return kv_with_head_dimension(cache->head_dimension, [&](auto hd) -> mi355q_status {
         constexpr int HD = decltype(hd)::value;
