@@ -260,7 +260,8 @@ __device__ __forceinline__ uint32_t sum_key(float v) {
 
 constexpr uint32_t kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
 constexpr uint32_t kSelectBins = 2048;
-constexpr uint32_t kSelectKeys = 32768;              // keys that fit LDS; a longer sequence's others are read again
+constexpr uint32_t kSelectKeys = 28672;              // keys that fit LDS; a longer sequence's others are read again
+constexpr uint32_t kSelectList = 4096;
 constexpr uint32_t kSelectGroup = 8;                 // blocks of a wavefront in flight
 
 // Exclusive sums of two counts over the workgroup's threads; `totals` is LDS for one pair a wavefront.
@@ -296,8 +297,9 @@ __global__ __launch_bounds__(kSelectThreads) void kv_block_select_kernel(KvBlock
     extern __shared__ uint32_t lds_keys[];
     __shared__ uint32_t bins[kSelectBins];
     __shared__ uint64_t keep_masks[kSelectThreads], tie_masks[kSelectThreads];
+    __shared__ uint32_t listed_keys[kSelectList];        // keys that begin with the first digit found
     __shared__ uint2 totals[kSelectWaves];
-    __shared__ uint32_t found, left;
+    __shared__ uint32_t found, left, listed;
     const uint32_t head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
     const uint32_t length = (uint32_t)kv_length(a, b);
@@ -312,44 +314,60 @@ __global__ __launch_bounds__(kSelectThreads) void kv_block_select_kernel(KvBlock
     const uint32_t low = e.sinks, high = length - e.recent, blocks = (length + kKvTokens - 1) / kKvTokens;
     uint32_t need = e.budget - e.sinks - e.recent;
     const bool some = need > 0;
-    // f(block, key of the lane's token, whether it is one of [low, high)) for the blocks of a wavefront in [first, last)
-    auto each = [&](uint32_t first, uint32_t last, bool fresh, auto&& f) {
+    // f(block, key of the lane's token) for a wavefront's share of blocks [first, last): from memory, eight in flight, or LDS
+    const uint32_t held = min(room / kKvTokens, blocks);
+    auto each_read = [&](uint32_t first, uint32_t last, auto&& f) {
         for (uint32_t j0 = first + wave; j0 < last; j0 += kSelectWaves * kSelectGroup) {
-            uint32_t key[kSelectGroup];
+            float v[kSelectGroup];
 #pragma unroll
             for (uint32_t g = 0; g < kSelectGroup; g++) {
-                const uint32_t j = j0 + g * kSelectWaves, t = j * kKvTokens + lane;
-                key[g] = 0;
-                if (j >= last) continue;
-                if (!fresh && j < room / kKvTokens) {
-                    key[g] = lds_keys[t];
-                } else {
-                    const int32_t block = scalar_block_id(a, table, (int32_t)j);
-                    key[g] = __float_as_uint(block < 0 ? 0.0f : kv_sums(a, block, head)[lane]);
-                }
+                const int32_t block = scalar_block_id(a, table, (int32_t)min(j0 + g * kSelectWaves, last - 1));
+                v[g] = block < 0 ? 0.0f : kv_sums(a, block, head)[lane];
             }
 #pragma unroll
-            for (uint32_t g = 0; g < kSelectGroup; g++) {
-                const uint32_t j = j0 + g * kSelectWaves, t = j * kKvTokens + lane;
-                if (j >= last) continue;
-                if (fresh || j >= room / kKvTokens) key[g] = sum_key(__uint_as_float(key[g]));
-                f(j, key[g], t >= low && t < high);
-            }
+            for (uint32_t g = 0; g < kSelectGroup; g++)
+                if (j0 + g * kSelectWaves < last) f(j0 + g * kSelectWaves, sum_key(v[g]));
         }
     };
+    auto each = [&](uint32_t first, uint32_t last, auto&& f) {
+        for (uint32_t j = first + wave; j < min(last, held); j += kSelectWaves) f(j, lds_keys[j * kKvTokens + lane]);
+        if (last > held) each_read(max(first, held), last, f);
+    };
+    auto between = [&](uint32_t j) { return j * kKvTokens + lane - low < high - low; };
     uint32_t prefix = 0;
     if (some) {
 #pragma unroll
         for (int digit = 0; digit < 3; digit++) {
-            constexpr uint32_t shifts[3] = {21, 10, 0}, widths[3] = {11, 11, 10};
-            const uint32_t shift = shifts[digit];
+            constexpr uint32_t shifts[3] = {21, 10, 0};
             for (uint32_t i = tid; i < kSelectBins; i += kSelectThreads) bins[i] = 0;
             __syncthreads();
-            each(0, blocks, digit == 0, [&](uint32_t j, uint32_t key, bool there) {
-                if (digit == 0 && j < room / kKvTokens) lds_keys[j * kKvTokens + lane] = key;
-                if (there && (digit == 0 || key >> (shift + widths[digit]) == prefix >> (shift + widths[digit])))
-                    atomicAdd(&bins[(key >> shift) & ((1u << widths[digit]) - 1)], 1u);
-            });
+            if (digit == 0) {
+                if (tid == 0) listed = 0;
+                each_read(0, blocks, [&](uint32_t j, uint32_t key) {
+                    if (j < held) lds_keys[j * kKvTokens + lane] = key;
+                    if (between(j)) atomicAdd(&bins[key >> 21], 1u);
+                });
+            } else if (digit == 1) {
+                each(0, blocks, [&](uint32_t j, uint32_t key) {
+                    const bool match = between(j) && key >> 21 == prefix >> 21;
+                    const uint64_t mask = __ballot(match);
+                    if (!mask) return;
+                    uint32_t at = 0;
+                    if (lane == 0) at = atomicAdd(&listed, (uint32_t)__popcll(mask));
+                    at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + (uint32_t)__popcll(mask & ((1ull << lane) - 1));
+                    if (match) {
+                        atomicAdd(&bins[(key >> 10) & 2047u], 1u);
+                        if (at < kSelectList) listed_keys[at] = key;
+                    }
+                });
+            } else if (listed <= kSelectList) {
+                for (uint32_t i = tid; i < listed; i += kSelectThreads)
+                    if (listed_keys[i] >> 10 == prefix >> 10) atomicAdd(&bins[listed_keys[i] & 1023u], 1u);
+            } else {
+                each(0, blocks, [&](uint32_t j, uint32_t key) {
+                    if (between(j) && key >> 10 == prefix >> 10) atomicAdd(&bins[key & 1023u], 1u);
+                });
+            }
             __syncthreads();
             // counts from the highest bin down, two bins a thread: the one in which the need is met
             const uint32_t bin = kSelectBins - 1 - 2 * tid, upper = bins[bin], pair = upper + bins[bin - 1];
@@ -361,7 +379,7 @@ __global__ __launch_bounds__(kSelectThreads) void kv_block_select_kernel(KvBlock
                 left = need - before - (first ? 0 : upper);
             }
             __syncthreads();
-            prefix |= found << shift;
+            prefix |= found << shifts[digit];
             need = left;
         }
     }
@@ -370,9 +388,9 @@ __global__ __launch_bounds__(kSelectThreads) void kv_block_select_kernel(KvBlock
     for (uint32_t first = 0; first < blocks; first += kSelectThreads) {
         const uint32_t last = min(first + kSelectThreads, blocks);
         __syncthreads();
-        each(first, last, false, [&](uint32_t j, uint32_t key, bool there) {
-            const uint32_t t = j * kKvTokens + lane;
-            const uint64_t keep = __ballot(there ? some && key > prefix : t < length), tie = __ballot(there && some && key == prefix);
+        each(first, last, [&](uint32_t j, uint32_t key) {
+            const bool there = between(j);
+            const uint64_t keep = __ballot(there ? some && key > prefix : j * kKvTokens + lane < length), tie = __ballot(there && some && key == prefix);
             if (lane == 0) { keep_masks[j - first] = keep; tie_masks[j - first] = tie; }
         });
         __syncthreads();
@@ -381,7 +399,7 @@ __global__ __launch_bounds__(kSelectThreads) void kv_block_select_kernel(KvBlock
         uint2 all;
         const uint2 before = scan_counts(make_uint2((uint32_t)__popcll(keep), (uint32_t)__popcll(tie)), totals, lane, wave, &all);
         const uint32_t ties_before = ties + before.y;
-        const uint32_t place = written + before.x + min(ties_before, need) - min(ties, need);
+        uint32_t place = written + before.x + min(ties_before, need) - min(ties, need);
         // the block's ties that are kept are its first: drop the last set bits until they fit
         uint32_t fit = ties_before < need ? need - ties_before : 0;
         if ((uint32_t)__popcll(tie) > fit) {
@@ -392,23 +410,18 @@ __global__ __launch_bounds__(kSelectThreads) void kv_block_select_kernel(KvBlock
             }
             tie = chosen;
         }
-        keep |= tie;
-        // (a thread's masks pass from its lane to the whole wavefront)
-        for (uint32_t k = 0; k < 64; k++) {
-            const uint32_t j = first + wave * 64 + k;
-            if (j >= last) break;
-            const uint64_t mask = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(keep >> 32), (int)k) << 32) |
-                                  (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)keep, (int)k);
-            const uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)place, (int)k) + (uint32_t)__popcll(mask & ((1ull << lane) - 1));
-            if ((mask >> lane) & 1) out[at] = (int32_t)(j * kKvTokens + lane);
-        }
+        for (keep |= tie; keep; keep &= keep - 1) out[place++] = (int32_t)((first + tid) * kKvTokens + (uint32_t)__builtin_ctzll(keep));
         written += all.x + min(ties + all.y, need) - min(ties, need);
         ties += all.y;
     }
 }
 
 // One workgroup per new block, head and sequence: keys and values of its 64 kept tokens, gathered piece by piece (keys)
-// and code by code (values, whose pieces hold sixteen tokens), brought to the largest of their scales.
+// and code by code (values, whose pieces hold sixteen tokens), brought to the largest of their scales.  Bound by cache
+// lines: a line of 128 bytes holds pieces of eight tokens' keys or eight dimensions' values, so as soon as one token in
+// eight is kept, nearly all of the old blocks is read (8 sequences of 8192 tokens, 8 heads of 128, to 2048: 134 MB read
+// and 34 written in 38 us).  Passing the old blocks' values through LDS in whole, and picking the codes there, took
+// 47 us: the reads are the same, and a workgroup waits for its blocks behind two barriers more.
 template <int HD>
 __global__ __launch_bounds__(2 * HD) void kv_block_gather_kernel(KvBlockArgs a, EvictArgs e) {
     __shared__ int32_t block_of[kKvTokens];               // source block of each kept token, -1: none
