@@ -40,9 +40,14 @@ struct AttentionArgs {
     float* scores;
     float* lse2;
     uint32_t score_rows, score_stride;
+    // weights of many rows: the rows as operands, [sequence * kv_heads + head][32 rows][HD / 16][lane], and their factors
+    u32x4* operands;
+    float* factors;
+    uint32_t operand_tiles;
 };
 
 constexpr float kLowest = -3.402823466e38f;
+constexpr uint32_t kFewParts = 4;
 constexpr uint32_t kMostParts = 128;                  // parts that the visible blocks of a row tile are split into
 constexpr float kRaise = 8.0f, kHeadroom = 6.0f;      // log2: how far scores may pass m, and p = 2^6 at the maximum
 
@@ -493,6 +498,12 @@ __global__ __launch_bounds__(64 * WAVES, HD == 256 ? 1 : 2) void kv_block_attent
 #pragma unroll
         for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
 
+    if (a.operands && part == 0 && working) {              // for the weight sums: the rows as they are multiplied
+        const size_t at = ((size_t)b * a.kv.kv_heads + head) * a.operand_tiles + w0 / 32;
+#pragma unroll
+        for (int k = 0; k < HD / 16; k++) a.operands[(at * (HD / 16) + k) * 64 + lane] = __builtin_bit_cast(u32x4, q[k >> 2][(k >> 1) & 1][k & 1]);
+        if (h == 0) a.factors[at * 32 + n] = factor;
+    }
     TileLoader<HD, WAVES> raw;
     BlockScales scales[2] = {};
     int32_t id[2] = {-1, -1};
@@ -606,80 +617,61 @@ __global__ __launch_bounds__(64 * WAVES, HD == 256 ? 1 : 2) void kv_block_attent
 }
 
 // Weight sums of many rows: the scores are computed again, tokens against all rows that see them.  A wavefront holds the
-// keys of 32 tokens as operands and adds up 2^(x - lse2) over the rows, which pass through LDS 32 at a time; the sums of
-// its lanes, which hold different rows, are added at the end, so every sum is made in one fixed order.
+// keys of 32 tokens as operands and adds up 2^(x - lse2) over the rows, whose operands the tiles kernel left in memory and
+// which pass through LDS 32 at a time, 32 more on their way meanwhile; the sums of its lanes, which hold different rows,
+// are added at the end, so every sum is made in one fixed order.
+constexpr uint32_t kWeightWaves = 4;
 template <int HD>
-__global__ __launch_bounds__(256, 2) void kv_block_weights_tiles_kernel(AttentionArgs a) {
-    constexpr int S = HD / 64;
+__global__ __launch_bounds__(64 * kWeightWaves, 2) void kv_block_weights_tiles_kernel(AttentionArgs a) {
+    constexpr int S = HD / 64, PER = HD / 16 / kWeightWaves;      // operands of 64 lanes that a wavefront moves
     __shared__ u32x4 lds_q[2][(HD / 16) * 64];
-    __shared__ float lds_factor[2][32], lds_lse[2][32];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
     const uint32_t n = lane & 31, h = lane >> 5;
     const uint32_t head = blockIdx.x % a.kv.kv_heads, chunk = blockIdx.x / a.kv.kv_heads, b = blockIdx.z;
     const KvSequence s = kv_sequence(a.kv, b);
-    const int32_t start = (int32_t)chunk * 128, base = start + (int32_t)wave * 32;      // the workgroup's first token, the wavefront's
+    // the last blocks of a prompt are seen by fewest rows: they start last
+    const int32_t start = (int32_t)(chunk * kWeightWaves * 32), base = start + (int32_t)(wave * 32);
     if (start >= s.length || s.rows <= 0) return;
     const uint32_t rows = (uint32_t)s.rows * a.group;
-    // rows that see any of the workgroup's tokens: positions start .. start + 127 + window - 1
-    const uint32_t r_first = (uint32_t)max(start - s.first(), 0) * a.group;
-    const int64_t behind = a.window ? (int64_t)start + 127 + a.window - s.first() : (int64_t)s.rows;      // the first token past them
+    // rows that see any of the workgroup's tokens, in tiles of 32
+    const uint32_t r_first = (uint32_t)max(start - s.first(), 0) * a.group / 32 * 32;
+    const int64_t behind = a.window ? (int64_t)start + kWeightWaves * 32 - 1 + a.window - s.first() : (int64_t)s.rows;
     const uint32_t r_last = (uint32_t)max((int64_t)0, min((int64_t)s.rows, behind)) * a.group;
-    const int32_t id = base < s.length ? kv_block_id(a.kv, s.table, base / (int32_t)kKvTokens) : -1;
-    const int32_t block = id < 0 ? 0 : id;
-    const uint32_t half = (uint32_t)(base / 32) & 1;
+    const int32_t id = base < s.length ? scalar_block_id(a.kv, s.table, base / (int32_t)kKvTokens) : -1;
+    const float ks = scalar_scales(a.kv, id, head).key;
     half8 k[HD / 16];
     {
-        const u32x4* const kp = (const u32x4*)kv_codes<HD>(a.kv, block, head, 0);
+        const u32x4* const kp = (const u32x4*)kv_codes<HD>(a.kv, id < 0 ? 0 : id, head, 0) + (wave & 1) * 2 * S * 64;
 #pragma unroll
         for (int i = 0; i < S; i++)
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-                const u32x4 w = biased(kp[((half * 2 + (n >> 4)) * S + i) * 64 + (c * 2 + h) * 16 + (n & 15)]);
+                const u32x4 w = biased(kp[((n >> 4) * S + i) * 64 + (c * 2 + h) * 16 + (n & 15)]);
                 k[i * 4 + c * 2] = codes_f16(w.x, w.y);
                 k[i * 4 + c * 2 + 1] = codes_f16(w.z, w.w);
             }
     }
-    const float ks = *kv_scale(a.kv, block, head, 0);
     float sum[16];
 #pragma unroll
     for (int i = 0; i < 16; i++) sum[i] = 0.0f;
-    // a thread stages 16 dimensions of a row at a time: HD / 16 threads a row
-    constexpr uint32_t PER_ROW = HD / 16, AT_ONCE = 256 / PER_ROW;
-    auto stage = [&](uint32_t first, int slot) {
+    const size_t slot = (size_t)b * a.kv.kv_heads + head;
+    u32x4 next[PER];
+    float next_factor = 0.0f, next_lse = INFINITY;
+    auto fetch = [&](uint32_t first) {
+        const size_t at = slot * a.operand_tiles + first / 32;
 #pragma unroll
-        for (uint32_t pass = 0; pass < 32 / (AT_ONCE < 32 ? AT_ONCE : 32); pass++) {
-            const uint32_t row = pass * AT_ONCE + tid / PER_ROW, piece = tid % PER_ROW;
-            if (row >= 32) continue;
-            const uint32_t r = first + row, token = r / a.group, q_head = head * a.group + r % a.group;
-            const bool there = r < rows;
-            float x[16], top = 0.0f;
-            widen_query16(a, there, load_query16(a, (there ? (size_t)(s.row0 + (int32_t)token) * a.q_stride + (size_t)q_head * HD : 0) + piece * 16), x);
-#pragma unroll
-            for (int e = 0; e < 16; e++) top = fmaxf(top, fabsf(x[e]));
-#pragma unroll
-            for (uint32_t o = 1; o < PER_ROW; o *= 2) top = fmaxf(top, __shfl_xor(top, (int)o));
-            float up, down;
-            row_power(top, up, down);
-            half8 v[2];
-#pragma unroll
-            for (int e = 0; e < 16; e++) v[e >> 3][e & 7] = (_Float16)(x[e] * up);
-            // dimensions 64 i + 16 (2 c + h) .. : fragments 4 i + 2 c and the next, slot 32 h + row
-            const uint32_t fragment = (piece >> 2) * 4 + ((piece >> 1) & 1) * 2, place = (piece & 1) * 32 + row;
-            lds_q[slot][fragment * 64 + place] = __builtin_bit_cast(u32x4, v[0]);
-            lds_q[slot][(fragment + 1) * 64 + place] = __builtin_bit_cast(u32x4, v[1]);
-            if (piece == 0) {
-                lds_factor[slot][row] = a.scale_log2 * down;
-                // a row that is not there, or saw nothing, gives weights of 2^-inf
-                const float lse2 = there ? a.lse2[((size_t)b * a.kv.kv_heads + head) * a.score_rows + r] : INFINITY;
-                lds_lse[slot][row] = lse2 == -INFINITY ? INFINITY : lse2;
-            }
-        }
+        for (int i = 0; i < PER; i++) next[i] = a.operands[(at * (HD / 16) + wave * PER + i) * 64 + lane];
+        next_factor = a.factors[at * 32 + n];
+        next_lse = first + n < rows ? a.lse2[slot * a.score_rows + first + n] : INFINITY;
     };
-    int slot = 0;
-    if (r_first < r_last) stage(r_first, 0);
-    __syncthreads();
-    for (uint32_t first = r_first; first < r_last; first += 32, slot ^= 1) {
-        if (first + 32 < r_last) stage(first + 32, slot ^ 1);
+    if (r_first < r_last) fetch(r_first);
+    int buffer = 0;
+    for (uint32_t first = r_first; first < r_last; first += 32, buffer ^= 1) {
+#pragma unroll
+        for (int i = 0; i < PER; i++) lds_q[buffer][(wave * PER + i) * 64 + lane] = next[i];
+        const float f = fmaxf(next_factor * ks, 1e-37f), lse2 = next_lse == -INFINITY ? INFINITY : next_lse;
+        __syncthreads();                                   // (the other buffer's readers are all past the barrier before)
+        if (first + 32 < r_last) fetch(first + 32);
         const int32_t position = s.first() + (int32_t)((first + n) / a.group), low = row_low(a, position);
         const int32_t p_low = s.first() + (int32_t)(first / a.group), p_high = s.first() + (int32_t)((first + 31) / a.group);
         if (id >= 0 && p_high >= base && base + 31 >= row_low(a, p_low)) {
@@ -688,8 +680,7 @@ __global__ __launch_bounds__(256, 2) void kv_block_weights_tiles_kernel(Attentio
             for (int i = 0; i < 16; i++) x[i] = 0.0f;
 #pragma unroll
             for (int i = 0; i < HD / 16; i++)
-                x = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i], __builtin_bit_cast(half8, lds_q[slot][i * 64 + lane]), x, 0, 0, 0);
-            const float f = fmaxf(lds_factor[slot][n] * ks, 1e-37f), lse2 = lds_lse[slot][n];
+                x = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i], __builtin_bit_cast(half8, lds_q[buffer][i * 64 + lane]), x, 0, 0, 0);
             if (!(base + 31 <= p_low && base >= row_low(a, p_high))) {
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
@@ -700,15 +691,65 @@ __global__ __launch_bounds__(256, 2) void kv_block_weights_tiles_kernel(Attentio
 #pragma unroll
             for (int i = 0; i < 16; i++) sum[i] += __builtin_amdgcn_exp2f(fmaf(x[i], f, -lse2));
         }
-        __syncthreads();
     }
     if (id < 0) return;
+    float* const at = kv_sums(a.kv, id, head) + (wave & 1) * 32;
 #pragma unroll
     for (int i = 0; i < 16; i++) {
         float v = sum[i];
         v += lane_xor<1>(v); v += lane_xor<2>(v); v += lane_xor<4>(v); v += lane_xor<8>(v); v += lane_xor<16>(v);
-        const int32_t at = base + (i >> 2) * 8 + (int32_t)h * 4 + (i & 3);
-        if (n == 0 && at < s.length) kv_sums(a.kv, block, head)[at % (int32_t)kKvTokens] += v;
+        const int32_t token = (i >> 2) * 8 + (int32_t)h * 4 + (i & 3);
+        if (n == 0 && base + token < s.length) at[token] += v;
+    }
+}
+
+// Joins few parts (kFewParts at most) of a row: one wavefront per row, added in order.
+template <int HD>
+__global__ __launch_bounds__(256) void kv_block_attention_join_few_kernel(AttentionArgs a, uint32_t tile_rows) {
+    constexpr int E = HD / 64;
+    const uint32_t lane = threadIdx.x & 63, head = blockIdx.y, b = blockIdx.z;
+    const uint32_t r = (uint32_t)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+    const KvSequence s = kv_sequence(a.kv, b);
+    const uint32_t rows = (uint32_t)s.rows * a.group;
+    if (r >= rows) return;
+    const uint32_t tile = r / tile_rows, r0 = tile * tile_rows;
+    const uint32_t parts = part_count(a, row_range(a, s, r0, min(r0 + tile_rows, rows)));
+    if (parts == 1) return;
+    const size_t slot = (((size_t)b * a.kv.kv_heads + head) * a.tiles + tile) * a.parts * tile_rows + (r - r0);
+    float2 ml[kFewParts];
+    float x[kFewParts][E], top = kLowest;
+#pragma unroll
+    for (uint32_t p = 0; p < kFewParts; p++) {
+        const size_t at = slot + (size_t)(p < parts ? p : 0) * tile_rows;
+        ml[p] = a.part_ml[at];
+        if (p >= parts) ml[p] = make_float2(kLowest, 0.0f);
+#pragma unroll
+        for (int e = 0; e < E; e++) x[p][e] = a.part_out[at * HD + e * 64 + lane];
+        top = fmaxf(top, ml[p].x);
+    }
+    float l = 0.0f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) o[e] = 0.0f;
+#pragma unroll
+    for (uint32_t p = 0; p < kFewParts; p++) {
+        const float f = p < parts ? exp2f(ml[p].x - top) : 0.0f;
+        l += ml[p].y * f;
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] += x[p][e] * f;
+    }
+    const uint32_t token = r / a.group, h = head * a.group + r % a.group;
+    const size_t row = (size_t)(s.row0 + (int32_t)token);
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const size_t at = row * a.out_stride + (size_t)h * HD + e * 64 + lane;
+        if (a.out_dtype == MI355Q_BF16) ((uint16_t*)a.out)[at] = f32_to_bf16_rne(o[e] * f);
+        else ((uint16_t*)a.out)[at] = f32_to_f16_rne(o[e] * f);
+    }
+    if (lane == 0) {
+        const float lse2 = l == 0.0f ? -INFINITY : top + log2f(l);
+        if (a.lse) a.lse[row * a.heads + h] = lse2 * 0.6931471805599453f;
+        if (a.lse2) a.lse2[((size_t)b * a.kv.kv_heads + head) * a.score_rows + r] = lse2;
     }
 }
 
@@ -823,6 +864,16 @@ void choose_parts(AttentionArgs* a, uint64_t blocks, uint64_t groups, uint32_t w
     a->parts = (uint32_t)((blocks + a->part_blocks - 1) / a->part_blocks);
 }
 
+template <int HD>
+mi355q_status launch_join(hipStream_t s, const AttentionArgs& a, uint32_t rows, uint32_t tile_rows) {
+    if (a.parts <= kFewParts)
+        kv_block_attention_join_few_kernel<HD><<<dim3((rows + 3) / 4, a.kv.kv_heads, a.kv.sequences), 256, 0, s>>>(a, tile_rows);
+    else
+        kv_block_attention_join_kernel<HD><<<dim3(rows, a.kv.kv_heads, a.kv.sequences), 256, 0, s>>>(a, tile_rows);
+    MI355Q_HIP(hipGetLastError());
+    return MI355Q_OK;
+}
+
 template <int HD, int WAVES>
 mi355q_status launch_tiles(mi355q_context* ctx, hipStream_t s, AttentionArgs a, bool weights) {
     constexpr uint32_t ROWS = 32 * WAVES;
@@ -837,7 +888,13 @@ mi355q_status launch_tiles(mi355q_context* ctx, hipStream_t s, AttentionArgs a, 
             a.part_out = buf.take<float>(groups * a.parts * ROWS * HD);
             a.part_ml = buf.take<float2>(groups * a.parts * ROWS);
         }
-        if (weights) a.lse2 = buf.take<float>((size_t)a.kv.sequences * a.kv.kv_heads * rows);
+        if (weights) {
+            const size_t slots = (size_t)a.kv.sequences * a.kv.kv_heads;
+            a.operand_tiles = a.tiles * WAVES;
+            a.lse2 = buf.take<float>(slots * rows);
+            a.operands = buf.take<u32x4>(slots * a.operand_tiles * (HD / 16) * 64);
+            a.factors = buf.take<float>(slots * a.operand_tiles * 32);
+        }
         if (!pass && buf.used)
             if (mi355q_status st = ensure_workspace(ctx, buf.used)) return st;
     }
@@ -846,11 +903,11 @@ mi355q_status launch_tiles(mi355q_context* ctx, hipStream_t s, AttentionArgs a, 
     kv_block_attention_tiles_kernel<HD, WAVES><<<dim3(a.kv.kv_heads * a.parts, a.tiles, a.kv.sequences), 64 * WAVES, lds, s>>>(a);
     MI355Q_HIP(hipGetLastError());
     if (a.parts > 1) {
-        kv_block_attention_join_kernel<HD><<<dim3(rows, a.kv.kv_heads, a.kv.sequences), 256, 0, s>>>(a, ROWS);
-        MI355Q_HIP(hipGetLastError());
+        if (mi355q_status st = launch_join<HD>(s, a, rows, ROWS)) return st;
     }
     if (weights) {
-        kv_block_weights_tiles_kernel<HD><<<dim3((a.kv.max_length + 127) / 128 * a.kv.kv_heads, 1, a.kv.sequences), 256, 0, s>>>(a);
+        const uint32_t tokens = kWeightWaves * 32;
+        kv_block_weights_tiles_kernel<HD><<<dim3((a.kv.max_length + tokens - 1) / tokens * a.kv.kv_heads, 1, a.kv.sequences), 64 * kWeightWaves, 0, s>>>(a);
         MI355Q_HIP(hipGetLastError());
     }
     return MI355Q_OK;
@@ -880,8 +937,7 @@ mi355q_status launch_rows(mi355q_context* ctx, hipStream_t s, AttentionArgs a, b
     kv_block_attention_rows_kernel<HD, RT><<<dim3(a.kv.kv_heads * a.parts, 1, a.kv.sequences), 256, 0, s>>>(a);
     MI355Q_HIP(hipGetLastError());
     if (a.parts > 1) {
-        kv_block_attention_join_kernel<HD><<<dim3(rows, a.kv.kv_heads, a.kv.sequences), 256, 0, s>>>(a, 16 * RT);
-        MI355Q_HIP(hipGetLastError());
+        if (mi355q_status st = launch_join<HD>(s, a, rows, 16 * RT)) return st;
     }
     if (weights) {
         kv_block_weights_kernel<<<dim3((a.kv.max_length + 1023) / 1024 * a.kv.kv_heads, 1, a.kv.sequences), 256, 0, s>>>(a);
