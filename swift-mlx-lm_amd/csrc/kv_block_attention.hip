@@ -399,10 +399,13 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void kv_block_attention_row
 }
 
 // ---- many rows: prompts and prompt chunks ------------------------------------------------------------------------------
-// A workgroup takes 32 WAVES rows of one KV head, 32 a wavefront, and walks the visible blocks (or one part of them).  A
+// A workgroup takes 128 rows of one KV head, 32 a wavefront, and walks the visible blocks (or one part of them).  A
 // block's codes are read once per workgroup, 16 bytes a lane, become f16 on the way into LDS, and lie there as the
 // fragments of 32 x 32 x 16 products, so that an operand is one conflict-free 16-byte read a lane: the loads of block
-// j + 2 and the conversion of block j + 1 overlap the products of block j.
+// j + 2 and the conversion of block j + 1 overlap the products of block j.  Two wavefronts a SIMD take turns on the matrix
+// cores and the vector unit, which need about the same time.  With heads of 256 the accumulators and rows of 32 rows fill
+// half of the register file and the blocks the LDS of a CU: there two wavefronts share their rows, each taking half of a
+// block's tokens (TS = 2), and add up their results at the end.
 template <int HD, int WAVES>
 struct TileLds {
     u32x4 key[2 * (HD / 16) * 64];      // fragment (32-token half, sixteen dimensions)
@@ -466,14 +469,16 @@ __device__ __forceinline__ float load_query_tile(const AttentionArgs& a, bool th
     return a.scale_log2 * down;
 }
 
-template <int HD, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, HD == 256 ? 1 : 2) void kv_block_attention_tiles_kernel(AttentionArgs a) {
-    constexpr int S = HD / 64, DT = HD / 32;
-    constexpr uint32_t ROWS = 32 * WAVES;
+constexpr uint32_t kTileRows = 128;
+
+template <int HD, int TS>
+__global__ __launch_bounds__(256 * TS, 2) void kv_block_attention_tiles_kernel(AttentionArgs a) {
+    constexpr int S = HD / 64, DT = HD / 32, WAVES = 4 * TS, TT = 2 / TS;      // TT: 32-token halves of a wavefront
+    constexpr uint32_t ROWS = kTileRows;
     extern __shared__ __align__(16) uint8_t lds_raw[];
     TileLds<HD, WAVES>* const lds = (TileLds<HD, WAVES>*)lds_raw;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
-    const uint32_t n = lane & 31, h = lane >> 5;
+    const uint32_t n = lane & 31, h = lane >> 5, group = wave & 3, share = wave >> 2;      // rows, and which half of the tokens
     // the last rows of a prompt see most: they start first
     const uint32_t head = blockIdx.x % a.kv.kv_heads, part = blockIdx.x / a.kv.kv_heads, tile = gridDim.y - 1 - blockIdx.y, b = blockIdx.z;
     const KvSequence s = kv_sequence(a.kv, b);
@@ -485,7 +490,7 @@ __global__ __launch_bounds__(64 * WAVES, HD == 256 ? 1 : 2) void kv_block_attent
     if (part >= parts) return;
     const int32_t begin = g.first + (int32_t)(part * a.part_blocks), end = min(begin + (int32_t)a.part_blocks, g.last);
 
-    const uint32_t w0 = r0 + wave * 32, r = w0 + n, token = r / a.group, out_head = head * a.group + r % a.group;
+    const uint32_t w0 = r0 + group * 32, r = w0 + n, token = r / a.group, out_head = head * a.group + r % a.group;
     const bool working = w0 < r1;                          // a wavefront without rows only moves blocks
     const int32_t position = s.first() + (int32_t)token, low = row_low(a, position);
     const RowRange own = row_range(a, s, w0, working ? min(w0 + 32, r1) : w0 + 1);
@@ -498,7 +503,7 @@ __global__ __launch_bounds__(64 * WAVES, HD == 256 ? 1 : 2) void kv_block_attent
 #pragma unroll
         for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
 
-    if (a.operands && part == 0 && working) {              // for the weight sums: the rows as they are multiplied
+    if (a.operands && part == 0 && working && share == 0) {              // for the weight sums: the rows as they are multiplied
         const size_t at = ((size_t)b * a.kv.kv_heads + head) * a.operand_tiles + w0 / 32;
 #pragma unroll
         for (int k = 0; k < HD / 16; k++) a.operands[(at * (HD / 16) + k) * 64 + lane] = __builtin_bit_cast(u32x4, q[k >> 2][(k >> 1) & 1][k & 1]);
@@ -525,15 +530,16 @@ __global__ __launch_bounds__(64 * WAVES, HD == 256 ? 1 : 2) void kv_block_attent
         const int32_t id_now = id[slot];
         const int32_t base = j * (int32_t)kKvTokens;
         const bool visible = working && id_now >= 0 && j >= own.first && j < own.last;
-        floatx16 x[2];
+        floatx16 x[TT];
+        const uint32_t key_lane = share * (HD / 16) * 64 + lane, value_lane = share * 2 * 64 + lane;
         if (visible) {
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
+            for (int t = 0; t < TT; t++) {
 #pragma unroll
                 for (int i = 0; i < 16; i++) x[t][i] = 0.0f;
 #pragma unroll
                 for (int k = 0; k < HD / 16; k++)
-                    x[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, cur.key[(t * (HD / 16) + k) * 64 + lane]),
+                    x[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, cur.key[(t * (HD / 16) + k) * 64 + key_lane]),
                                                                   q[k >> 2][(k >> 1) & 1][k & 1], x[t], 0, 0, 0);
             }
         }
@@ -544,16 +550,16 @@ __global__ __launch_bounds__(64 * WAVES, HD == 256 ? 1 : 2) void kv_block_attent
             const float vlog = now.value > 0.0f ? log2f(now.value) : 0.0f, vinv = exp2f(-vlog);
             if (!(base + 63 <= own.low && (!a.window || base >= row_low(a, own.high)))) {
 #pragma unroll
-                for (int t = 0; t < 2; t++)
+                for (int t = 0; t < TT; t++)
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        const int32_t at = base + t * 32 + (i >> 2) * 8 + (int32_t)h * 4 + (i & 3);
+                        const int32_t at = base + (int32_t)(t + share) * 32 + (i >> 2) * 8 + (int32_t)h * 4 + (i & 3);
                         x[t][i] = at >= low && at <= position ? x[t][i] : -INFINITY;
                     }
             }
-            float top = fmaxf(x[0][0], x[1][0]);
+            float top = x[0][0];
 #pragma unroll
-            for (int i = 1; i < 16; i++) top = fmaxf(top, fmaxf(x[0][i], x[1][i]));
+            for (int i = 1; i < 16 * TT; i++) top = fmaxf(top, x[i >> 4][i & 15]);
             top = top * f + (vlog - kHeadroom);
             if (__ballot(top > m + kRaise)) {
                 const float raised = fmaxf(m, fmaxf(top, lane_xor<32>(top)));
@@ -565,9 +571,9 @@ __global__ __launch_bounds__(64 * WAVES, HD == 256 ? 1 : 2) void kv_block_attent
             }
             const float shift = vlog - m;
             float sum = 0.0f;
-            half8 p[2][2];
+            half8 p[TT][2];
 #pragma unroll
-            for (int t = 0; t < 2; t++)
+            for (int t = 0; t < TT; t++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const float w = __builtin_amdgcn_exp2f(fmaf(x[t][i], f, shift));
@@ -578,8 +584,8 @@ __global__ __launch_bounds__(64 * WAVES, HD == 256 ? 1 : 2) void kv_block_attent
 #pragma unroll
             for (int d = 0; d < DT; d++)
 #pragma unroll
-                for (int k = 0; k < 4; k++)
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, cur.value[(d * 4 + k) * 64 + lane]),
+                for (int k = 0; k < 2 * TT; k++)
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, cur.value[(d * 4 + k) * 64 + value_lane]),
                                                                   p[k >> 1][k & 1], o[d], 0, 0, 0);
         }
         __syncthreads();
@@ -590,6 +596,26 @@ __global__ __launch_bounds__(64 * WAVES, HD == 256 ? 1 : 2) void kv_block_attent
     }
 
     l += lane_xor<32>(l);
+    if constexpr (TS == 2) {                               // the second half's results to the first, over the blocks' LDS
+        float* const other = (float*)lds_raw + group * (DT * 16 + 2) * 64;
+        if (share) {
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) other[(d * 16 + i) * 64 + lane] = o[d][i];
+            other[DT * 16 * 64 + lane] = m;
+            other[(DT * 16 + 1) * 64 + lane] = l;
+        }
+        __syncthreads();
+        if (share) return;
+        const float om = other[DT * 16 * 64 + lane], top = fmaxf(m, om), f0 = exp2f(m - top), f1 = exp2f(om - top);
+        l = l * f0 + other[(DT * 16 + 1) * 64 + lane] * f1;
+        m = top;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[d][i] = o[d][i] * f0 + other[(d * 16 + i) * 64 + lane] * f1;
+    }
     if (r >= r1) return;
     if (parts > 1) {
         const size_t slot = ((((size_t)b * a.kv.kv_heads + head) * a.tiles + tile) * a.parts + part) * ROWS + (r - r0);
@@ -874,9 +900,10 @@ mi355q_status launch_join(hipStream_t s, const AttentionArgs& a, uint32_t rows, 
     return MI355Q_OK;
 }
 
-template <int HD, int WAVES>
+template <int HD>
 mi355q_status launch_tiles(mi355q_context* ctx, hipStream_t s, AttentionArgs a, bool weights) {
-    constexpr uint32_t ROWS = 32 * WAVES;
+    constexpr int TS = HD == 256 ? 2 : 1;
+    constexpr uint32_t ROWS = kTileRows;
     const uint32_t rows = a.kv.max_rows * a.group;
     a.tiles = (rows + ROWS - 1) / ROWS;
     const uint64_t groups = (uint64_t)a.kv.kv_heads * a.tiles * a.kv.sequences;
@@ -890,7 +917,7 @@ mi355q_status launch_tiles(mi355q_context* ctx, hipStream_t s, AttentionArgs a, 
         }
         if (weights) {
             const size_t slots = (size_t)a.kv.sequences * a.kv.kv_heads;
-            a.operand_tiles = a.tiles * WAVES;
+            a.operand_tiles = a.tiles * (ROWS / 32);
             a.lse2 = buf.take<float>(slots * rows);
             a.operands = buf.take<u32x4>(slots * a.operand_tiles * (HD / 16) * 64);
             a.factors = buf.take<float>(slots * a.operand_tiles * 32);
@@ -898,9 +925,10 @@ mi355q_status launch_tiles(mi355q_context* ctx, hipStream_t s, AttentionArgs a, 
         if (!pass && buf.used)
             if (mi355q_status st = ensure_workspace(ctx, buf.used)) return st;
     }
-    constexpr size_t lds = 2 * sizeof(TileLds<HD, WAVES>);
-    if (mi355q_status st = raise_lds_limit((const void*)kv_block_attention_tiles_kernel<HD, WAVES>, lds)) return st;
-    kv_block_attention_tiles_kernel<HD, WAVES><<<dim3(a.kv.kv_heads * a.parts, a.tiles, a.kv.sequences), 64 * WAVES, lds, s>>>(a);
+    // (two halves of a block's tokens add up in the room of the blocks: two rows of 64 numbers more)
+    constexpr size_t blocks = 2 * sizeof(TileLds<HD, 4 * TS>), lds = TS == 1 ? blocks : std::max(blocks, (size_t)4 * (HD / 2 + 2) * 256);
+    if (mi355q_status st = raise_lds_limit((const void*)kv_block_attention_tiles_kernel<HD, TS>, lds)) return st;
+    kv_block_attention_tiles_kernel<HD, TS><<<dim3(a.kv.kv_heads * a.parts, a.tiles, a.kv.sequences), 256 * TS, lds, s>>>(a);
     MI355Q_HIP(hipGetLastError());
     if (a.parts > 1) {
         if (mi355q_status st = launch_join<HD>(s, a, rows, ROWS)) return st;
@@ -987,6 +1015,6 @@ extern "C" mi355q_status mi355q_kv_block_attention(mi355q_context* ctx, void* st
         const uint32_t rows = a.kv.max_rows * a.group;
         if (rows <= 16) return launch_rows<HD, 1>(ctx, (hipStream_t)stream, a, accumulate_weights != 0);
         if (HD < 256 && rows <= 32) return launch_rows<HD < 256 ? HD : 64, 2>(ctx, (hipStream_t)stream, a, accumulate_weights != 0);
-        return launch_tiles<HD, 4>(ctx, (hipStream_t)stream, a, accumulate_weights != 0);
+        return launch_tiles<HD>(ctx, (hipStream_t)stream, a, accumulate_weights != 0);
     });
 }
