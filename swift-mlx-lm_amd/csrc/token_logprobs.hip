@@ -6,9 +6,9 @@
 //
 // Alternatives: logits are ordered by 64-bit keys (ordered value, ~index), all distinct, so equal logits need no rule of
 // their own.  The pass itself only notes, for every lane, the largest logit of each of its steps of sixteen (one LDS
-// store).  At the end a wavefront takes the top_count-th largest of its 64 lanes' maxima as a limit that top_count logits
-// reach, and only the steps whose maximum reaches it -- some two dozen of the slice's hundreds or thousands -- are read
-// again, from the cache, and their keys collected in LDS and cut to the largest.
+// store).  At the end the top_count-th largest of a wavefront's 64 lane maxima is a limit that top_count logits reach, and
+// only the steps whose maximum reaches the highest limit of the workgroup's four wavefronts -- about top_count of the
+// slice's hundreds or thousands -- are read again, from the cache, and their keys collected in LDS and cut to the largest.
 #include "device_utils.h"
 
 namespace mi355q {
@@ -172,6 +172,7 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(LogprobArgs a) {
     __shared__ unsigned long long room[4][kTopRoom];
     __shared__ uint16_t maxima[4][kSliceSteps][64];  // of each step, each lane: the bf16 number at or above it
     __shared__ LogSum sums[4];
+    __shared__ float limits[4];
     __shared__ uint32_t counts[4];
     constexpr uint32_t VE = D == MI355Q_F32 ? 4 : 8;             // logits of a 16-byte load
     const uint32_t row = blockIdx.x / a.slices, slice = blockIdx.x - row * a.slices;
@@ -231,8 +232,11 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(LogprobArgs a) {
         if (a.top) maxima[wave][steps][lane] = bf16_above(top);
     }
     TopKeys keys{room[wave], kMaskedKey, 0, a.top, lane};
-    if (a.top && steps) {
-        const float limit = keys.limit_of(s.m);
+    if (a.top) {
+        const float own = steps ? keys.limit_of(s.m) : kMasked;
+        if (lane == 0) limits[wave] = own;
+        __syncthreads();
+        const float limit = fmaxf(fmaxf(limits[0], limits[1]), fmaxf(limits[2], limits[3]));
         const unsigned long long key = logit_key(limit, 0xFFFFFFFFu);
         keys.threshold = key > kMaskedKey ? key : kMaskedKey;
         // the steps of sixteen that reach the limit, as step * 64 + lane, over the maxima that have been looked at
@@ -309,7 +313,7 @@ __global__ __launch_bounds__(64) void token_logprobs_join_kernel(LogprobArgs a) 
         TopKeys keys{room, kMaskedKey, 0, a.top, lane};
         const size_t base = (size_t)row * a.slices * a.top;
         const uint32_t all = a.slices * a.top;
-        if (all > kTopRoom) {
+        if (all > 64) {
             // a limit that `top` keys reach: the slices' keys are in order, so if n of their q-th keys reach it, n q do
             const uint32_t lists = a.slices < 64 ? a.slices : 64, q = (a.top + lists - 1) / lists, n = (a.top + q - 1) / q;
             const unsigned long long own = lane < lists ? a.part_keys[base + (size_t)lane * a.top + q - 1] : 0;
