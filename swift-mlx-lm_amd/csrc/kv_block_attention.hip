@@ -44,6 +44,9 @@ struct AttentionArgs {
     u32x4* operands;
     float* factors;
     uint32_t operand_tiles;
+    // and what each of `sum_parts` shares of the rows adds, [share][sequence * kv_heads + head][sum_stride]
+    float* sums;
+    uint32_t sum_parts, sum_stride;
 };
 
 constexpr float kLowest = -3.402823466e38f;
@@ -645,7 +648,8 @@ __global__ __launch_bounds__(256 * TS, 2) void kv_block_attention_tiles_kernel(A
 // Weight sums of many rows: the scores are computed again, tokens against all rows that see them.  A wavefront holds the
 // keys of 32 tokens as operands and adds up 2^(x - lse2) over the rows, whose operands the tiles kernel left in memory and
 // which pass through LDS 32 at a time, 32 more on their way meanwhile; the sums of its lanes, which hold different rows,
-// are added at the end, so every sum is made in one fixed order.
+// are added at the end, so every sum is made in one fixed order.  Where there are few tokens and heads, the rows are dealt
+// to several workgroups, whose sums another launch adds in order.
 constexpr uint32_t kWeightWaves = 4;
 template <int HD>
 __global__ __launch_bounds__(64 * kWeightWaves, 2) void kv_block_weights_tiles_kernel(AttentionArgs a) {
@@ -660,9 +664,15 @@ __global__ __launch_bounds__(64 * kWeightWaves, 2) void kv_block_weights_tiles_k
     if (start >= s.length || s.rows <= 0) return;
     const uint32_t rows = (uint32_t)s.rows * a.group;
     // rows that see any of the workgroup's tokens, in tiles of 32
-    const uint32_t r_first = (uint32_t)max(start - s.first(), 0) * a.group / 32 * 32;
+    uint32_t r_first = (uint32_t)max(start - s.first(), 0) * a.group / 32 * 32;
     const int64_t behind = a.window ? (int64_t)start + kWeightWaves * 32 - 1 + a.window - s.first() : (int64_t)s.rows;
-    const uint32_t r_last = (uint32_t)max((int64_t)0, min((int64_t)s.rows, behind)) * a.group;
+    uint32_t r_last = (uint32_t)max((int64_t)0, min((int64_t)s.rows, behind)) * a.group;
+    const uint32_t share = blockIdx.y;
+    if (a.sum_parts > 1 && r_first < r_last) {
+        const uint32_t each = ((r_last - r_first + 31) / 32 + a.sum_parts - 1) / a.sum_parts * 32;
+        r_first += min(share * each, r_last - r_first);
+        r_last = min(r_first + each, r_last);
+    }
     const int32_t id = base < s.length ? scalar_block_id(a.kv, s.table, base / (int32_t)kKvTokens) : -1;
     const float ks = scalar_scales(a.kv, id, head).key;
     half8 k[HD / 16];
@@ -718,15 +728,31 @@ __global__ __launch_bounds__(64 * kWeightWaves, 2) void kv_block_weights_tiles_k
             for (int i = 0; i < 16; i++) sum[i] += __builtin_amdgcn_exp2f(fmaf(x[i], f, -lse2));
         }
     }
-    if (id < 0) return;
-    float* const at = kv_sums(a.kv, id, head) + (wave & 1) * 32;
+    float* const at = a.sum_parts > 1 ? a.sums + (share * (size_t)a.kv.sequences * a.kv.kv_heads + slot) * a.sum_stride + base
+                                      : kv_sums(a.kv, id < 0 ? 0 : id, head) + (wave & 1) * 32;
+    if (a.sum_parts == 1 && id < 0) return;
 #pragma unroll
     for (int i = 0; i < 16; i++) {
         float v = sum[i];
         v += lane_xor<1>(v); v += lane_xor<2>(v); v += lane_xor<4>(v); v += lane_xor<8>(v); v += lane_xor<16>(v);
         const int32_t token = (i >> 2) * 8 + (int32_t)h * 4 + (i & 3);
-        if (n == 0 && base + token < s.length) at[token] += v;
+        if (n == 0 && base + token < s.length) at[token] = a.sum_parts > 1 ? v : at[token] + v;
     }
+}
+
+// Adds the shares of the weight sums to the cache's, a thread per token.
+__global__ __launch_bounds__(256) void kv_block_weights_add_kernel(AttentionArgs a) {
+    const uint32_t head = blockIdx.x % a.kv.kv_heads, b = blockIdx.z;
+    const int32_t t = (int32_t)(blockIdx.x / a.kv.kv_heads * 256 + threadIdx.x);
+    const KvSequence s = kv_sequence(a.kv, b);
+    if (s.rows <= 0 || t >= s.length) return;
+    const int32_t id = kv_block_id(a.kv, s.table, t / (int32_t)kKvTokens);
+    if (id < 0) return;
+    const size_t slots = (size_t)a.kv.sequences * a.kv.kv_heads, slot = (size_t)b * a.kv.kv_heads + head;
+    float sum = 0.0f;
+#pragma unroll 4
+    for (uint32_t p = 0; p < a.sum_parts; p++) sum += a.sums[(p * slots + slot) * a.sum_stride + t];
+    kv_sums(a.kv, id, head)[t % (int32_t)kKvTokens] += sum;
 }
 
 // Joins few parts (kFewParts at most) of a row: one wavefront per row, added in order.
@@ -875,7 +901,7 @@ struct Buffers {
 };
 
 // Blocks that the rows of a tile can see, and the parts they are split into so that the launch has about `wanted`
-// workgroups; a part is a multiple of `unit` blocks.
+// workgroups; a part is a multiple of `unit` blocks, one for each wavefront.
 uint64_t visible_blocks(const AttentionArgs& a, uint32_t tile_rows) {
     const uint64_t blocks = (a.kv.max_length + kKvTokens - 1) / kKvTokens;
     if (!a.window) return blocks;
@@ -887,6 +913,23 @@ void choose_parts(AttentionArgs* a, uint64_t blocks, uint64_t groups, uint32_t w
     parts = std::min(parts, (blocks + unit - 1) / unit);
     parts = std::max<uint64_t>(1, std::min<uint64_t>(parts, kMostParts));
     a->part_blocks = (uint32_t)(((blocks + parts - 1) / parts + unit - 1) / unit * unit);
+    a->parts = (uint32_t)((blocks + a->part_blocks - 1) / a->part_blocks);
+}
+
+// The tiles kernel fills the chip with 512 workgroups.  Below that the blocks are split where it pays: a workgroup takes
+// about 1.1, 1.8 or 3.4 us a block (heads of 64, 128, 256), parts cost a launch (4 us) and their partial results in and
+// out at 4 TB/s.  (Prompts of 512, 1024 and 1500 rows, 32 heads of 128 on 8: one part 20, 33 and 46 us, as many as fill
+// the chip 25, 48 and 70; 200 rows on 5000 tokens: one part 150 us, nine 54.)
+void choose_tile_parts(AttentionArgs* a, int hd, uint64_t blocks, uint64_t groups) {
+    const double block_us = hd == 64 ? 1.1 : hd == 128 ? 1.8 : 3.4, part_us = (double)groups * kTileRows * hd * 8 / 4e6;
+    const uint64_t most = std::max<uint64_t>(1, std::min<uint64_t>({512 / groups, blocks, kMostParts}));
+    uint64_t parts = 1;
+    double best = (double)blocks * block_us;
+    for (uint64_t p = 2; p <= most; p++) {
+        const double us = (double)((blocks + p - 1) / p) * block_us + 4.0 + (double)p * part_us;
+        if (us < best) { best = us; parts = p; }
+    }
+    a->part_blocks = (uint32_t)((blocks + parts - 1) / parts);
     a->parts = (uint32_t)((blocks + a->part_blocks - 1) / a->part_blocks);
 }
 
@@ -907,8 +950,13 @@ mi355q_status launch_tiles(mi355q_context* ctx, hipStream_t s, AttentionArgs a, 
     const uint32_t rows = a.kv.max_rows * a.group;
     a.tiles = (rows + ROWS - 1) / ROWS;
     const uint64_t groups = (uint64_t)a.kv.kv_heads * a.tiles * a.kv.sequences;
-    choose_parts(&a, visible_blocks(a, ROWS), groups, 512, 4);
+    choose_tile_parts(&a, HD, visible_blocks(a, ROWS), groups);
     a.score_rows = rows;
+    // shares of the rows for the weight sums: about three workgroups a CU, each with eight tiles of 32 rows at least
+    const uint32_t tokens = kWeightWaves * 32, chunks = (a.kv.max_length + tokens - 1) / tokens;
+    const uint64_t owners = (uint64_t)chunks * a.kv.kv_heads * a.kv.sequences;
+    a.sum_stride = chunks * tokens;
+    a.sum_parts = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({(768 + owners - 1) / owners, (rows + 255) / 256, 64}));
     for (int pass = 0; pass < 2; pass++) {
         Buffers buf{pass ? (char*)ctx->workspace : nullptr, 0};
         if (a.parts > 1) {
@@ -921,6 +969,7 @@ mi355q_status launch_tiles(mi355q_context* ctx, hipStream_t s, AttentionArgs a, 
             a.lse2 = buf.take<float>(slots * rows);
             a.operands = buf.take<u32x4>(slots * a.operand_tiles * (HD / 16) * 64);
             a.factors = buf.take<float>(slots * a.operand_tiles * 32);
+            if (a.sum_parts > 1) a.sums = buf.take<float>(a.sum_parts * slots * a.sum_stride);
         }
         if (!pass && buf.used)
             if (mi355q_status st = ensure_workspace(ctx, buf.used)) return st;
@@ -934,9 +983,12 @@ mi355q_status launch_tiles(mi355q_context* ctx, hipStream_t s, AttentionArgs a, 
         if (mi355q_status st = launch_join<HD>(s, a, rows, ROWS)) return st;
     }
     if (weights) {
-        const uint32_t tokens = kWeightWaves * 32;
-        kv_block_weights_tiles_kernel<HD><<<dim3((a.kv.max_length + tokens - 1) / tokens * a.kv.kv_heads, 1, a.kv.sequences), 64 * kWeightWaves, 0, s>>>(a);
+        kv_block_weights_tiles_kernel<HD><<<dim3(chunks * a.kv.kv_heads, a.sum_parts, a.kv.sequences), 64 * kWeightWaves, 0, s>>>(a);
         MI355Q_HIP(hipGetLastError());
+        if (a.sum_parts > 1) {
+            kv_block_weights_add_kernel<<<dim3((a.kv.max_length + 255) / 256 * a.kv.kv_heads, 1, a.kv.sequences), 256, 0, s>>>(a);
+            MI355Q_HIP(hipGetLastError());
+        }
     }
     return MI355Q_OK;
 }
