@@ -805,26 +805,14 @@ __global__ __launch_bounds__(256) void kv_block_attention_join_few_kernel(Attent
     }
 }
 
-// Joins the parts of a row: one workgroup per row, 1024 / HD parts at a time, added in a fixed order.
-template <int HD>
-__global__ __launch_bounds__(256) void kv_block_attention_join_kernel(AttentionArgs a, uint32_t tile_rows) {
-    constexpr uint32_t LANES = HD / 4, AT_ONCE = 256 / LANES;     // a thread holds four dimensions of every AT_ONCE-th part
-    __shared__ floatx4 lds_out[256];
-    __shared__ float lds_f[kMostParts];
-    const uint32_t tid = threadIdx.x, lane = tid & 63, head = blockIdx.y, b = blockIdx.z, r = blockIdx.x;
-    const KvSequence s = kv_sequence(a.kv, b);
-    const uint32_t rows = (uint32_t)s.rows * a.group;
-    if (r >= rows) return;
-    const uint32_t tile = r / tile_rows, r0 = tile * tile_rows;
-    const uint32_t parts = part_count(a, row_range(a, s, r0, min(r0 + tile_rows, rows)));
-    if (parts == 1) return;
-    const size_t slot = (((size_t)b * a.kv.kv_heads + head) * a.tiles + tile) * a.parts * tile_rows + (r - r0);
-    // every wavefront: the common maximum and the sum
+// The common maximum and the sum of a row's parts, by a wavefront: (m, l) of the row at the same units, and each part's
+// factor 2^(m_part - m) for the lanes' parts.
+__device__ __forceinline__ float2 join_sums(const float2* ml_at, uint32_t parts, uint32_t tile_rows, uint32_t lane, float (&f)[kMostParts / 64]) {
     float2 ml[kMostParts / 64];
     float top = kLowest;
 #pragma unroll
     for (uint32_t i = 0; i < kMostParts / 64; i++) {
-        ml[i] = i * 64 + lane < parts ? a.part_ml[slot + (size_t)(i * 64 + lane) * tile_rows] : make_float2(kLowest, 0.0f);
+        ml[i] = i * 64 + lane < parts ? ml_at[(size_t)(i * 64 + lane) * tile_rows] : make_float2(kLowest, 0.0f);
         top = fmaxf(top, ml[i].x);
     }
     top = max_across(top, lane);
@@ -832,11 +820,29 @@ __global__ __launch_bounds__(256) void kv_block_attention_join_kernel(AttentionA
     float l = 0.0f;
 #pragma unroll
     for (uint32_t i = 0; i < kMostParts / 64; i++) {
-        const float f = exp2f(ml[i].x - top);
-        l += ml[i].y * f;
-        if (tid < 64) lds_f[i * 64 + lane] = f;
+        f[i] = exp2f(ml[i].x - top);
+        l += ml[i].y * f[i];
     }
-    l = wave_reduce_sum(l);
+    return make_float2(top, wave_reduce_sum(l));
+}
+
+// Joins the parts of a row: one workgroup per row, 1024 / HD parts at a time, added in a fixed order.
+template <int HD>
+__device__ __forceinline__ void join_row(const AttentionArgs& a, uint32_t tile_rows, uint32_t r, uint32_t head, uint32_t b, floatx4* lds_out, float* lds_f) {
+    constexpr uint32_t LANES = HD / 4, AT_ONCE = 256 / LANES;     // a thread holds four dimensions of every AT_ONCE-th part
+    const uint32_t tid = threadIdx.x, lane = tid & 63;
+    const KvSequence s = kv_sequence(a.kv, b);
+    const uint32_t rows = (uint32_t)s.rows * a.group;
+    if (r >= rows) return;
+    const uint32_t tile = r / tile_rows, r0 = tile * tile_rows;
+    const uint32_t parts = part_count(a, row_range(a, s, r0, min(r0 + tile_rows, rows)));
+    if (parts == 1) return;
+    const size_t slot = (((size_t)b * a.kv.kv_heads + head) * a.tiles + tile) * a.parts * tile_rows + (r - r0);
+    float f[kMostParts / 64];
+    const float2 ml = join_sums(a.part_ml + slot, parts, tile_rows, lane, f);
+#pragma unroll
+    for (uint32_t i = 0; i < kMostParts / 64; i++)
+        if (tid < 64) lds_f[i * 64 + lane] = f[i];
     __syncthreads();
     floatx4 o = {0, 0, 0, 0};
     const uint32_t d = tid % LANES * 4;
@@ -850,33 +856,47 @@ __global__ __launch_bounds__(256) void kv_block_attention_join_kernel(AttentionA
     for (uint32_t i = 1; i < AT_ONCE; i++) o += lds_out[i * LANES + tid];
     const uint32_t token = r / a.group, h = head * a.group + r % a.group;
     const size_t row = (size_t)(s.row0 + (int32_t)token);
-    store_row4(a, row * a.out_stride + (size_t)h * HD + d, o, l == 0.0f ? 0.0f : 1.0f / l);
+    store_row4(a, row * a.out_stride + (size_t)h * HD + d, o, ml.y == 0.0f ? 0.0f : 1.0f / ml.y);
     if (tid == 0) {
-        const float lse2 = l == 0.0f ? -INFINITY : top + log2f(l);
+        const float lse2 = ml.y == 0.0f ? -INFINITY : ml.x + log2f(ml.y);
         if (a.lse) a.lse[row * a.heads + h] = lse2 * 0.6931471805599453f;
         if (a.lse2) a.lse2[((size_t)b * a.kv.kv_heads + head) * a.score_rows + r] = lse2;
     }
 }
 
-// Weight sums from the stored scores: four tokens a thread, over the rows of its KV head.  Scores that a row does not see
-// were stored as -inf.
-__global__ __launch_bounds__(256) void kv_block_weights_kernel(AttentionArgs a) {
-    const uint32_t head = blockIdx.x % a.kv.kv_heads, chunk = blockIdx.x / a.kv.kv_heads, b = blockIdx.z;
+// Weight sums from the stored scores of at most 32 rows: four tokens a thread, over the rows of its KV head.  Scores that a
+// row does not see were stored as -inf.  The rows' sums come from their parts, so this needs no launch of its own behind
+// the joining one.
+__device__ __forceinline__ void weigh_tokens(const AttentionArgs& a, uint32_t tile_rows, uint32_t chunk, uint32_t head, uint32_t b, float* lds_lse) {
+    const uint32_t lane = threadIdx.x & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const KvSequence s = kv_sequence(a.kv, b);
     const uint32_t rows = (uint32_t)s.rows * a.group;
     if (!rows) return;
     const RowRange g = row_range(a, s, 0, rows);
     const int32_t t = (int32_t)(chunk * 1024 + threadIdx.x * 4), j = t / (int32_t)kKvTokens;
+    if ((int32_t)(chunk * 16) >= g.last || (int32_t)(chunk * 16 + 15) < g.first) return;
+    const uint32_t parts = part_count(a, g);
+    const size_t slot = (size_t)b * a.kv.kv_heads + head;
+    for (uint32_t r = wave; r < rows; r += 4) {
+        float lse2;
+        if (parts == 1) {
+            lse2 = scalar_load(a.lse2 + slot * a.score_rows + r);
+        } else {
+            float f[kMostParts / 64];
+            const float2 ml = join_sums(a.part_ml + slot * a.parts * tile_rows + r, parts, tile_rows, lane, f);
+            lse2 = ml.y == 0.0f ? -INFINITY : ml.x + log2f(ml.y);
+        }
+        if (lane == 0) lds_lse[r] = lse2 == -INFINITY ? INFINITY : lse2;      // a row that sees nothing
+    }
+    __syncthreads();
     if (j < g.first || j >= g.last) return;
     const int32_t block = kv_block_id(a.kv, s.table, j);
-    const size_t slot = ((size_t)b * a.kv.kv_heads + head) * a.score_rows;
-    const floatx4* const scores = (const floatx4*)(a.scores + slot * a.score_stride + t);
+    const floatx4* const scores = (const floatx4*)(a.scores + slot * a.score_rows * a.score_stride + t);
     floatx4 sum = {0, 0, 0, 0};
 #pragma unroll 4
     for (uint32_t r = 0; r < rows; r++) {
         const floatx4 x = scores[(size_t)r * (a.score_stride / 4)];
-        float lse2 = scalar_load(a.lse2 + slot + r);
-        lse2 = lse2 == -INFINITY ? INFINITY : lse2;      // a row that sees nothing
+        const float lse2 = lds_lse[r];
 #pragma unroll
         for (int i = 0; i < 4; i++) sum[i] += __builtin_amdgcn_exp2f(x[i] - lse2);
     }
@@ -885,6 +905,15 @@ __global__ __launch_bounds__(256) void kv_block_weights_kernel(AttentionArgs a) 
 #pragma unroll
     for (int i = 0; i < 4; i++)
         if (t + i < s.length) at[i] += sum[i];
+}
+
+// Workgroups [0, join_rows) join a row each, the others add up weights of 1024 tokens each.
+template <int HD>
+__global__ __launch_bounds__(256) void kv_block_attention_join_kernel(AttentionArgs a, uint32_t tile_rows, uint32_t join_rows) {
+    __shared__ floatx4 lds_out[256];
+    __shared__ float lds_f[kMostParts];
+    if (blockIdx.x < join_rows) join_row<HD>(a, tile_rows, blockIdx.x, blockIdx.y, blockIdx.z, lds_out, lds_f);
+    else weigh_tokens(a, tile_rows, blockIdx.x - join_rows, blockIdx.y, blockIdx.z, lds_f);
 }
 
 namespace {
@@ -938,7 +967,7 @@ mi355q_status launch_join(hipStream_t s, const AttentionArgs& a, uint32_t rows, 
     if (a.parts <= kFewParts)
         kv_block_attention_join_few_kernel<HD><<<dim3((rows + 3) / 4, a.kv.kv_heads, a.kv.sequences), 256, 0, s>>>(a, tile_rows);
     else
-        kv_block_attention_join_kernel<HD><<<dim3(rows, a.kv.kv_heads, a.kv.sequences), 256, 0, s>>>(a, tile_rows);
+        kv_block_attention_join_kernel<HD><<<dim3(rows, a.kv.kv_heads, a.kv.sequences), 256, 0, s>>>(a, tile_rows, rows);
     MI355Q_HIP(hipGetLastError());
     return MI355Q_OK;
 }
@@ -1016,14 +1045,13 @@ mi355q_status launch_rows(mi355q_context* ctx, hipStream_t s, AttentionArgs a, b
     }
     kv_block_attention_rows_kernel<HD, RT><<<dim3(a.kv.kv_heads * a.parts, 1, a.kv.sequences), 256, 0, s>>>(a);
     MI355Q_HIP(hipGetLastError());
-    if (a.parts > 1) {
-        if (mi355q_status st = launch_join<HD>(s, a, rows, 16 * RT)) return st;
-    }
     if (weights) {
-        kv_block_weights_kernel<<<dim3((a.kv.max_length + 1023) / 1024 * a.kv.kv_heads, 1, a.kv.sequences), 256, 0, s>>>(a);
+        const uint32_t join_rows = a.parts > 1 ? rows : 0, chunks = (a.kv.max_length + 1023) / 1024;
+        kv_block_attention_join_kernel<HD><<<dim3(join_rows + chunks, a.kv.kv_heads, a.kv.sequences), 256, 0, s>>>(a, 16 * RT, join_rows);
         MI355Q_HIP(hipGetLastError());
+        return MI355Q_OK;
     }
-    return MI355Q_OK;
+    return a.parts > 1 ? launch_join<HD>(s, a, rows, 16 * RT) : MI355Q_OK;
 }
 
 }  // namespace
