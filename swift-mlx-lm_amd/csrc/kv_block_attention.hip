@@ -35,11 +35,11 @@ struct AttentionArgs {
     uint32_t tiles, parts, part_blocks;
     float* part_out;          // [slot row][HD], in units of 2^m
     float2* part_ml;          // [slot row] (m, l)
-    // weights wanted: scores in units of log2, [sequence * kv_heads + head][score_rows][score_stride], and each row's
+    // weights wanted: scores in units of log2, [sequence * kv_heads + head][score_blocks][score_rows][64], and each row's
     // log2 of the sum
     float* scores;
     float* lse2;
-    uint32_t score_rows, score_stride;
+    uint32_t score_rows, score_blocks;
     // weights of many rows: the rows as operands, [sequence * kv_heads + head][32 rows][HD / 16][lane], and their factors
     u32x4* operands;
     float* factors;
@@ -300,7 +300,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void kv_block_attention_row
 #pragma unroll
                 for (int i = 0; i < 4; i++) top = fmaxf(top, x[t][k][i]);
             if (a.scores && t * 16 + n < rows) {
-                float* const at = a.scores + ((size_t)(b * a.kv.kv_heads + head) * a.score_rows + t * 16 + n) * a.score_stride + base + c * 4;
+                float* const at = a.scores + ((((size_t)b * a.kv.kv_heads + head) * a.score_blocks + j) * a.score_rows + t * 16 + n) * kKvTokens + c * 4;
 #pragma unroll
                 for (int k = 0; k < 4; k++) *(floatx4*)(at + k * 16) = x[t][k];
             }
@@ -891,11 +891,11 @@ __device__ __forceinline__ void weigh_tokens(const AttentionArgs& a, uint32_t ti
     __syncthreads();
     if (j < g.first || j >= g.last) return;
     const int32_t block = kv_block_id(a.kv, s.table, j);
-    const floatx4* const scores = (const floatx4*)(a.scores + slot * a.score_rows * a.score_stride + t);
+    const floatx4* const scores = (const floatx4*)(a.scores + (slot * a.score_blocks + j) * a.score_rows * kKvTokens + t % (int32_t)kKvTokens);
     floatx4 sum = {0, 0, 0, 0};
 #pragma unroll 4
     for (uint32_t r = 0; r < rows; r++) {
-        const floatx4 x = scores[(size_t)r * (a.score_stride / 4)];
+        const floatx4 x = scores[r * (kKvTokens / 4)];
         const float lse2 = lds_lse[r];
 #pragma unroll
         for (int i = 0; i < 4; i++) sum[i] += __builtin_amdgcn_exp2f(x[i] - lse2);
@@ -1029,7 +1029,7 @@ mi355q_status launch_rows(mi355q_context* ctx, hipStream_t s, AttentionArgs a, b
     const uint64_t groups = (uint64_t)a.kv.kv_heads * a.kv.sequences;
     choose_parts(&a, visible_blocks(a, 16 * RT), groups, 1024, 4);
     a.score_rows = rows;
-    a.score_stride = (uint32_t)((a.kv.max_length + kKvTokens - 1) / kKvTokens * kKvTokens);
+    a.score_blocks = (a.kv.max_length + kKvTokens - 1) / kKvTokens;
     for (int pass = 0; pass < 2; pass++) {
         Buffers buf{pass ? (char*)ctx->workspace : nullptr, 0};
         if (a.parts > 1) {
@@ -1037,7 +1037,7 @@ mi355q_status launch_rows(mi355q_context* ctx, hipStream_t s, AttentionArgs a, b
             a.part_ml = buf.take<float2>(groups * a.parts * 16 * RT);
         }
         if (weights) {
-            a.scores = buf.take<float>((size_t)a.kv.sequences * a.kv.kv_heads * rows * a.score_stride);
+            a.scores = buf.take<float>((size_t)a.kv.sequences * a.kv.kv_heads * a.score_blocks * rows * kKvTokens);
             a.lse2 = buf.take<float>((size_t)a.kv.sequences * a.kv.kv_heads * rows);
         }
         if (!pass && buf.used)
