@@ -564,6 +564,28 @@ MI355Q_API mi355q_status mi355q_plan_add_output_head(mi355q_plan* plan, const mi
                                                      const void* x_dev, mi355q_dtype x_dtype,
                                                      float* logits_f32_dev, int32_t* token_out_dev,
                                                      uint32_t flags, const char* tensor_name);
+/* One step for the block cache or for token log probabilities (bindings as mi355q_kv_block_append,
+ * mi355q_kv_block_attention and mi355q_token_logprobs; the structs are copied, the tables they point to are read at every
+ * replay, so a graph built once serves a growing sequence up to the bounds it was built with).  Building the graph runs
+ * the steps once: lengths of 0 meanwhile make that pass one without effect on caches and weight sums. */
+struct mi355q_kv_block_cache;
+struct mi355q_kv_sequences;
+MI355Q_API mi355q_status mi355q_plan_add_kv_block_append(mi355q_plan* plan, const struct mi355q_kv_block_cache* cache,
+                                                         const struct mi355q_kv_sequences* sequences, const void* k_dev,
+                                                         const void* v_dev, mi355q_dtype dtype, uint32_t row_stride,
+                                                         int32_t layer_index, const char* tensor_name);
+MI355Q_API mi355q_status mi355q_plan_add_kv_block_attention(mi355q_plan* plan, const struct mi355q_kv_block_cache* cache,
+                                                            const struct mi355q_kv_sequences* sequences, const void* q_dev,
+                                                            mi355q_dtype q_dtype, uint32_t q_row_stride, uint32_t head_count,
+                                                            float scale, uint32_t window, void* out_dev,
+                                                            mi355q_dtype out_dtype, uint32_t out_row_stride, float* lse_dev,
+                                                            int accumulate_weights, int32_t layer_index,
+                                                            const char* tensor_name);
+MI355Q_API mi355q_status mi355q_plan_add_token_logprobs(mi355q_plan* plan, const void* logits_dev, mi355q_dtype dtype,
+                                                        uint32_t row_count, uint32_t vocabulary_size, uint32_t row_stride,
+                                                        const int32_t* token_ids_dev, float* logprob_dev,
+                                                        float* entropy_dev, uint32_t top_count, int32_t* top_ids_dev,
+                                                        float* top_logprobs_dev, const char* tensor_name);
 MI355Q_API int32_t mi355q_plan_step_count(const mi355q_plan* plan);
 /* The planned launch and its quantization-plan entry for step `index`; layer_index_out and
  * tensor_name_out (capacity name_cap) may be NULL. */
@@ -710,7 +732,7 @@ MI355Q_API mi355q_status mi355q_kv_cache_read(mi355q_context* ctx, void* stream,
  *   (d / 16 * 4 + t / 4 % 4) * 256 + d % 16 * 16 + t / 32 * 8 + t / 16 % 2 * 4 + t % 4: the orders in which the matrix
  *   cores take their operands, so that the attention kernels read whole cache lines and never transpose.
  * scales_dev: fp32 [block_count][kv_head_count][2], one scale for the block's keys and one for its values; a number is
- *   code * scale.
+ *   code * scale.  Scales are not negative.
  * weight_sums_dev: fp32 [block_count][kv_head_count][64], the attention weight each cached token has received (needed
  *   by mi355q_kv_block_evict and by attention with accumulate_weights; may be NULL otherwise).
  * head_dimension is 64, 128 or 256. */

@@ -206,6 +206,10 @@ def library() -> C.CDLL:
                                                   C.c_char_p]),
         "mi355q_plan_add_gated_mlp": (i32, [vp, vp, vp, vp, C.c_int, vp, C.c_int, u32, u32, u32, C.c_int, u32, i32, C.c_char_p]),
         "mi355q_plan_add_output_head": (i32, [vp, vp, vp, C.c_int, vp, vp, u32, C.c_char_p]),
+        "mi355q_plan_add_kv_block_append": (i32, [vp, P(_KvBlockCache), P(_KvSequences), vp, vp, C.c_int, u32, i32, C.c_char_p]),
+        "mi355q_plan_add_kv_block_attention": (i32, [vp, P(_KvBlockCache), P(_KvSequences), vp, C.c_int, u32, u32, C.c_float,
+                                                     u32, vp, C.c_int, u32, vp, C.c_int, i32, C.c_char_p]),
+        "mi355q_plan_add_token_logprobs": (i32, [vp, vp, C.c_int, u32, u32, u32, vp, vp, vp, u32, vp, vp, C.c_char_p]),
         "mi355q_plan_step_count": (i32, [vp]),
         "mi355q_plan_step_at": (i32, [vp, i32, P(_Step), P(i32), C.c_char_p, sz]),
         "mi355q_plan_encode": (i32, [vp, vp, u32, u32]),
@@ -488,6 +492,35 @@ class DispatchPlan:
                                                      Context._ptr(logits_f32), Context._ptr(token_out), flags,
                                                      tensor_name.encode() if tensor_name else None))
         self._keep.append((w, x, logits_f32, token_out))
+
+    def add_kv_block_append(self, cache: "KVBlockCache", sequences: "KVSequences", k, v, dtype, row_stride=0, layer_index=-1,
+                            tensor_name: str | None = None):
+        """The rows of k and v become the last tokens of their sequences (Context.kv_block_append)."""
+        _check(library().mi355q_plan_add_kv_block_append(self.handle, cache._c, sequences._c, Context._ptr(k), Context._ptr(v),
+                                                         dtype, row_stride, layer_index,
+                                                         tensor_name.encode() if tensor_name else None))
+        self._keep.append((cache, sequences, k, v))
+
+    def add_kv_block_attention(self, cache: "KVBlockCache", sequences: "KVSequences", q, q_dtype, head_count, out, out_dtype,
+                               scale, window=0, lse=None, accumulate_weights=False, q_row_stride=0, out_row_stride=0,
+                               layer_index=-1, tensor_name: str | None = None):
+        """Attention of the rows over the cached tokens of their sequences (Context.kv_block_attention)."""
+        _check(library().mi355q_plan_add_kv_block_attention(self.handle, cache._c, sequences._c, Context._ptr(q), q_dtype,
+                                                            q_row_stride, head_count, scale, window, Context._ptr(out),
+                                                            out_dtype, out_row_stride, Context._ptr(lse),
+                                                            1 if accumulate_weights else 0, layer_index,
+                                                            tensor_name.encode() if tensor_name else None))
+        self._keep.append((cache, sequences, q, out, lse))
+
+    def add_token_logprobs(self, logits, dtype, row_count, vocabulary_size, token_ids=None, top_count=0, logprob=None,
+                           entropy=None, top_ids=None, top_logprobs=None, row_stride=0, tensor_name: str | None = None):
+        """Log probability, entropy and likeliest tokens of each row (Context.token_logprobs)."""
+        _check(library().mi355q_plan_add_token_logprobs(self.handle, Context._ptr(logits), dtype, row_count, vocabulary_size,
+                                                        row_stride, Context._ptr(token_ids), Context._ptr(logprob),
+                                                        Context._ptr(entropy), top_count, Context._ptr(top_ids),
+                                                        Context._ptr(top_logprobs),
+                                                        tensor_name.encode() if tensor_name else None))
+        self._keep.append((logits, token_ids, logprob, entropy, top_ids, top_logprobs))
 
     def __len__(self):
         return library().mi355q_plan_step_count(self.handle)

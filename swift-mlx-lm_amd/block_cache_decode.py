@@ -1,0 +1,221 @@
+"""Serving loop over the 8-bit block cache: ragged prompts, then greedy decoding in a captured graph, with eviction.
+
+A small decoder stack with random 4-bit weights (projections, gated MLP and output head of the library; no norms, no
+positions) shows how the operators of the cache go together:
+
+    prompts   embedding, q+k+v, append, attention, o, gated MLP, down, head, log probabilities of the prompt's own tokens
+    a token   the same steps in a plan, captured once as a graph and replayed with longer lengths; the likeliest token of
+              each row, which token_logprobs leaves in device memory, is the next step's input
+    eviction  when the sequences reach `limit` tokens, every layer keeps the first `sinks`, the last `recent` and the
+              tokens with most attention weight, `budget` in all, in a second set of blocks, and the block table is
+              exchanged under the captured graph
+
+    python swift-mlx-lm_amd/block_cache_decode.py [--tokens N] [--eager]
+"""
+import argparse
+import importlib.util
+import os
+import sys
+import time
+
+import numpy as np
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+
+
+def load_package():
+    if "swift_mlx_lm_amd" in sys.modules:
+        return sys.modules["swift_mlx_lm_amd"]
+    spec = importlib.util.spec_from_file_location("swift_mlx_lm_amd", os.path.join(HERE, "__init__.py"),
+                                                  submodule_search_locations=[HERE])
+    mod = importlib.util.module_from_spec(spec)
+    sys.modules[spec.name] = mod
+    spec.loader.exec_module(mod)
+    return mod
+
+
+class BlockCacheDecoder:
+    """`sequences` sequences of up to `limit` tokens (a multiple of the block) with one cache per layer."""
+
+    def __init__(self, pkg, ctx, sequences=4, limit=512, budget=256, sinks=4, recent=64, layers=2, hidden=1024, heads=16,
+                 kv_heads=4, head_dimension=64, inner=2048, vocabulary=4096, seed=0):
+        if limit % pkg.KV_BLOCK_TOKENS or not 0 < budget < limit:
+            raise ValueError("the limit must be whole blocks and the budget below it")
+        self.pkg, self.ctx, self.count, self.limit, self.vocabulary = pkg, ctx, sequences, limit, vocabulary
+        self.budget, self.sinks, self.recent = budget, sinks, recent
+        self.hidden, self.heads, self.kv_heads, self.head_dimension, self.inner = hidden, heads, kv_heads, head_dimension, inner
+        self.rng = np.random.default_rng(seed)
+        self.embedding, self.head = self._weight(vocabulary, hidden, 32.0), self._weight(vocabulary, hidden, 4.0)
+        width, kv_width = heads * head_dimension, kv_heads * head_dimension
+        self.layers = [dict(q=self._weight(width, hidden), k=self._weight(kv_width, hidden), v=self._weight(kv_width, hidden),
+                            o=self._weight(hidden, width, 2.0), gate=self._weight(inner, hidden), up=self._weight(inner, hidden),
+                            down=self._weight(hidden, inner, 2.0)) for _ in range(layers)]
+        # every sequence owns two sets of blocks and uses one: eviction moves what it keeps to the other
+        self.blocks = limit // pkg.KV_BLOCK_TOKENS
+        total = 2 * sequences * self.blocks
+        self.tables = np.arange(total, dtype=np.int32).reshape(2, sequences, self.blocks)
+        self.caches = []
+        for _ in range(layers):
+            codes = self._zeros(pkg.KVBlockCache.codes_bytes(kv_heads, head_dimension, total))
+            scales = self._zeros(pkg.KVBlockCache.scales_bytes(kv_heads, total))
+            sums = self._zeros(pkg.KVBlockCache.weight_sums_bytes(kv_heads, total))
+            self.caches.append(pkg.KVBlockCache(kv_heads, head_dimension, total, codes, scales, sums))
+        self.lengths = np.zeros(sequences, np.int32)
+        self.table_dev, self.spare_dev = ctx.upload(self.tables[0]), ctx.upload(self.tables[1])
+        self.lengths_dev, self.evicted_dev = ctx.upload(self.lengths), ctx.alloc(4 * sequences)
+        self.stream = ctx.stream_create()
+        self.plan = None
+        self.evictions = 0
+
+    def _zeros(self, nbytes):
+        buf = self.ctx.alloc(nbytes)
+        self.ctx.fill(buf, 0)
+        return buf
+
+    def _weight(self, n, k, gain=1.0):
+        """Uniform random 4-bit codes, scaled so that unit rows come out with a standard deviation of `gain`."""
+        fmt = self.pkg.QuantizationFormatRegistry.format_for_mlx_quantization(4, 64)
+        words = self.rng.integers(0, 1 << 32, (n, k // 8), dtype=np.uint64).astype(np.uint32)
+        scale = np.float32(gain / (4.61 * k ** 0.5))
+        scales = np.full((n, k // 64), scale, np.float32)
+        return self.ctx.weight_prepare_mlx(fmt, words, scales.astype(np.float16).view(np.uint16),
+                                           (scales * np.float32(-7.5)).astype(np.float16).view(np.uint16), self.pkg.F16)
+
+    def _rows(self, rows):
+        """Activation buffers for `rows` rows."""
+        widths = dict(x=self.hidden, q=self.heads * self.head_dimension, k=self.kv_heads * self.head_dimension,
+                      v=self.kv_heads * self.head_dimension, attended=self.heads * self.head_dimension, mixed=self.hidden,
+                      inner=self.inner)
+        buffers = {name: self.ctx.alloc(rows * width * 2) for name, width in widths.items()}
+        buffers["logits"] = self.ctx.alloc(rows * self.vocabulary * 4)
+        return buffers
+
+    def _sequences(self, starts, rows, maximum_rows):
+        starts_dev = self.ctx.upload(np.asarray(starts, np.int32))
+        return self.pkg.KVSequences(self.count, self.table_dev, self.blocks, self.lengths_dev, starts_dev, rows, maximum_rows,
+                                    self.limit)
+
+    def _record(self, rows, seq, b):
+        """The steps of one pass over all layers for `rows` rows, behind the embedding."""
+        pkg, plan = self.pkg, self.pkg.DispatchPlan(self.ctx)
+        t = pkg.BF16
+        for i, (w, cache) in enumerate(zip(self.layers, self.caches)):
+            plan.add_batched_linear([w["q"], w["k"], w["v"]], b["x"], t, [b["q"], b["k"], b["v"]], t, rows, layer_index=i)
+            plan.add_kv_block_append(cache, seq, b["k"], b["v"], t, layer_index=i)
+            plan.add_kv_block_attention(cache, seq, b["q"], t, self.heads, b["attended"], t, self.head_dimension ** -0.5,
+                                        accumulate_weights=True, layer_index=i)
+            plan.add_linear(w["o"], b["attended"], t, b["mixed"], t, rows, layer_index=i)
+            plan.add_gated_mlp(w["gate"], w["up"], b["mixed"], t, b["inner"], t, rows, layer_index=i)
+            plan.add_linear(w["down"], b["inner"], t, b["x"], t, rows, layer_index=i)
+        plan.add_linear(self.head, b["x"], t, b["logits"], pkg.F32, rows)
+        return plan
+
+    def prompts(self, prompts, alternatives=4):
+        """Takes the sequences' prompts (lists of token ids) into the cache and scores them.  Returns, for the rows of all
+        prompts behind one another, the log probability of each row's next prompt token (0 for a prompt's last row), the
+        entropy, and the likeliest tokens; decoding goes on from the likeliest token of each prompt's last row."""
+        if len(prompts) != self.count or any(not 0 < len(p) < self.limit for p in prompts):
+            raise ValueError("one prompt of at least one and fewer than `limit` tokens for every sequence")
+        ctx, pkg = self.ctx, self.pkg
+        starts = np.cumsum([0] + [len(p) for p in prompts]).astype(np.int32)
+        rows = int(starts[-1])
+        self.lengths[:] = [len(p) for p in prompts]
+        self.lengths_dev.upload(self.lengths)
+        buffers, seq = self._rows(rows), self._sequences(starts, rows, max(len(p) for p in prompts))
+        plan = self._record(rows, seq, buffers)
+        ids = ctx.upload(np.concatenate(prompts).astype(np.int32))
+        following = np.concatenate([list(p[1:]) + [-1] for p in prompts]).astype(np.int32)
+        following_dev, logprob, entropy = ctx.upload(following), ctx.alloc(rows * 4), ctx.alloc(rows * 4)
+        top_ids, top_logprobs = ctx.alloc(rows * alternatives * 4), ctx.alloc(rows * alternatives * 4)
+        plan.add_token_logprobs(buffers["logits"], pkg.F32, rows, self.vocabulary, following_dev, alternatives, logprob, entropy,
+                                top_ids, top_logprobs)
+        ctx.embedding_lookup(self.embedding, ids, rows, buffers["x"], pkg.BF16, stream=self.stream)
+        plan.encode(self.stream)
+        ctx.synchronize(self.stream)
+        plan.destroy()
+        logprobs = np.where(following < 0, 0, logprob.download(np.float32))
+        tops = top_ids.download(np.int32, (rows, alternatives))
+        result = logprobs, entropy.download(np.float32), tops, top_logprobs.download(np.float32, (rows, alternatives))
+        self.next = np.ascontiguousarray(tops[starts[1:] - 1, 0])
+        for buf in list(buffers.values()) + [ids, following_dev, logprob, entropy, top_ids, top_logprobs]:
+            buf.free()
+        return result
+
+    def _prepare(self, graph):
+        """The decode step's plan, one row a sequence.  Lengths of 0 keep the pass that building the graph makes from
+        touching the caches."""
+        ctx, pkg = self.ctx, self.pkg
+        self.buffers = self._rows(self.count)
+        self.seq = self._sequences(range(self.count + 1), self.count, 1)
+        self.ids, self.chosen, self.entropy = ctx.alloc(self.count * 4), ctx.alloc(self.count * 4), ctx.alloc(self.count * 4)
+        self.plan = self._record(self.count, self.seq, self.buffers)
+        self.plan.add_token_logprobs(self.buffers["logits"], pkg.F32, self.count, self.vocabulary, top_count=1,
+                                     entropy=self.entropy, top_ids=self.ids, top_logprobs=self.chosen)
+        if graph:
+            self.lengths_dev.upload(np.zeros(self.count, np.int32))
+            ctx.embedding_lookup(self.embedding, ctx.upload(self.next), self.count, self.buffers["x"], pkg.BF16, stream=self.stream)
+            self.plan.graph_build(self.stream)
+            ctx.synchronize(self.stream)
+        self.replay = self.plan.graph_launch if graph else self.plan.encode
+        self.ids.upload(self.next)
+
+    def evict(self):
+        """Every layer down to the budget, into the blocks that are free; the table changes under the captured graph."""
+        spare = 1 - self.evictions % 2
+        for cache in self.caches:
+            self.ctx.kv_block_evict(cache, self.seq, self.budget, self.spare_dev, self.blocks, self.evicted_dev, self.recent,
+                                    self.sinks, stream=self.stream)
+        self.ctx.synchronize(self.stream)
+        self.lengths[:] = self.evicted_dev.download(np.int32)
+        self.table_dev.upload(self.tables[spare])
+        self.spare_dev.upload(self.tables[1 - spare])
+        self.evictions += 1
+
+    def step(self, graph=True):
+        """One token for every sequence.  Returns the tokens, their log probabilities and the entropies."""
+        if self.plan is None:
+            self._prepare(graph)
+        if self.lengths.max() == self.limit:
+            self.lengths_dev.upload(self.lengths)
+            self.evict()
+        self.lengths += 1
+        self.lengths_dev.upload(self.lengths)
+        self.ctx.embedding_lookup(self.embedding, self.ids, self.count, self.buffers["x"], self.pkg.BF16, stream=self.stream)
+        self.replay(self.stream)
+        self.ctx.synchronize(self.stream)
+        return self.ids.download(np.int32), self.chosen.download(np.float32), self.entropy.download(np.float32)
+
+    def close(self):
+        if self.plan is not None:
+            self.plan.destroy()
+            self.plan = None
+        self.ctx.synchronize(self.stream)
+        self.ctx.stream_destroy(self.stream)
+
+
+def main():
+    ap = argparse.ArgumentParser()
+    ap.add_argument("--tokens", type=int, default=400, help="tokens to decode for every sequence")
+    ap.add_argument("--eager", action="store_true", help="launch the plan's steps one by one, without a graph")
+    a = ap.parse_args()
+    pkg = load_package()
+    ctx = pkg.Context(0)
+    decoder = BlockCacheDecoder(pkg, ctx)
+    prompts = [decoder.rng.integers(0, decoder.vocabulary, n) for n in (300, 7, 129, 450)]
+    logprobs, entropy, _, _ = decoder.prompts(prompts)
+    print(f"prompts of {[len(p) for p in prompts]} tokens: {-logprobs.sum():.1f} nats, mean entropy {entropy.mean():.3f}")
+    decoder.step(not a.eager)
+    start = time.perf_counter()
+    for _ in range(a.tokens - 1):
+        tokens, chosen, entropy = decoder.step(not a.eager)
+    seconds = time.perf_counter() - start
+    print(f"{a.tokens} tokens a sequence, {decoder.evictions} evictions, lengths {decoder.lengths.tolist()}, "
+          f"{1e6 * seconds / max(1, a.tokens - 1):.0f} us a step")
+    print(f"last tokens {tokens.tolist()}, log probabilities {[f'{x:.3f}' for x in chosen]}, "
+          f"entropies {[f'{x:.3f}' for x in entropy]}")
+    decoder.close()
+    ctx.close()
+
+
+if __name__ == "__main__":
+    main()

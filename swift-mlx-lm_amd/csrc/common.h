@@ -497,6 +497,22 @@ bool gemm_two_step_eligible(const WView& w, int x_dtype, uint32_t m, uint32_t x_
 bool gemm_two_step_chosen(const WView& w, int x_dtype, uint32_t m, uint32_t x_stride, uint32_t flags);
 mi355q_status launch_qgemm_two_step(hipStream_t s, mi355q_context* ctx, const WView& w, const void* x, int x_dtype,
                                     void* y, int y_dtype, uint32_t m, uint32_t x_stride, uint32_t y_stride);
+// Block KV cache and token log probabilities (kv_block_cache.hip, kv_block_attention.hip, token_logprobs.hip): what the
+// entry points and the plan steps run.  `run` false: the checks alone; `record` (or null) gets the launch.
+mi355q_status dispatch_kv_block_append(mi355q_context* ctx, hipStream_t s, const mi355q_kv_block_cache* cache,
+                                       const mi355q_kv_sequences* sequences, const void* k, const void* v, int dtype,
+                                       uint32_t row_stride, bool run, mi355q_step* record);
+mi355q_status dispatch_kv_block_attention(mi355q_context* ctx, hipStream_t s, const mi355q_kv_block_cache* cache,
+                                          const mi355q_kv_sequences* sequences, const void* q, int q_dtype, uint32_t q_stride,
+                                          uint32_t head_count, float scale, uint32_t window, void* out, int out_dtype,
+                                          uint32_t out_stride, float* lse, bool weights, bool run, mi355q_step* record);
+mi355q_status dispatch_token_logprobs(mi355q_context* ctx, hipStream_t s, const void* logits, int dtype, uint32_t rows,
+                                      uint32_t vocabulary, uint32_t row_stride, const int32_t* tokens, float* logprob,
+                                      float* entropy, uint32_t top, int32_t* top_ids, float* top_logprobs, bool run,
+                                      mi355q_step* record);
+// fills the fields of a step that is no projection
+void describe_step(mi355q_step* record, const char* name, const char* kernel, uint32_t grid_x, uint32_t grid_y, uint32_t grid_z,
+                   uint32_t block, uint32_t lds_bytes);
 mi355q_status launch_gemm_bf16_mfma(hipStream_t s, mi355q_context* ctx, const void* a,
                                     int a_dtype, const uint16_t* b, void* c, int c_dtype,
                                     uint32_t m, uint32_t n, uint32_t k, uint32_t a_stride,

@@ -973,7 +973,7 @@ mi355q_status launch_join(hipStream_t s, const AttentionArgs& a, uint32_t rows, 
 }
 
 template <int HD>
-mi355q_status launch_tiles(mi355q_context* ctx, hipStream_t s, AttentionArgs a, bool weights) {
+mi355q_status launch_tiles(mi355q_context* ctx, hipStream_t s, AttentionArgs a, bool weights, bool run, mi355q_step* record) {
     constexpr int TS = HD == 256 ? 2 : 1;
     constexpr uint32_t ROWS = kTileRows;
     const uint32_t rows = a.kv.max_rows * a.group;
@@ -981,6 +981,12 @@ mi355q_status launch_tiles(mi355q_context* ctx, hipStream_t s, AttentionArgs a, 
     const uint64_t groups = (uint64_t)a.kv.kv_heads * a.tiles * a.kv.sequences;
     choose_tile_parts(&a, HD, visible_blocks(a, ROWS), groups);
     a.score_rows = rows;
+    // (two halves of a block's tokens add up in the room of the blocks: two rows of 64 numbers more)
+    constexpr size_t room = 2 * sizeof(TileLds<HD, 4 * TS>), lds = TS == 1 ? room : std::max(room, (size_t)4 * (HD / 2 + 2) * 256);
+    if (record)
+        describe_step(record, "kv_block_attention", "kv_block_attention_tiles", a.kv.kv_heads * a.parts, a.tiles, a.kv.sequences, 256 * TS, (uint32_t)lds);
+    if (!run) return MI355Q_OK;
+    MI355Q_HIP(hipSetDevice(ctx->device));
     // shares of the rows for the weight sums: about three workgroups a CU, each with eight tiles of 32 rows at least
     const uint32_t tokens = kWeightWaves * 32, chunks = (a.kv.max_length + tokens - 1) / tokens;
     const uint64_t owners = (uint64_t)chunks * a.kv.kv_heads * a.kv.sequences;
@@ -1003,8 +1009,6 @@ mi355q_status launch_tiles(mi355q_context* ctx, hipStream_t s, AttentionArgs a, 
         if (!pass && buf.used)
             if (mi355q_status st = ensure_workspace(ctx, buf.used)) return st;
     }
-    // (two halves of a block's tokens add up in the room of the blocks: two rows of 64 numbers more)
-    constexpr size_t blocks = 2 * sizeof(TileLds<HD, 4 * TS>), lds = TS == 1 ? blocks : std::max(blocks, (size_t)4 * (HD / 2 + 2) * 256);
     if (mi355q_status st = raise_lds_limit((const void*)kv_block_attention_tiles_kernel<HD, TS>, lds)) return st;
     kv_block_attention_tiles_kernel<HD, TS><<<dim3(a.kv.kv_heads * a.parts, a.tiles, a.kv.sequences), 256 * TS, lds, s>>>(a);
     MI355Q_HIP(hipGetLastError());
@@ -1023,11 +1027,15 @@ mi355q_status launch_tiles(mi355q_context* ctx, hipStream_t s, AttentionArgs a, 
 }
 
 template <int HD, int RT>
-mi355q_status launch_rows(mi355q_context* ctx, hipStream_t s, AttentionArgs a, bool weights) {
+mi355q_status launch_rows(mi355q_context* ctx, hipStream_t s, AttentionArgs a, bool weights, bool run, mi355q_step* record) {
     const uint32_t rows = a.kv.max_rows * a.group;
     a.tiles = 1;
     const uint64_t groups = (uint64_t)a.kv.kv_heads * a.kv.sequences;
     choose_parts(&a, visible_blocks(a, 16 * RT), groups, 1024, 4);
+    if (record)
+        describe_step(record, "kv_block_attention", "kv_block_attention_rows", a.kv.kv_heads * a.parts, 1, a.kv.sequences, 256, 2 * 16 * RT * HD * 4);
+    if (!run) return MI355Q_OK;
+    MI355Q_HIP(hipSetDevice(ctx->device));
     a.score_rows = rows;
     a.score_blocks = (a.kv.max_length + kKvTokens - 1) / kKvTokens;
     for (int pass = 0; pass < 2; pass++) {
@@ -1055,6 +1063,42 @@ mi355q_status launch_rows(mi355q_context* ctx, hipStream_t s, AttentionArgs a, b
 }
 
 }  // namespace
+
+mi355q_status dispatch_kv_block_attention(mi355q_context* ctx, hipStream_t s, const mi355q_kv_block_cache* cache,
+                                          const mi355q_kv_sequences* sequences, const void* q, int q_dtype, uint32_t q_stride,
+                                          uint32_t head_count, float scale, uint32_t window, void* out, int out_dtype,
+                                          uint32_t out_stride, float* lse, bool weights, bool run, mi355q_step* record) {
+    AttentionArgs a{};
+    if (mi355q_status st = kv_block_prepare(ctx, cache, sequences, true, &a.kv)) return st;
+    if (!q || !out) return fail(MI355Q_ERR_INVALID_ARGUMENT, "null queries or output");
+    if ((q_dtype != MI355Q_F16 && q_dtype != MI355Q_BF16) || (out_dtype != MI355Q_F16 && out_dtype != MI355Q_BF16))
+        return fail(MI355Q_ERR_INVALID_ARGUMENT, "attention takes and gives f16 or bf16 rows (got types %d and %d)", q_dtype, out_dtype);
+    if (!head_count || head_count % a.kv.kv_heads)
+        return fail(MI355Q_ERR_SHAPE, "%u query heads do not share %u KV heads evenly", head_count, a.kv.kv_heads);
+    if (head_count > 32767) return fail(MI355Q_ERR_SHAPE, "%u query heads: at most 32767", head_count);
+    if ((uint64_t)a.kv.max_rows * (head_count / a.kv.kv_heads) > (1u << 22))
+        return fail(MI355Q_ERR_SHAPE, "%u rows of %u heads share a KV head: at most 2^22 together", a.kv.max_rows, head_count / a.kv.kv_heads);
+    const uint64_t width = (uint64_t)head_count * cache->head_dimension;
+    if (q_stride == 0) q_stride = (uint32_t)width;
+    if (out_stride == 0) out_stride = (uint32_t)width;
+    if (q_stride < width || out_stride < width)
+        return fail(MI355Q_ERR_SHAPE, "row strides %u and %u: shorter than heads x head dimension = %llu", q_stride, out_stride, (unsigned long long)width);
+    if (!(scale > 0.0f) || scale > 1e30f) return fail(MI355Q_ERR_INVALID_ARGUMENT, "the scale must be a positive number (got %g)", (double)scale);
+    if ((uintptr_t)q % 2 || (uintptr_t)out % 2 || (uintptr_t)lse % 4) return fail(MI355Q_ERR_INVALID_ARGUMENT, "misaligned pointer");
+    if (weights && !a.kv.sums) return fail(MI355Q_ERR_INVALID_ARGUMENT, "the cache has no weight sums to add to");
+    a.q = q; a.out = out; a.lse = lse;
+    a.q_stride = q_stride; a.out_stride = out_stride;
+    a.q_aligned = (uintptr_t)q % 16 == 0 && q_stride % 8 == 0;
+    a.heads = head_count; a.group = head_count / a.kv.kv_heads; a.window = window;
+    a.q_dtype = (uint32_t)q_dtype; a.out_dtype = (uint32_t)out_dtype; a.scale_log2 = scale * 1.4426950408889634f;
+    return kv_with_head_dimension(cache->head_dimension, [&](auto hd) -> mi355q_status {
+        constexpr int HD = decltype(hd)::value;
+        const uint32_t rows = a.kv.max_rows * a.group;
+        if (rows <= 16) return launch_rows<HD, 1>(ctx, s, a, weights, run, record);
+        if (HD < 256 && rows <= 32) return launch_rows<HD < 256 ? HD : 64, 2>(ctx, s, a, weights, run, record);
+        return launch_tiles<HD>(ctx, s, a, weights, run, record);
+    });
+}
 }  // namespace mi355q
 
 using namespace mi355q;
@@ -1064,37 +1108,9 @@ extern "C" mi355q_status mi355q_kv_block_attention(mi355q_context* ctx, void* st
                                                    mi355q_dtype q_dtype, uint32_t q_row_stride, uint32_t head_count,
                                                    float scale, uint32_t window, void* out_dev, mi355q_dtype out_dtype,
                                                    uint32_t out_row_stride, float* lse_dev, int accumulate_weights) {
-    AttentionArgs a{};
-    if (mi355q_status st = kv_block_prepare(ctx, cache, sequences, true, &a.kv)) return st;
-    if (!q_dev || !out_dev) return fail(MI355Q_ERR_INVALID_ARGUMENT, "null queries or output");
-    if ((q_dtype != MI355Q_F16 && q_dtype != MI355Q_BF16) || (out_dtype != MI355Q_F16 && out_dtype != MI355Q_BF16))
-        return fail(MI355Q_ERR_INVALID_ARGUMENT, "attention takes and gives f16 or bf16 rows (got types %d and %d)", (int)q_dtype, (int)out_dtype);
-    if (!head_count || head_count % a.kv.kv_heads)
-        return fail(MI355Q_ERR_SHAPE, "%u query heads do not share %u KV heads evenly", head_count, a.kv.kv_heads);
-    if (head_count > 32767) return fail(MI355Q_ERR_SHAPE, "%u query heads: at most 32767", head_count);
-    if ((uint64_t)a.kv.max_rows * (head_count / a.kv.kv_heads) > (1u << 22))
-        return fail(MI355Q_ERR_SHAPE, "%u rows of %u heads share a KV head: at most 2^22 together", a.kv.max_rows, head_count / a.kv.kv_heads);
-    const uint64_t width = (uint64_t)head_count * cache->head_dimension;
-    if (q_row_stride == 0) q_row_stride = (uint32_t)width;
-    if (out_row_stride == 0) out_row_stride = (uint32_t)width;
-    if (q_row_stride < width || out_row_stride < width)
-        return fail(MI355Q_ERR_SHAPE, "row strides %u and %u: shorter than heads x head dimension = %llu", q_row_stride, out_row_stride, (unsigned long long)width);
-    if (!(scale > 0.0f) || scale > 1e30f) return fail(MI355Q_ERR_INVALID_ARGUMENT, "the scale must be a positive number (got %g)", (double)scale);
-    if ((uintptr_t)q_dev % 2 || (uintptr_t)out_dev % 2 || (uintptr_t)lse_dev % 4) return fail(MI355Q_ERR_INVALID_ARGUMENT, "misaligned pointer");
-    if (accumulate_weights && !a.kv.sums) return fail(MI355Q_ERR_INVALID_ARGUMENT, "the cache has no weight sums to add to");
-    MI355Q_HIP(hipSetDevice(ctx->device));
     ScratchGuard guard(ctx, (hipStream_t)stream);
     if (guard.status) return guard.status;
-    a.q = q_dev; a.out = out_dev; a.lse = lse_dev;
-    a.q_stride = q_row_stride; a.out_stride = out_row_stride;
-    a.q_aligned = (uintptr_t)q_dev % 16 == 0 && q_row_stride % 8 == 0;
-    a.heads = head_count; a.group = head_count / a.kv.kv_heads; a.window = window;
-    a.q_dtype = (uint32_t)q_dtype; a.out_dtype = (uint32_t)out_dtype; a.scale_log2 = scale * 1.4426950408889634f;
-    return kv_with_head_dimension(cache->head_dimension, [&](auto hd) -> mi355q_status {
-        constexpr int HD = decltype(hd)::value;
-        const uint32_t rows = a.kv.max_rows * a.group;
-        if (rows <= 16) return launch_rows<HD, 1>(ctx, (hipStream_t)stream, a, accumulate_weights != 0);
-        if (HD < 256 && rows <= 32) return launch_rows<HD < 256 ? HD : 64, 2>(ctx, (hipStream_t)stream, a, accumulate_weights != 0);
-        return launch_tiles<HD>(ctx, (hipStream_t)stream, a, accumulate_weights != 0);
-    });
+    return dispatch_kv_block_attention(ctx, (hipStream_t)stream, cache, sequences, q_dev, (int)q_dtype, q_row_stride, head_count,
+                                       scale, window, out_dev, (int)out_dtype, out_row_stride, lse_dev, accumulate_weights != 0,
+                                       true, nullptr);
 }

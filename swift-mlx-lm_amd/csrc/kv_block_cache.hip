@@ -555,6 +555,29 @@ mi355q_status check_rows(const KvBlockArgs& a, uint32_t hd, const void* k, const
 }
 
 }  // namespace
+
+mi355q_status dispatch_kv_block_append(mi355q_context* ctx, hipStream_t s, const mi355q_kv_block_cache* cache,
+                                       const mi355q_kv_sequences* sequences, const void* k, const void* v, int dtype,
+                                       uint32_t row_stride, bool run, mi355q_step* record) {
+    KvBlockArgs a;
+    bool vec;
+    if (mi355q_status st = kv_block_prepare(ctx, cache, sequences, true, &a)) return st;
+    if (mi355q_status st = check_rows(a, cache->head_dimension, k, v, dtype, &row_stride, &vec)) return st;
+    // blocks that `rows` consecutive tokens can touch: one more than they fill, if they start behind a block's first
+    const uint32_t rows = a.max_rows < a.max_length ? a.max_rows : a.max_length;
+    const dim3 grid((rows + kKvTokens - 2) / kKvTokens + 1, 2 * a.kv_heads, a.sequences);
+    return kv_with_head_dimension(cache->head_dimension, [&](auto hd) -> mi355q_status {
+        constexpr int HD = decltype(hd)::value;
+        if (record) describe_step(record, "kv_block_append", "kv_block_append", grid.x, grid.y, grid.z, 2 * HD, kKvLdsBytes<HD>);
+        if (!run) return MI355Q_OK;
+        MI355Q_HIP(hipSetDevice(ctx->device));
+        if (dtype == MI355Q_F32) kv_block_append_kernel<HD, MI355Q_F32><<<grid, 2 * HD, 0, s>>>(a, k, v, row_stride, vec);
+        else if (dtype == MI355Q_BF16) kv_block_append_kernel<HD, MI355Q_BF16><<<grid, 2 * HD, 0, s>>>(a, k, v, row_stride, vec);
+        else kv_block_append_kernel<HD, MI355Q_F16><<<grid, 2 * HD, 0, s>>>(a, k, v, row_stride, vec);
+        MI355Q_HIP(hipGetLastError());
+        return MI355Q_OK;
+    });
+}
 }  // namespace mi355q
 
 using namespace mi355q;
@@ -564,23 +587,7 @@ extern "C" {
 mi355q_status mi355q_kv_block_append(mi355q_context* ctx, void* stream, const mi355q_kv_block_cache* cache,
                                      const mi355q_kv_sequences* sequences, const void* k_dev, const void* v_dev,
                                      mi355q_dtype dtype, uint32_t row_stride) {
-    KvBlockArgs a;
-    bool vec;
-    if (mi355q_status st = kv_block_prepare(ctx, cache, sequences, true, &a)) return st;
-    if (mi355q_status st = check_rows(a, cache->head_dimension, k_dev, v_dev, (int)dtype, &row_stride, &vec)) return st;
-    MI355Q_HIP(hipSetDevice(ctx->device));
-    // blocks that `rows` consecutive tokens can touch: one more than they fill, if they start behind a block's first
-    const uint32_t rows = a.max_rows < a.max_length ? a.max_rows : a.max_length;
-    const dim3 grid((rows + kKvTokens - 2) / kKvTokens + 1, 2 * a.kv_heads, a.sequences);
-    return kv_with_head_dimension(cache->head_dimension, [&](auto hd) -> mi355q_status {
-        constexpr int HD = decltype(hd)::value;
-        const hipStream_t s = (hipStream_t)stream;
-        if (dtype == MI355Q_F32) kv_block_append_kernel<HD, MI355Q_F32><<<grid, 2 * HD, 0, s>>>(a, k_dev, v_dev, row_stride, vec);
-        else if (dtype == MI355Q_BF16) kv_block_append_kernel<HD, MI355Q_BF16><<<grid, 2 * HD, 0, s>>>(a, k_dev, v_dev, row_stride, vec);
-        else kv_block_append_kernel<HD, MI355Q_F16><<<grid, 2 * HD, 0, s>>>(a, k_dev, v_dev, row_stride, vec);
-        MI355Q_HIP(hipGetLastError());
-        return MI355Q_OK;
-    });
+    return dispatch_kv_block_append(ctx, (hipStream_t)stream, cache, sequences, k_dev, v_dev, (int)dtype, row_stride, true, nullptr);
 }
 
 mi355q_status mi355q_kv_block_read(mi355q_context* ctx, void* stream, const mi355q_kv_block_cache* cache,

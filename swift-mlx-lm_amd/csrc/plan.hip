@@ -1,6 +1,7 @@
 // Dispatch plan: an ordered list of projection steps built once and replayed per token, the
 // stand-in for MetalDispatchPlan + MetalDecodeEncoder.encodeSteps
 // (Sources/MetalCompiler/Execution/MetalDecodePlan.swift:6-140, MetalDecodeEncoder.swift:18-36).
+#include <functional>
 #include <new>
 #include <string>
 #include <vector>
@@ -12,7 +13,7 @@ using namespace mi355q;
 
 namespace {
 
-enum StepKind { kLinear = 0, kOutputHead = 1, kBatched = 2, kGated = 3 };
+enum StepKind { kLinear = 0, kOutputHead = 1, kBatched = 2, kGated = 3, kCall = 4 };
 
 struct PlanStep {
     StepKind kind;
@@ -30,6 +31,8 @@ struct PlanStep {
     const mi355q_weight* ws[3];
     void* ysv[3];
     int activation;     // kGated: ws[0] = gate_proj, ws[1] = up_proj, y = the one output
+    // kCall: a step that is no projection, with its arguments; (stream, run, record) as the dispatch functions take them
+    std::function<mi355q_status(hipStream_t, bool, mi355q_step*)> call;
 };
 
 }  // namespace
@@ -61,6 +64,8 @@ mi355q_status encode_range(mi355q_plan* plan, hipStream_t s, uint32_t first, uin
         else if (st.kind == kBatched)
             rc = dispatch_batched(plan->ctx, s, st.count, st.ws, st.x, st.x_dtype, st.ysv, st.y_dtype, st.m, st.xs,
                                   st.flags);
+        else if (st.kind == kCall)
+            rc = st.call(s, true, nullptr);
         else
             rc = dispatch_output_head(plan->ctx, s, st.w, st.x, st.x_dtype, (float*)st.y, st.token, st.flags,
                                       HeadKeys{plan->ctx->argmax_partials, kArgmaxPartialCapacity});
@@ -69,7 +74,37 @@ mi355q_status encode_range(mi355q_plan* plan, hipStream_t s, uint32_t first, uin
     return MI355Q_OK;
 }
 
+// A step that is no projection: checked now, run at every replay.
+mi355q_status add_call(mi355q_plan* plan, int32_t layer_index, const char* tensor_name, uint32_t rows,
+                       std::function<mi355q_status(hipStream_t, bool, mi355q_step*)> call) {
+    if (plan->graph_exec) return fail(MI355Q_ERR_INVALID_ARGUMENT, "plan is frozen: its graph has been built");
+    PlanStep st{};
+    st.kind = kCall;
+    if (mi355q_status rc = call(nullptr, false, &st.record)) return rc;
+    st.m = rows;
+    st.record.path = rows <= 8 ? MI355Q_PATH_DECODE_PROJECTION : MI355Q_PATH_PREFILL_PROJECTION;
+    st.record.sequence_length = rows;
+    st.layer_index = layer_index;
+    if (tensor_name) st.tensor_name = tensor_name;
+    st.call = std::move(call);
+    plan->steps.push_back(std::move(st));
+    return MI355Q_OK;
+}
+
 }  // namespace
+
+namespace mi355q {
+void describe_step(mi355q_step* record, const char* name, const char* kernel, uint32_t grid_x, uint32_t grid_y, uint32_t grid_z,
+                   uint32_t block, uint32_t lds_bytes) {
+    std::memset(record, 0, sizeof *record);
+    std::snprintf(record->kernel_name, sizeof record->kernel_name, "%s", name);
+    std::snprintf(record->device_kernel, sizeof record->device_kernel, "%s", kernel);
+    std::snprintf(record->kernel_family, sizeof record->kernel_family, "%s", name);
+    record->grid[0] = grid_x; record->grid[1] = grid_y; record->grid[2] = grid_z;
+    record->block[0] = block; record->block[1] = record->block[2] = 1;
+    record->lds_bytes = lds_bytes;
+}
+}  // namespace mi355q
 
 extern "C" {
 
@@ -280,6 +315,45 @@ mi355q_status mi355q_plan_add_output_head(mi355q_plan* plan, const mi355q_weight
     st.record = two[0];
     plan->steps.push_back(st);
     return MI355Q_OK;
+}
+
+mi355q_status mi355q_plan_add_kv_block_append(mi355q_plan* plan, const mi355q_kv_block_cache* cache,
+                                              const mi355q_kv_sequences* sequences, const void* k_dev, const void* v_dev,
+                                              mi355q_dtype dtype, uint32_t row_stride, int32_t layer_index,
+                                              const char* tensor_name) {
+    if (!plan) return fail(MI355Q_ERR_NULL_HANDLE, "plan is null");
+    if (!cache || !sequences) return fail(MI355Q_ERR_INVALID_ARGUMENT, "null cache or sequences");
+    return add_call(plan, layer_index, tensor_name, sequences->maximum_rows,
+                    [ctx = plan->ctx, c = *cache, q = *sequences, k_dev, v_dev, dtype, row_stride](hipStream_t s, bool run, mi355q_step* record) {
+                        return dispatch_kv_block_append(ctx, s, &c, &q, k_dev, v_dev, (int)dtype, row_stride, run, record);
+                    });
+}
+
+mi355q_status mi355q_plan_add_kv_block_attention(mi355q_plan* plan, const mi355q_kv_block_cache* cache,
+                                                 const mi355q_kv_sequences* sequences, const void* q_dev,
+                                                 mi355q_dtype q_dtype, uint32_t q_row_stride, uint32_t head_count, float scale,
+                                                 uint32_t window, void* out_dev, mi355q_dtype out_dtype,
+                                                 uint32_t out_row_stride, float* lse_dev, int accumulate_weights,
+                                                 int32_t layer_index, const char* tensor_name) {
+    if (!plan) return fail(MI355Q_ERR_NULL_HANDLE, "plan is null");
+    if (!cache || !sequences) return fail(MI355Q_ERR_INVALID_ARGUMENT, "null cache or sequences");
+    return add_call(plan, layer_index, tensor_name, sequences->maximum_rows,
+                    [=, ctx = plan->ctx, c = *cache, q = *sequences](hipStream_t s, bool run, mi355q_step* record) {
+                        return dispatch_kv_block_attention(ctx, s, &c, &q, q_dev, (int)q_dtype, q_row_stride, head_count, scale,
+                                                           window, out_dev, (int)out_dtype, out_row_stride, lse_dev,
+                                                           accumulate_weights != 0, run, record);
+                    });
+}
+
+mi355q_status mi355q_plan_add_token_logprobs(mi355q_plan* plan, const void* logits_dev, mi355q_dtype dtype, uint32_t row_count,
+                                             uint32_t vocabulary_size, uint32_t row_stride, const int32_t* token_ids_dev,
+                                             float* logprob_dev, float* entropy_dev, uint32_t top_count,
+                                             int32_t* top_ids_dev, float* top_logprobs_dev, const char* tensor_name) {
+    if (!plan) return fail(MI355Q_ERR_NULL_HANDLE, "plan is null");
+    return add_call(plan, -1, tensor_name, row_count, [=, ctx = plan->ctx](hipStream_t s, bool run, mi355q_step* record) {
+        return dispatch_token_logprobs(ctx, s, logits_dev, (int)dtype, row_count, vocabulary_size, row_stride, token_ids_dev,
+                                       logprob_dev, entropy_dev, top_count, top_ids_dev, top_logprobs_dev, run, record);
+    });
 }
 
 int32_t mi355q_plan_step_count(const mi355q_plan* plan) { return plan ? (int32_t)plan->steps.size() : -1; }

@@ -363,6 +363,43 @@ mi355q_status launch_logprobs(hipStream_t s, const LogprobArgs& a) {
 }
 
 }  // namespace
+
+mi355q_status dispatch_token_logprobs(mi355q_context* ctx, hipStream_t s, const void* logits, int dtype, uint32_t rows,
+                                      uint32_t vocabulary, uint32_t row_stride, const int32_t* tokens, float* logprob,
+                                      float* entropy, uint32_t top, int32_t* top_ids, float* top_logprobs, bool run,
+                                      mi355q_step* record) {
+    if (!ctx) return fail(MI355Q_ERR_NULL_HANDLE, "context is null");
+    if (!logits) return fail(MI355Q_ERR_INVALID_ARGUMENT, "null logits");
+    if (dtype != MI355Q_F16 && dtype != MI355Q_BF16 && dtype != MI355Q_F32)
+        return fail(MI355Q_ERR_INVALID_ARGUMENT, "unknown element type %d", dtype);
+    if (!rows || !vocabulary) return fail(MI355Q_ERR_SHAPE, "no rows or an empty vocabulary");
+    if (rows > (1u << 24) || vocabulary > (1u << 30))
+        return fail(MI355Q_ERR_SHAPE, "%u rows of %u logits: at most 2^24 rows and 2^30 logits a row", rows, vocabulary);
+    if (row_stride == 0) row_stride = vocabulary;
+    if (row_stride < vocabulary) return fail(MI355Q_ERR_SHAPE, "row stride %u is shorter than the vocabulary of %u", row_stride, vocabulary);
+    if (top > kTopMost) return fail(MI355Q_ERR_SHAPE, "%u alternatives a row: at most %u", top, kTopMost);
+    if (!tokens != !logprob) return fail(MI355Q_ERR_INVALID_ARGUMENT, "token ids and their log probabilities go together");
+    if (top && (!top_ids || !top_logprobs)) return fail(MI355Q_ERR_INVALID_ARGUMENT, "null buffers for the alternatives");
+    if (!logprob && !entropy && !top) return fail(MI355Q_ERR_INVALID_ARGUMENT, "nothing is asked for");
+    if ((uintptr_t)logits % (dtype == MI355Q_F32 ? 4 : 2) || (uintptr_t)tokens % 4 || (uintptr_t)logprob % 4 ||
+        (uintptr_t)entropy % 4 || (uintptr_t)top_ids % 4 || (uintptr_t)top_logprobs % 4)
+        return fail(MI355Q_ERR_INVALID_ARGUMENT, "misaligned pointer");
+    LogprobArgs a{logits, tokens, logprob, entropy, top_ids, top_logprobs,
+                  rows, vocabulary, row_stride, top, 1, 0, nullptr, nullptr};
+    logprob_slices(&a);
+    if (record) describe_step(record, "token_logprobs", "token_logprobs", a.rows * a.slices, 1, 1, 256, 0);
+    if (!run) return MI355Q_OK;
+    MI355Q_HIP(hipSetDevice(ctx->device));
+    if (a.slices > 1) {
+        const size_t parts = (size_t)a.rows * a.slices;
+        if (mi355q_status st = ensure_workspace(ctx, parts * (sizeof(float4) + a.top * 8))) return st;
+        a.parts = (float4*)ctx->workspace;
+        a.part_keys = (unsigned long long*)(a.parts + parts);
+    }
+    if (dtype == MI355Q_F32) return launch_logprobs<MI355Q_F32>(s, a);
+    if (dtype == MI355Q_BF16) return launch_logprobs<MI355Q_BF16>(s, a);
+    return launch_logprobs<MI355Q_F16>(s, a);
+}
 }  // namespace mi355q
 
 using namespace mi355q;
@@ -371,35 +408,9 @@ extern "C" mi355q_status mi355q_token_logprobs(mi355q_context* ctx, void* stream
                                                uint32_t row_count, uint32_t vocabulary_size, uint32_t row_stride,
                                                const int32_t* token_ids_dev, float* logprob_dev, float* entropy_dev,
                                                uint32_t top_count, int32_t* top_ids_dev, float* top_logprobs_dev) {
-    if (!ctx) return fail(MI355Q_ERR_NULL_HANDLE, "context is null");
-    if (!logits_dev) return fail(MI355Q_ERR_INVALID_ARGUMENT, "null logits");
-    if (dtype != MI355Q_F16 && dtype != MI355Q_BF16 && dtype != MI355Q_F32)
-        return fail(MI355Q_ERR_INVALID_ARGUMENT, "unknown element type %d", (int)dtype);
-    if (!row_count || !vocabulary_size) return fail(MI355Q_ERR_SHAPE, "no rows or an empty vocabulary");
-    if (row_count > (1u << 24) || vocabulary_size > (1u << 30))
-        return fail(MI355Q_ERR_SHAPE, "%u rows of %u logits: at most 2^24 rows and 2^30 logits a row", row_count, vocabulary_size);
-    if (row_stride == 0) row_stride = vocabulary_size;
-    if (row_stride < vocabulary_size) return fail(MI355Q_ERR_SHAPE, "row stride %u is shorter than the vocabulary of %u", row_stride, vocabulary_size);
-    if (top_count > kTopMost) return fail(MI355Q_ERR_SHAPE, "%u alternatives a row: at most %u", top_count, kTopMost);
-    if (!token_ids_dev != !logprob_dev) return fail(MI355Q_ERR_INVALID_ARGUMENT, "token ids and their log probabilities go together");
-    if (top_count && (!top_ids_dev || !top_logprobs_dev)) return fail(MI355Q_ERR_INVALID_ARGUMENT, "null buffers for the alternatives");
-    if (!logprob_dev && !entropy_dev && !top_count) return fail(MI355Q_ERR_INVALID_ARGUMENT, "nothing is asked for");
-    if ((uintptr_t)logits_dev % (dtype == MI355Q_F32 ? 4 : 2) || (uintptr_t)token_ids_dev % 4 || (uintptr_t)logprob_dev % 4 ||
-        (uintptr_t)entropy_dev % 4 || (uintptr_t)top_ids_dev % 4 || (uintptr_t)top_logprobs_dev % 4)
-        return fail(MI355Q_ERR_INVALID_ARGUMENT, "misaligned pointer");
-    MI355Q_HIP(hipSetDevice(ctx->device));
     ScratchGuard guard(ctx, (hipStream_t)stream);
     if (guard.status) return guard.status;
-    LogprobArgs a{logits_dev, token_ids_dev, logprob_dev, entropy_dev, top_ids_dev, top_logprobs_dev,
-                  row_count, vocabulary_size, row_stride, top_count, 1, 0, nullptr, nullptr};
-    logprob_slices(&a);
-    if (a.slices > 1) {
-        const size_t parts = (size_t)a.rows * a.slices;
-        if (mi355q_status st = ensure_workspace(ctx, parts * (sizeof(float4) + a.top * 8))) return st;
-        a.parts = (float4*)ctx->workspace;
-        a.part_keys = (unsigned long long*)(a.parts + parts);
-    }
-    if (dtype == MI355Q_F32) return launch_logprobs<MI355Q_F32>((hipStream_t)stream, a);
-    if (dtype == MI355Q_BF16) return launch_logprobs<MI355Q_BF16>((hipStream_t)stream, a);
-    return launch_logprobs<MI355Q_F16>((hipStream_t)stream, a);
+    return dispatch_token_logprobs(ctx, (hipStream_t)stream, logits_dev, (int)dtype, row_count, vocabulary_size, row_stride,
+                                   token_ids_dev, logprob_dev, entropy_dev, top_count, top_ids_dev, top_logprobs_dev, true,
+                                   nullptr);
 }
