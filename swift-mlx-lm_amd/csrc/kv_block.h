@@ -86,6 +86,18 @@ __device__ __forceinline__ uint32_t kv_value_byte(uint32_t t, uint32_t d) {
     return ((d >> 4) * 4 + ((t >> 2) & 3)) * 256 + (d & 15) * 16 + (t >> 5) * 8 + ((t >> 4) & 1) * 4 + (t & 3);
 }
 
+// Pieces of the context's scratch, 256 bytes apart at least: counted with `at` null, then handed out.
+struct Buffers {
+    char* at;
+    size_t used;
+    template <typename T>
+    T* take(size_t count) {
+        T* const p = (T*)(at ? at + used : nullptr);
+        used += (count * sizeof(T) + 255) & ~(size_t)255;
+        return p;
+    }
+};
+
 // Checks shared by the entry points; fills the kernel arguments (kv_block_cache.hip).  `rows`: the call reads row tables.
 mi355q_status kv_block_prepare(const mi355q_context* ctx, const mi355q_kv_block_cache* cache,
                                const mi355q_kv_sequences* sequences, bool rows, KvBlockArgs* out);

@@ -918,17 +918,6 @@ __global__ __launch_bounds__(256) void kv_block_attention_join_kernel(AttentionA
 
 namespace {
 
-struct Buffers {
-    char* at;
-    size_t used;
-    template <typename T>
-    T* take(size_t count) {
-        T* const p = (T*)(at ? at + used : nullptr);
-        used += (count * sizeof(T) + 255) & ~(size_t)255;
-        return p;
-    }
-};
-
 // Blocks that the rows of a tile can see, and the parts they are split into so that the launch has about `wanted`
 // workgroups; a part is a multiple of `unit` blocks, one for each wavefront.
 uint64_t visible_blocks(const AttentionArgs& a, uint32_t tile_rows) {

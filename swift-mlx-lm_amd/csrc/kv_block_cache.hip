@@ -260,9 +260,44 @@ __device__ __forceinline__ uint32_t sum_key(float v) {
 
 constexpr uint32_t kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
 constexpr uint32_t kSelectBins = 2048;
-constexpr uint32_t kSelectKeys = 28672;              // keys that fit LDS; a longer sequence's others are read again
-constexpr uint32_t kSelectList = 4096;
+// Keys that one workgroup takes: 128 of the 160 KB of LDS.  Eviction of one sequence of 4 heads to 64 tokens, one workgroup
+// against chunks: 28672 tokens 35 / 32 us, 32768 39 / 31, 60001 61 / 37; 16 sequences of 8 heads 43 / 50, 46 / 52, 74 / 73.
+constexpr uint32_t kSelectKeys = 32768;
+constexpr uint32_t kSelectList = 8192;               // listed keys held in LDS; more are read again
 constexpr uint32_t kSelectGroup = 8;                 // blocks of a wavefront in flight
+// Chunks of a sequence and head: as many as make 128 workgroups, 2 at least and 32 at most (32 heads and 60001 tokens: 64
+// workgroups 61 us, 128 44, 256 44, 512 57: every one of them sums the histograms of all chunks), of 32 blocks or more
+constexpr uint32_t kSelectChunks = 32, kSelectChunkBlocks = 32, kSelectGroups = 128;
+constexpr uint32_t kSelectShift = 21;                // bits under the first digit
+
+// A sequence's share of a call: which of its tokens compete, and for how many places.
+struct SelectTask {
+    const int32_t* table;
+    int32_t* out;
+    uint32_t head, lane, wave, length, blocks, low, count, need;
+    // budget >= sinks + recent and length > budget: the tokens [low, low + count) between the two are more than those wanted
+    __device__ SelectTask(const KvBlockArgs& a, const EvictArgs& e, uint32_t head, uint32_t b)
+        : table(a.table + (size_t)b * a.table_stride), out(e.positions + ((size_t)b * a.kv_heads + head) * e.budget), head(head),
+          lane(threadIdx.x & 63), wave((uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6))),
+          length((uint32_t)kv_length(a, b)), blocks((length + kKvTokens - 1) / kKvTokens), low(e.sinks),
+          count(length - e.recent - e.sinks), need(e.budget - e.sinks - e.recent) {}
+    __device__ bool competes(uint32_t j) const { return j * kKvTokens + lane - low < count; }
+    // f(block, key of the lane's token) for a wavefront's share of blocks [first, last), eight of them in flight
+    template <typename F>
+    __device__ void each(const KvBlockArgs& a, uint32_t first, uint32_t last, F&& f) const {
+        for (uint32_t j0 = first + wave; j0 < last; j0 += kSelectWaves * kSelectGroup) {
+            float v[kSelectGroup];
+#pragma unroll
+            for (uint32_t g = 0; g < kSelectGroup; g++) {
+                const int32_t block = scalar_block_id(a, table, (int32_t)min(j0 + g * kSelectWaves, last - 1));
+                v[g] = block < 0 ? 0.0f : kv_sums(a, block, head)[lane];
+            }
+#pragma unroll
+            for (uint32_t g = 0; g < kSelectGroup; g++)
+                if (j0 + g * kSelectWaves < last) f(j0 + g * kSelectWaves, sum_key(v[g]));
+        }
+    }
+};
 
 // Exclusive sums of two counts over the workgroup's threads; `totals` is LDS for one pair a wavefront.
 __device__ __forceinline__ uint2 scan_counts(uint2 own, uint2* totals, uint32_t lane, uint32_t wave, uint2* all) {
@@ -288,116 +323,56 @@ __device__ __forceinline__ uint2 scan_counts(uint2 own, uint2* totals, uint32_t 
     return before;
 }
 
-// One workgroup per sequence and head, a wavefront per block of 64 tokens at a time.  Latency-bound (a workgroup has one
-// sequence's few hundred kilobytes): the sums are read once, eight blocks of a wavefront in flight, and their keys held in
-// LDS; the key of the last token kept is found in three digits of 11, 11 and 10 bits from histograms; then every block's
-// kept tokens and ties become bit masks, whose counts give each block its place in the list.  Ties with the last key are
-// kept from the lowest position on.
-__global__ __launch_bounds__(kSelectThreads) void kv_block_select_kernel(KvBlockArgs a, EvictArgs e, uint32_t room) {
-    extern __shared__ uint32_t lds_keys[];
-    __shared__ uint32_t bins[kSelectBins];
-    __shared__ uint64_t keep_masks[kSelectThreads], tie_masks[kSelectThreads];
-    __shared__ uint32_t listed_keys[kSelectList];        // keys that begin with the first digit found
-    __shared__ uint2 totals[kSelectWaves];
-    __shared__ uint32_t found, left, listed;
-    const uint32_t head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
-    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
-    const uint32_t length = (uint32_t)kv_length(a, b);
-    const int32_t* const table = a.table + (size_t)b * a.table_stride;
-    int32_t* const out = e.positions + ((size_t)b * a.kv_heads + head) * e.budget;
-    if (head == 0 && tid == 0) e.new_lengths[b] = (int32_t)min(length, e.budget);
-    if (length <= e.budget) {
-        for (uint32_t t = tid; t < length; t += kSelectThreads) out[t] = (int32_t)t;
-        return;
+// One more in bins[bin] for every lane with `counts`.  Lanes that all agree are added at once: tokens that never received
+// weight have the same key, and 64 additions to one word wait for each other (32768 such tokens of 4 heads 113 -> 52 us).
+__device__ __forceinline__ void count_bin(uint32_t* bins, uint32_t bin, bool counts) {
+    const uint64_t mask = __ballot(counts);
+    if (!mask) return;
+    const uint32_t leader = (uint32_t)__builtin_ctzll(mask), first = (uint32_t)__builtin_amdgcn_readlane((int)bin, (int)leader);
+    if (__ballot(counts && bin == first) == mask) {
+        if ((threadIdx.x & 63) == leader) atomicAdd(&bins[first], (uint32_t)__popcll(mask));
+    } else if (counts) {
+        atomicAdd(&bins[bin], 1u);
     }
-    // budget >= sinks + recent and length > budget: the tokens [low, high) between the two are more than those wanted
-    const uint32_t low = e.sinks, high = length - e.recent, blocks = (length + kKvTokens - 1) / kKvTokens;
-    uint32_t need = e.budget - e.sinks - e.recent;
-    const bool some = need > 0;
-    // f(block, key of the lane's token) for a wavefront's share of blocks [first, last): from memory, eight in flight, or LDS
-    const uint32_t held = min(room / kKvTokens, blocks);
-    auto each_read = [&](uint32_t first, uint32_t last, auto&& f) {
-        for (uint32_t j0 = first + wave; j0 < last; j0 += kSelectWaves * kSelectGroup) {
-            float v[kSelectGroup];
-#pragma unroll
-            for (uint32_t g = 0; g < kSelectGroup; g++) {
-                const int32_t block = scalar_block_id(a, table, (int32_t)min(j0 + g * kSelectWaves, last - 1));
-                v[g] = block < 0 ? 0.0f : kv_sums(a, block, head)[lane];
-            }
-#pragma unroll
-            for (uint32_t g = 0; g < kSelectGroup; g++)
-                if (j0 + g * kSelectWaves < last) f(j0 + g * kSelectWaves, sum_key(v[g]));
-        }
-    };
-    auto each = [&](uint32_t first, uint32_t last, auto&& f) {
-        for (uint32_t j = first + wave; j < min(last, held); j += kSelectWaves) f(j, lds_keys[j * kKvTokens + lane]);
-        if (last > held) each_read(max(first, held), last, f);
-    };
-    auto between = [&](uint32_t j) { return j * kKvTokens + lane - low < high - low; };
-    uint32_t prefix = 0;
-    if (some) {
-#pragma unroll
-        for (int digit = 0; digit < 3; digit++) {
-            constexpr uint32_t shifts[3] = {21, 10, 0};
-            for (uint32_t i = tid; i < kSelectBins; i += kSelectThreads) bins[i] = 0;
-            __syncthreads();
-            if (digit == 0) {
-                if (tid == 0) listed = 0;
-                each_read(0, blocks, [&](uint32_t j, uint32_t key) {
-                    if (j < held) lds_keys[j * kKvTokens + lane] = key;
-                    if (between(j)) atomicAdd(&bins[key >> 21], 1u);
-                });
-            } else if (digit == 1) {
-                each(0, blocks, [&](uint32_t j, uint32_t key) {
-                    const bool match = between(j) && key >> 21 == prefix >> 21;
-                    const uint64_t mask = __ballot(match);
-                    if (!mask) return;
-                    uint32_t at = 0;
-                    if (lane == 0) at = atomicAdd(&listed, (uint32_t)__popcll(mask));
-                    at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + (uint32_t)__popcll(mask & ((1ull << lane) - 1));
-                    if (match) {
-                        atomicAdd(&bins[(key >> 10) & 2047u], 1u);
-                        if (at < kSelectList) listed_keys[at] = key;
-                    }
-                });
-            } else if (listed <= kSelectList) {
-                for (uint32_t i = tid; i < listed; i += kSelectThreads)
-                    if (listed_keys[i] >> 10 == prefix >> 10) atomicAdd(&bins[listed_keys[i] & 1023u], 1u);
-            } else {
-                each(0, blocks, [&](uint32_t j, uint32_t key) {
-                    if (between(j) && key >> 10 == prefix >> 10) atomicAdd(&bins[key & 1023u], 1u);
-                });
-            }
-            __syncthreads();
-            // counts from the highest bin down, two bins a thread: the one in which the need is met
-            const uint32_t bin = kSelectBins - 1 - 2 * tid, upper = bins[bin], pair = upper + bins[bin - 1];
-            uint2 all;
-            const uint32_t before = scan_counts(make_uint2(pair, 0), totals, lane, wave, &all).x;
-            if (before < need && need <= before + pair) {
-                const bool first = need <= before + upper;
-                found = first ? bin : bin - 1;
-                left = need - before - (first ? 0 : upper);
-            }
-            __syncthreads();
-            prefix |= found << shifts[digit];
-            need = left;
-        }
+}
+
+// The bin in which `need` is met, counted from the highest down, and what is left to find in it.  Thread i owns the pair
+// of bins 2046 - 2 i and 2047 - 2 i with these counts; `at` is LDS.
+__device__ __forceinline__ uint2 find_bin(uint32_t lower, uint32_t upper, uint32_t need, uint2* totals, uint2* at, uint32_t lane, uint32_t wave) {
+    const uint32_t bin = kSelectBins - 1 - 2 * threadIdx.x, pair = upper + lower;
+    uint2 all;
+    const uint32_t before = scan_counts(make_uint2(pair, 0), totals, lane, wave, &all).x;
+    if (before < need && need <= before + pair) {
+        const bool first = need <= before + upper;
+        *at = make_uint2(first ? bin : bin - 1, need - before - (first ? 0 : upper));
     }
-    // `need` tokens with exactly this key, the first of them, and all with a larger one, 1024 blocks at a time
-    uint32_t written = 0, ties = 0;
-    for (uint32_t first = 0; first < blocks; first += kSelectThreads) {
-        const uint32_t last = min(first + kSelectThreads, blocks);
+    __syncthreads();
+    return *at;
+}
+
+struct SelectMasks {
+    uint64_t keep[kSelectThreads], tie[kSelectThreads];
+};
+
+// Writes the positions kept in blocks [first, last), 1024 blocks at a time: every token outside the competition, those with
+// a key over `last_key` and of those that equal it the first `need`, `ties` of which lie in front; `written` tokens kept
+// lie in front.  keys(first, last, f) calls f(block, key) for the wavefront's blocks.
+template <typename K>
+__device__ __forceinline__ void write_kept(const SelectTask& s, uint32_t first, uint32_t last, bool some, uint32_t last_key, uint32_t need,
+                                           uint32_t written, uint32_t ties, SelectMasks* masks, uint2* totals, K&& keys) {
+    for (uint32_t from = first; from < last; from += kSelectThreads) {
+        const uint32_t to = min(from + kSelectThreads, last);
         __syncthreads();
-        each(first, last, [&](uint32_t j, uint32_t key) {
-            const bool there = between(j);
-            const uint64_t keep = __ballot(there ? some && key > prefix : j * kKvTokens + lane < length), tie = __ballot(there && some && key == prefix);
-            if (lane == 0) { keep_masks[j - first] = keep; tie_masks[j - first] = tie; }
+        keys(from, to, [&](uint32_t j, uint32_t key) {
+            const bool there = s.competes(j);
+            const uint64_t keep = __ballot(there ? some && key > last_key : j * kKvTokens + s.lane < s.length), tie = __ballot(there && some && key == last_key);
+            if (s.lane == 0) { masks->keep[j - from] = keep; masks->tie[j - from] = tie; }
         });
         __syncthreads();
-        const bool mine = first + tid < last;
-        uint64_t keep = mine ? keep_masks[tid] : 0, tie = mine ? tie_masks[tid] : 0;
+        const bool mine = from + threadIdx.x < to;
+        uint64_t keep = mine ? masks->keep[threadIdx.x] : 0, tie = mine ? masks->tie[threadIdx.x] : 0;
         uint2 all;
-        const uint2 before = scan_counts(make_uint2((uint32_t)__popcll(keep), (uint32_t)__popcll(tie)), totals, lane, wave, &all);
+        const uint2 before = scan_counts(make_uint2((uint32_t)__popcll(keep), (uint32_t)__popcll(tie)), totals, s.lane, s.wave, &all);
         const uint32_t ties_before = ties + before.y;
         uint32_t place = written + before.x + min(ties_before, need) - min(ties, need);
         // the block's ties that are kept are its first: drop the last set bits until they fit
@@ -410,10 +385,231 @@ __global__ __launch_bounds__(kSelectThreads) void kv_block_select_kernel(KvBlock
             }
             tie = chosen;
         }
-        for (keep |= tie; keep; keep &= keep - 1) out[place++] = (int32_t)((first + tid) * kKvTokens + (uint32_t)__builtin_ctzll(keep));
+        for (keep |= tie; keep; keep &= keep - 1) s.out[place++] = (int32_t)((from + threadIdx.x) * kKvTokens + (uint32_t)__builtin_ctzll(keep));
         written += all.x + min(ties + all.y, need) - min(ties, need);
         ties += all.y;
     }
+}
+
+// Sequences of up to 32768 tokens: one workgroup per sequence and head, a wavefront per block of 64 tokens at a time.
+// Latency-bound (a workgroup has one sequence's few tens of kilobytes): the sums are read once, eight blocks of a wavefront
+// in flight, and their keys held in LDS; the key of the last token kept is found in three digits of 11, 11 and 10 bits from
+// histograms; then every block's kept tokens and ties become bit masks, whose counts give each block its place in the list
+// (8 sequences of 8192 tokens, 8 heads: 17 us).
+// Ties with the last key are kept from the lowest position on.
+__global__ __launch_bounds__(kSelectThreads) void kv_block_select_kernel(KvBlockArgs a, EvictArgs e) {
+    extern __shared__ uint32_t lds_keys[];
+    __shared__ uint32_t bins[kSelectBins];
+    __shared__ SelectMasks masks;                        // before them the keys that begin with the first digit found
+    __shared__ uint2 totals[kSelectWaves], found;
+    __shared__ uint32_t listed;
+    uint32_t* const list = (uint32_t*)&masks;
+    constexpr uint32_t kSelectHeld = sizeof masks / 4;
+    const uint32_t tid = threadIdx.x;
+    const SelectTask s(a, e, blockIdx.x, blockIdx.y);
+    if (s.head == 0 && tid == 0) e.new_lengths[blockIdx.y] = (int32_t)min(s.length, e.budget);
+    if (s.length <= e.budget) {
+        for (uint32_t t = tid; t < s.length; t += kSelectThreads) s.out[t] = (int32_t)t;
+        return;
+    }
+    auto each = [&](uint32_t first, uint32_t last, auto&& f) {
+        for (uint32_t j = first + s.wave; j < last; j += kSelectWaves) f(j, lds_keys[j * kKvTokens + s.lane]);
+    };
+    const bool some = s.need > 0;
+    uint32_t prefix = 0, need = s.need;
+    if (tid == 0) listed = 0;
+    for (uint32_t i = tid; i < kSelectBins; i += kSelectThreads) bins[i] = 0;
+    __syncthreads();
+    s.each(a, 0, s.blocks, [&](uint32_t j, uint32_t key) {
+        lds_keys[j * kKvTokens + s.lane] = key;
+        count_bin(bins, key >> kSelectShift, s.competes(j));
+    });
+    if (some) {
+#pragma unroll
+        for (int digit = 0; digit < 3; digit++) {
+            constexpr uint32_t shifts[3] = {kSelectShift, 10, 0};
+            if (digit) {
+                for (uint32_t i = tid; i < kSelectBins; i += kSelectThreads) bins[i] = 0;
+                __syncthreads();
+            }
+            if (digit == 1) {
+                each(0, s.blocks, [&](uint32_t j, uint32_t key) {
+                    const bool match = s.competes(j) && key >> kSelectShift == prefix >> kSelectShift;
+                    const uint64_t mask = __ballot(match);
+                    if (!mask) return;
+                    uint32_t at = 0;
+                    if (s.lane == 0) at = atomicAdd(&listed, (uint32_t)__popcll(mask));
+                    at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + (uint32_t)__popcll(mask & ((1ull << s.lane) - 1));
+                    if (match && at < kSelectHeld) list[at] = key;
+                    count_bin(bins, (key >> 10) & 2047u, match);
+                });
+            } else if (digit == 2 && listed <= kSelectHeld) {
+                for (uint32_t i = tid; i < listed; i += kSelectThreads)
+                    if (list[i] >> 10 == prefix >> 10) atomicAdd(&bins[list[i] & 1023u], 1u);
+            } else if (digit == 2) {
+                each(0, s.blocks, [&](uint32_t j, uint32_t key) { count_bin(bins, key & 1023u, s.competes(j) && key >> 10 == prefix >> 10); });
+            }
+            __syncthreads();
+            const uint2 at = find_bin(bins[kSelectBins - 2 - 2 * tid], bins[kSelectBins - 1 - 2 * tid], need, totals, &found, s.lane, s.wave);
+            prefix |= at.x << shifts[digit];
+            need = at.y;
+        }
+    }
+    write_kept(s, 0, s.blocks, some, prefix, need, 0, 0, &masks, totals, each);
+}
+
+// Longer sequences: a workgroup per chunk of blocks, three launches.  `counts`: a chunk's histogram of the first digit.
+// `list`: with the histograms of all chunks every workgroup finds the first digit, counts its chunk's tokens that are kept
+// for sure and lists the keys that begin with it.  `write`: from the lists of all chunks every workgroup finds the other
+// digits and its chunk's place, and writes its positions.  What a workgroup does alike with the others of its sequence
+// and head are a few thousand numbers.  Latency-bound like the kernel above: 60001 tokens of 4 heads take 5 + 10 + 14 us, one
+// workgroup a head took 64 (60 tokens a thread: bound by instructions).
+struct SelectChunks {
+    uint32_t chunks, blocks;      // chunks of a sequence, blocks of a chunk
+    uint32_t* histogram;          // [sequence][head][chunk][2048]
+    uint32_t* keys;               // [sequence][head][chunk][blocks * 64]
+    uint2* counts;                // [sequence][head][chunk]: kept for sure, listed
+    uint2* digit;                 // [sequence][head]: first digit, tokens to keep of those that begin with it
+};
+
+__global__ __launch_bounds__(kSelectThreads) void kv_block_select_count_kernel(KvBlockArgs a, EvictArgs e, SelectChunks c) {
+    __shared__ uint32_t bins[kSelectBins];
+    const SelectTask s(a, e, blockIdx.y, blockIdx.z);
+    const uint32_t first = blockIdx.x * c.blocks, last = min(first + c.blocks, s.blocks);
+    if (s.length <= e.budget || first >= s.blocks || !s.need) return;
+    for (uint32_t i = threadIdx.x; i < kSelectBins; i += kSelectThreads) bins[i] = 0;
+    __syncthreads();
+    s.each(a, first, last, [&](uint32_t j, uint32_t key) { count_bin(bins, key >> kSelectShift, s.competes(j)); });
+    __syncthreads();
+    uint2* const out = (uint2*)c.histogram + (((size_t)blockIdx.z * a.kv_heads + s.head) * c.chunks + blockIdx.x) * (kSelectBins / 2);
+    out[threadIdx.x] = ((const uint2*)bins)[threadIdx.x];
+}
+
+__global__ __launch_bounds__(kSelectThreads) void kv_block_select_list_kernel(KvBlockArgs a, EvictArgs e, SelectChunks c) {
+    __shared__ uint2 totals[kSelectWaves], found;
+    __shared__ uint32_t sure, listed;
+    const SelectTask s(a, e, blockIdx.y, blockIdx.z);
+    const uint32_t first = blockIdx.x * c.blocks, last = min(first + c.blocks, s.blocks);
+    if (s.length <= e.budget || first >= s.blocks || !s.need) return;
+    const size_t pair = (size_t)blockIdx.z * a.kv_heads + s.head;
+    if (threadIdx.x == 0) sure = listed = 0;
+    const uint32_t used = (s.blocks + c.blocks - 1) / c.blocks;
+    const uint2* const all = (const uint2*)c.histogram + pair * c.chunks * (kSelectBins / 2) + (kSelectBins / 2 - 1 - threadIdx.x);
+    uint2 sum = make_uint2(0, 0);
+#pragma unroll 8
+    for (uint32_t i = 0; i < used; i++) {
+        const uint2 v = all[i * (kSelectBins / 2)];
+        sum.x += v.x;
+        sum.y += v.y;
+    }
+    const uint2 at = find_bin(sum.x, sum.y, s.need, totals, &found, s.lane, s.wave);
+    if (blockIdx.x == 0 && threadIdx.x == 0) c.digit[pair] = at;
+    uint32_t* const out = c.keys + (pair * c.chunks + blockIdx.x) * c.blocks * kKvTokens;
+    s.each(a, first, last, [&](uint32_t j, uint32_t key) {
+        const bool there = s.competes(j), match = there && key >> kSelectShift == at.x;
+        const uint64_t mask = __ballot(match), kept = __ballot(there ? key >> kSelectShift > at.x : j * kKvTokens + s.lane < s.length);
+        uint32_t place = 0;
+        if (s.lane == 0) {
+            if (kept) atomicAdd(&sure, (uint32_t)__popcll(kept));
+            if (mask) place = atomicAdd(&listed, (uint32_t)__popcll(mask));
+        }
+        place = (uint32_t)__builtin_amdgcn_readfirstlane((int)place) + (uint32_t)__popcll(mask & ((1ull << s.lane) - 1));
+        if (match) out[place] = key;
+    });
+    __syncthreads();
+    if (threadIdx.x == 0) c.counts[pair * c.chunks + blockIdx.x] = make_uint2(sure, listed);
+}
+
+__global__ __launch_bounds__(kSelectThreads) void kv_block_select_write_kernel(KvBlockArgs a, EvictArgs e, SelectChunks c) {
+    __shared__ uint32_t bins[kSelectBins], listed_keys[kSelectList];
+    __shared__ SelectMasks masks;
+    __shared__ uint2 totals[kSelectWaves], found;
+    __shared__ uint32_t sure[kSelectChunks], listed[kSelectChunks], offset[kSelectChunks + 1];
+    const uint32_t chunk = blockIdx.x, tid = threadIdx.x;
+    const SelectTask s(a, e, blockIdx.y, blockIdx.z);
+    const uint32_t first = chunk * c.blocks, last = min(first + c.blocks, s.blocks);
+    if (chunk == 0 && s.head == 0 && tid == 0) e.new_lengths[blockIdx.z] = (int32_t)min(s.length, e.budget);
+    if (first >= s.blocks) return;
+    if (s.length <= e.budget) {
+        for (uint32_t t = first * kKvTokens + tid; t < min(last * kKvTokens, s.length); t += kSelectThreads) s.out[t] = (int32_t)t;
+        return;
+    }
+    auto read = [&](uint32_t from, uint32_t to, auto&& f) { s.each(a, from, to, f); };
+    if (!s.need) {
+        const uint32_t t = first * kKvTokens, high = s.low + s.count;
+        write_kept(s, first, last, false, 0, 0, min(t, s.low) + (t > high ? t - high : 0), 0, &masks, totals, read);
+        return;
+    }
+    const size_t pair = (size_t)blockIdx.z * a.kv_heads + s.head;
+    const uint32_t used = (s.blocks + c.blocks - 1) / c.blocks;
+    const uint2 digit = c.digit[pair];
+    if (tid < used) {
+        const uint2 n = c.counts[pair * c.chunks + tid];
+        sure[tid] = n.x;
+        listed[tid] = n.y;
+    }
+    __syncthreads();
+    if (tid <= used) {
+        uint32_t sum = 0;
+        for (uint32_t i = 0; i < tid; i++) sum += listed[i];
+        offset[tid] = sum;
+    }
+    __syncthreads();
+    const bool held = offset[used] <= kSelectList;
+    // f(key, whether there is one) for the wavefront's share of `n` keys, from the one at k0 on, four loads in flight
+    auto each_of = [&](const uint32_t* keys, uint32_t n, uint32_t k0, uint32_t step, auto&& f) {
+        for (; k0 < n; k0 += step) {
+            uint32_t v[4];
+#pragma unroll
+            for (uint32_t g = 0; g < 4; g++) v[g] = keys[min(k0 + g * 64 + s.lane, n - 1)];
+#pragma unroll
+            for (uint32_t g = 0; g < 4; g++)
+                if (k0 + g * 64 < n) f(v[g], k0 + g * 64 + s.lane, k0 + g * 64 + s.lane < n);
+        }
+    };
+    const uint32_t* const keys = c.keys + pair * c.chunks * c.blocks * kKvTokens;
+    if (held) {
+        for (uint32_t i = s.wave; i < used; i += kSelectWaves)
+            each_of(keys + (size_t)i * c.blocks * kKvTokens, listed[i], 0, 256, [&](uint32_t key, uint32_t k, bool there) {
+                if (there) listed_keys[offset[i] + k] = key;
+            });
+        __syncthreads();
+    }
+    // f(key, whether there is one) for the keys that chunks [0, end) have listed
+    auto each_listed = [&](uint32_t end, auto&& f) {
+        if (held) {
+            for (uint32_t k = s.wave * 64 + s.lane; k - s.lane < offset[end]; k += kSelectThreads) f(listed_keys[min(k, kSelectList - 1)], k < offset[end]);
+        } else {
+            for (uint32_t i = 0; i < end; i++)
+                each_of(keys + (size_t)i * c.blocks * kKvTokens, listed[i], s.wave * 256, kSelectWaves * 256, [&](uint32_t key, uint32_t, bool there) { f(key, there); });
+        }
+    };
+    uint32_t prefix = digit.x << kSelectShift, need = digit.y;
+#pragma unroll
+    for (int d = 0; d < 2; d++) {
+        for (uint32_t i = tid; i < kSelectBins; i += kSelectThreads) bins[i] = 0;
+        __syncthreads();
+        each_listed(used, [&](uint32_t key, bool there) {
+            if (d == 0) count_bin(bins, (key >> 10) & 2047u, there);
+            else count_bin(bins, key & 1023u, there && key >> 10 == prefix >> 10);
+        });
+        __syncthreads();
+        const uint2 at = find_bin(bins[kSelectBins - 2 - 2 * tid], bins[kSelectBins - 1 - 2 * tid], need, totals, &found, s.lane, s.wave);
+        prefix |= d == 0 ? at.x << 10 : at.x;
+        need = at.y;
+    }
+    // listed tokens in front of the chunk that are kept for their key, and those that equal the last one
+    uint32_t larger = 0, equal = 0;
+    each_listed(chunk, [&](uint32_t key, bool there) {
+        larger += there && key > prefix;
+        equal += there && key == prefix;
+    });
+    uint2 in_front;
+    scan_counts(make_uint2(larger, equal), totals, s.lane, s.wave, &in_front);
+    const uint32_t ties = in_front.y;
+    uint32_t written = in_front.x;
+    for (uint32_t i = 0; i < chunk; i++) written += sure[i];
+    write_kept(s, first, last, true, prefix, need, written + min(ties, need), ties, &masks, totals, read);
 }
 
 // One workgroup per new block, head and sequence: keys and values of its 64 kept tokens, gathered piece by piece (keys)
@@ -630,13 +826,43 @@ mi355q_status mi355q_kv_block_evict(mi355q_context* ctx, void* stream, const mi3
     ScratchGuard guard(ctx, (hipStream_t)stream);
     if (guard.status) return guard.status;
     EvictArgs e{budget, recent, sinks, new_block_table_stride, new_block_table_dev, new_lengths_dev, positions_dev};
-    if (!e.positions) {
-        if (mi355q_status st = ensure_workspace(ctx, (size_t)a.sequences * a.kv_heads * budget * 4)) return st;
-        e.positions = (int32_t*)ctx->workspace;
+    const uint32_t tokens = (a.max_length + kKvTokens - 1) / kKvTokens * kKvTokens;
+    const dim3 pairs(a.kv_heads, a.sequences);
+    const size_t pair_count = (size_t)a.sequences * a.kv_heads;
+    SelectChunks c{};
+    if (tokens > kSelectKeys) {
+        const uint32_t most = (uint32_t)(kSelectGroups / std::min<size_t>(pair_count, kSelectGroups / 2));
+        const uint32_t all = tokens / kKvTokens;
+        c.blocks = std::max(kSelectChunkBlocks, (all - 1) / std::min(most, kSelectChunks) + 1);
+        c.chunks = (all - 1) / c.blocks + 1;
     }
-    const uint32_t tokens = (a.max_length + kKvTokens - 1) / kKvTokens * kKvTokens, room = tokens < kSelectKeys ? tokens : kSelectKeys;
-    if (mi355q_status st = raise_lds_limit((const void*)kv_block_select_kernel, (size_t)kSelectKeys * 4)) return st;
-    kv_block_select_kernel<<<dim3(a.kv_heads, a.sequences), kSelectThreads, (size_t)room * 4, (hipStream_t)stream>>>(a, e, room);
+    for (int pass = 0; pass < 2; pass++) {
+        Buffers buf{pass ? (char*)ctx->workspace : nullptr, 0};
+        if (c.chunks) {
+            const size_t chunks = pair_count * c.chunks;
+            c.histogram = buf.take<uint32_t>(chunks * kSelectBins);
+            c.keys = buf.take<uint32_t>(chunks * c.blocks * kKvTokens);
+            c.counts = buf.take<uint2>(chunks);
+            c.digit = buf.take<uint2>(pair_count);
+        }
+        if (!positions_dev) e.positions = buf.take<int32_t>(pair_count * budget);
+        if (!pass && buf.used)
+            if (mi355q_status st = ensure_workspace(ctx, buf.used)) return st;
+    }
+    const hipStream_t s = (hipStream_t)stream;
+    if (c.chunks) {
+        const dim3 grid(c.chunks, a.kv_heads, a.sequences);
+        if (budget > recent + sinks) {
+            kv_block_select_count_kernel<<<grid, kSelectThreads, 0, s>>>(a, e, c);
+            MI355Q_HIP(hipGetLastError());
+            kv_block_select_list_kernel<<<grid, kSelectThreads, 0, s>>>(a, e, c);
+            MI355Q_HIP(hipGetLastError());
+        }
+        kv_block_select_write_kernel<<<grid, kSelectThreads, 0, s>>>(a, e, c);
+    } else {
+        if (mi355q_status st = raise_lds_limit((const void*)kv_block_select_kernel, (size_t)kSelectKeys * 4)) return st;
+        kv_block_select_kernel<<<pairs, kSelectThreads, (size_t)tokens * 4, s>>>(a, e);
+    }
     MI355Q_HIP(hipGetLastError());
     return kv_with_head_dimension(cache->head_dimension, [&](auto hd) -> mi355q_status {
         constexpr int HD = decltype(hd)::value;

@@ -314,6 +314,64 @@ def test_evict(pkg, ctx, hd, heads, lengths, budget, recent, sinks, ties):
     assert np.array_equal(sums2[picked], sums[picked], equal_nan=True)
 
 
+LONG = [
+    # (KV heads, lengths, longest the host knows of, budget, recent, sinks)
+    (2, [40000, 200, 16385, 0, 16384], 40000, 9001, 1000, 4),
+    (1, [70003], 70003, 60000, 0, 0),
+    (3, [20000, 33000], 50000, 1, 0, 0),
+    (1, [17000, 30001], 30001, 5000, 4000, 1000),         # nothing competes
+    (1, [100, 16000], 20000, 300, 5, 64),                 # chunks behind the sequences
+    (1, [2_200_000], 2_200_000, 100_000, 64, 4),          # chunks of more than 1024 blocks
+    (140, [16500] * 4, 16500, 1000, 64, 4),               # two chunks a sequence
+]
+
+
+@pytest.mark.parametrize("sums", ["spread", "ties", "zeros", "close"])
+@pytest.mark.parametrize("heads,lengths,longest,budget,recent,sinks", LONG)
+def test_evict_long(pkg, ctx, heads, lengths, longest, budget, recent, sinks, sums):
+    """Sequences whose tokens are selected by several workgroups: positions against a stable sort, new lengths, and the sums
+    that go along with the tokens."""
+    rng = np.random.default_rng(len(lengths) + budget)
+    hd, per = 64, -(-budget // TOKENS)
+    tables, free, blocks = deal(rng, lengths, spare=per * len(lengths))
+    new_tables = free.reshape(len(lengths), per)
+    shape = (blocks, heads, TOKENS)
+    if sums == "spread":
+        own = (6 * rng.random(shape) ** 4).astype(np.float32)
+    elif sums == "ties":
+        own = rng.choice(np.array([0.0, -0.0, 1.0, 2.5, np.nan, np.inf, -1.0, 1.0000001], np.float32), shape)
+    elif sums == "zeros":
+        own = np.zeros(shape, np.float32)
+    else:                                     # all sums begin with the same eleven bits, many are equal
+        own = (1.0 + rng.integers(0, 3000, shape) * 2.0 ** -23).astype(np.float32)
+    d_sums, scales = ctx.upload(own), ctx.alloc(blocks * heads * 2 * 4)
+    codes = ctx.alloc(pkg.KVBlockCache.codes_bytes(heads, hd, blocks))
+    ctx.fill(scales, 0x3F800000); ctx.fill(codes, 0)
+    cache = pkg.KVBlockCache(heads, hd, blocks, codes, scales, d_sums)
+    seq = sequences(pkg, ctx, tables, lengths, [1] * len(lengths), (1, longest))
+    new_lengths, positions = ctx.upload(np.full(len(lengths), -1, np.int32)), ctx.upload(np.full((len(lengths), heads, budget), -7, np.int32))
+    ctx.kv_block_evict(cache, seq, budget, ctx.upload(new_tables), per, new_lengths, recent, sinks, positions)
+    ctx.synchronize()
+    assert new_lengths.download(np.int32, (len(lengths),)).tolist() == [min(n, budget) for n in lengths]
+    got = positions.download(np.int32, (len(lengths), heads, budget))
+    after = d_sums.download(np.float32, shape)
+    for b, n in enumerate(lengths):
+        weight = own[tables[b]].transpose(1, 0, 2).reshape(heads, -1)[:, :n] if n else np.zeros((heads, 0), np.float32)
+        moved = after[new_tables[b]].transpose(1, 0, 2).reshape(heads, -1)
+        for h in range(heads):
+            kept = np.arange(n)
+            if n > budget:
+                middle = np.nan_to_num(weight[h, sinks:n - recent], nan=-np.inf, posinf=np.inf, neginf=-np.inf)
+                order = np.argsort(-middle, kind="stable")[:budget - sinks - recent] + sinks
+                kept = np.concatenate([np.arange(sinks), np.sort(order), np.arange(n - recent, n)])
+            assert np.array_equal(got[b, h, :len(kept)], kept)
+            assert np.all(got[b, h, len(kept):] == -7)
+            assert np.array_equal(moved[h, :len(kept)], weight[h, kept], equal_nan=True)
+            assert not moved[h, len(kept):].any()
+    for buf in (codes, scales, d_sums, positions, new_lengths):
+        buf.free()
+
+
 def test_evict_with_absent_blocks(pkg, ctx):
     rng = np.random.default_rng(3)
     cache = Cache(pkg, ctx, 1, 64, 8, rng)
