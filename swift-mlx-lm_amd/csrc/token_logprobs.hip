@@ -6,9 +6,10 @@
 //
 // Alternatives: logits are ordered by 64-bit keys (ordered value, ~index), all distinct, so equal logits need no rule of
 // their own.  The pass itself only notes, for every lane, the largest logit of each of its steps of sixteen (one LDS
-// store).  At the end the top_count-th largest of a wavefront's 64 lane maxima is a limit that top_count logits reach, and
-// only the steps whose maximum reaches the highest limit of the workgroup's four wavefronts -- about top_count of the
-// slice's hundreds or thousands -- are read again, from the cache, and their keys collected in LDS and cut to the largest.
+// store).  At the end the largest logits of the 64 lane numbers, over the workgroup's four wavefronts, give a limit: the
+// top_count-th largest of them is reached by top_count logits, and only the steps of sixteen whose maximum reaches it --
+// little more than top_count of the slice's hundreds or thousands -- are read again, from the cache, and their keys collected
+// in LDS and cut to the largest.
 #include "device_utils.h"
 
 namespace mi355q {
@@ -172,7 +173,7 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(LogprobArgs a) {
     __shared__ unsigned long long room[4][kTopRoom];
     __shared__ uint16_t maxima[4][kSliceSteps][64];  // of each step, each lane: the bf16 number at or above it
     __shared__ LogSum sums[4];
-    __shared__ float limits[4];
+    __shared__ float columns[4][64], workgroup_limit;
     __shared__ uint32_t counts[4];
     constexpr uint32_t VE = D == MI355Q_F32 ? 4 : 8;             // logits of a 16-byte load
     const uint32_t row = blockIdx.x / a.slices, slice = blockIdx.x - row * a.slices;
@@ -183,30 +184,37 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(LogprobArgs a) {
     const uint32_t lead = (uint32_t)(((uintptr_t)a.logits + row_at * size) % 16) / size;
     const uint32_t begin = slice * a.slice_length + wave * (64 * kLogprobLane);
     const uint32_t end = min((slice + 1) * a.slice_length, a.vocabulary + lead);
+    const char* const row_start = (const char*)a.logits + row_at * size;
     LogSum s{kMasked, 0.0f, 0.0f};
     uint32_t steps = 0;
     for (uint32_t at = begin; at < end; at += kLogprobStep, steps++) {
+        // a row's first and last step may reach beyond it: pieces outside it are -inf, one on its edge is read by elements
+        const bool whole = at >= lead && at + 64 * kLogprobLane <= a.vocabulary + lead;
+        u32x4 w[kLogprobLane / VE];
+#pragma unroll
+        for (uint32_t i = 0; i < kLogprobLane / VE; i++) {
+            const uint32_t p = at + i * (64 * VE) + lane * VE;
+            if (whole || (p >= lead && p + VE <= a.vocabulary + lead)) w[i] = *(const u32x4*)(row_start + (size_t)(p - lead) * size);
+            else w[i] = u32x4{} + (D == MI355Q_F32 ? 0xFF800000u : D == MI355Q_BF16 ? 0xFF80FF80u : 0xFC00FC00u);
+        }
         float x[kLogprobLane];
-        if (at >= lead && at + 64 * kLogprobLane <= a.vocabulary + lead) {
+#pragma unroll
+        for (uint32_t i = 0; i < kLogprobLane; i++) {
+            if constexpr (D == MI355Q_F32) {
+                x[i] = __uint_as_float(w[i / 4][i % 4]);
+            } else {
+                const uint16_t h = (uint16_t)(w[i / 8][i % 8 / 2] >> (16 * (i & 1)));
+                x[i] = D == MI355Q_BF16 ? bf16_to_f32(h) : f16_to_f32(h);
+            }
+        }
+        if (!whole) {
 #pragma unroll
             for (uint32_t i = 0; i < kLogprobLane / VE; i++) {
-                const size_t p = row_at + (at - lead) + i * (64 * VE) + lane * VE;
-                if constexpr (D == MI355Q_F32) {
-                    const float4 w = *(const float4*)((const float*)a.logits + p);
-                    x[4 * i] = w.x; x[4 * i + 1] = w.y; x[4 * i + 2] = w.z; x[4 * i + 3] = w.w;
-                } else {
-                    const uint4 w = *(const uint4*)((const uint16_t*)a.logits + p);
-                    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+                const uint32_t p = at + i * (64 * VE) + lane * VE;
+                if ((p < lead && p + VE > lead) || (p < a.vocabulary + lead && p + VE > a.vocabulary + lead))
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const uint16_t h = (uint16_t)(ws[e >> 1] >> (16 * (e & 1)));
-                        x[8 * i + e] = D == MI355Q_BF16 ? bf16_to_f32(h) : f16_to_f32(h);
-                    }
-                }
+                    for (uint32_t e = 0; e < VE; e++) x[i * VE + e] = logit_at<D>(a, row_at, lead, p + e);
             }
-        } else {
-#pragma unroll
-            for (uint32_t i = 0; i < kLogprobLane; i++) x[i] = logit_at<D>(a, row_at, lead, at + i / VE * (64 * VE) + lane * VE + i % VE);
         }
         // a NaN is dropped by every maximum: by this one, by the clamp of z below (e^z = 0) and by `x > kMasked` of the keys
         float top = kMasked;
@@ -233,10 +241,15 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(LogprobArgs a) {
     }
     TopKeys keys{room[wave], kMaskedKey, 0, a.top, lane};
     if (a.top) {
-        const float own = steps ? keys.limit_of(s.m) : kMasked;
-        if (lane == 0) limits[wave] = own;
+        // the largest logit of each lane number over the four wavefronts: 64 different logits, of which `top` reach the limit
+        columns[wave][lane] = s.m;
         __syncthreads();
-        const float limit = fmaxf(fmaxf(limits[0], limits[1]), fmaxf(limits[2], limits[3]));
+        if (wave == 0) {
+            const float found = keys.limit_of(fmaxf(fmaxf(s.m, columns[1][lane]), fmaxf(columns[2][lane], columns[3][lane])));
+            if (lane == 0) workgroup_limit = found;
+        }
+        __syncthreads();
+        const float limit = workgroup_limit;
         const unsigned long long key = logit_key(limit, 0xFFFFFFFFu);
         keys.threshold = key > kMaskedKey ? key : kMaskedKey;
         // the steps of sixteen that reach the limit, as step * 64 + lane, over the maxima that have been looked at
@@ -373,8 +386,8 @@ mi355q_status dispatch_token_logprobs(mi355q_context* ctx, hipStream_t s, const 
     if (dtype != MI355Q_F16 && dtype != MI355Q_BF16 && dtype != MI355Q_F32)
         return fail(MI355Q_ERR_INVALID_ARGUMENT, "unknown element type %d", dtype);
     if (!rows || !vocabulary) return fail(MI355Q_ERR_SHAPE, "no rows or an empty vocabulary");
-    if (rows > (1u << 24) || vocabulary > (1u << 30))
-        return fail(MI355Q_ERR_SHAPE, "%u rows of %u logits: at most 2^24 rows and 2^30 logits a row", rows, vocabulary);
+    if (rows >= (1u << 24) || vocabulary > (1u << 30))
+        return fail(MI355Q_ERR_SHAPE, "%u rows of %u logits: fewer than 2^24 rows and at most 2^30 logits a row", rows, vocabulary);
     if (row_stride == 0) row_stride = vocabulary;
     if (row_stride < vocabulary) return fail(MI355Q_ERR_SHAPE, "row stride %u is shorter than the vocabulary of %u", row_stride, vocabulary);
     if (top > kTopMost) return fail(MI355Q_ERR_SHAPE, "%u alternatives a row: at most %u", top, kTopMost);
@@ -387,6 +400,8 @@ mi355q_status dispatch_token_logprobs(mi355q_context* ctx, hipStream_t s, const 
     LogprobArgs a{logits, tokens, logprob, entropy, top_ids, top_logprobs,
                   rows, vocabulary, row_stride, top, 1, 0, nullptr, nullptr};
     logprob_slices(&a);
+    if ((uint64_t)a.rows * a.slices >= (1u << 24))
+        return fail(MI355Q_ERR_SHAPE, "%u rows of %u logits: too many for one launch", rows, vocabulary);
     if (record) describe_step(record, "token_logprobs", "token_logprobs", a.rows * a.slices, 1, 1, 256, 0);
     if (!run) return MI355Q_OK;
     MI355Q_HIP(hipSetDevice(ctx->device));
