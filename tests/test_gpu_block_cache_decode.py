@@ -183,3 +183,63 @@ def test_eviction_follows_the_weights_of_the_attention(pkg, ctx):
         may = set(middle[w[middle] >= limit - slack])
         mid = set(kept[h]) & set(middle)
         assert must <= mid <= may
+
+
+def test_offsets_beyond_32_bits(pkg, ctx):
+    """Blocks more than 2^32 bytes into the codes, and rows more than 2^32 elements into their tensors: the same bits as the
+    same work on a small cache and dense rows."""
+    rng = np.random.default_rng(9)
+    hd, heads, group, small, far, lengths, rows = 256, 8, 1, 12, 20000, [300, 200], [68, 2]
+    total, width, stride = sum(rows), heads * group * hd, 1 << 26
+    assert far * heads * 2 * TOKENS * hd > 2 ** 32 and (total - 1) * stride > 2 ** 32
+    near = Cache(pkg, ctx, heads, hd, small, rng)
+    shift = far - small
+    sizes = [heads * 2 * TOKENS * hd, heads * 2 * 4, heads * TOKENS * 4]                 # bytes of a block
+    big = [ctx.alloc(far * n) for n in sizes]
+    parts = [pkg.DeviceBuffer(ctx, b.offset(shift * n), small * n) for b, n in zip(big, sizes)]
+    for part, own in zip(parts, (near.d_codes, near.d_scales, near.d_sums)):
+        ctx.copy(part, own, own.nbytes)
+    ctx.synchronize()
+    cache = pkg.KVBlockCache(heads, hd, far, *big)
+    tables = [[0, 3, 1, 5, 2], [4, 9, 6, 7]]
+    seqs = sequences(pkg, ctx, tables, lengths, rows), sequences(pkg, ctx, [[b + shift for b in t] for t in tables], lengths, rows)
+    q, k, v = (act_to_device_array(rng.standard_normal((total, width)).astype(np.float32), pkg.BF16, pkg) for _ in range(3))
+    dense = [ctx.upload(x) for x in (q, k, v)] + [ctx.alloc(total * width * 2) for _ in range(3)]
+    wide = ctx.alloc(total * stride * 2)                     # q, k, v, output and the rows read back, side by side
+    columns = [pkg.DeviceBuffer(ctx, wide.offset(i * width * 2), 0) for i in range(6)]
+    for column, x in zip(columns, (q, k, v)):
+        for r in range(total):
+            pkg.DeviceBuffer(ctx, column.offset(r * stride * 2), width * 2).upload(x[r])
+    for c, seq, bufs, step in ((near.c, seqs[0], dense, 0), (cache, seqs[1], columns, stride)):
+        ctx.kv_block_append(c, seq, bufs[1], bufs[2], pkg.BF16, step)
+        ctx.kv_block_attention(c, seq, bufs[0], pkg.BF16, heads * group, bufs[3], pkg.BF16, hd ** -0.5, accumulate_weights=True,
+                               q_row_stride=step, out_row_stride=step)
+        ctx.kv_block_read(c, seq, bufs[4], bufs[5], pkg.BF16, step)
+    ctx.synchronize()
+    for i in (3, 4, 5):
+        want = dense[i].download(np.uint16, (total, width))
+        for r in range(total):
+            got = pkg.DeviceBuffer(ctx, columns[i].offset(r * stride * 2), width * 2).download(np.uint16)
+            assert np.array_equal(got, want[r]), f"tensor {i}, row {r}"
+    for part, own in zip(parts, (near.d_codes, near.d_scales, near.d_sums)):
+        assert np.array_equal(part.download(np.uint8), own.download(np.uint8))
+    new = np.array([[8, 10], [11, -1]], np.int32)
+    far_new = np.where(new < 0, far, new + shift).astype(np.int32)
+    for c, seq, table in ((near.c, seqs[0], new), (cache, seqs[1], far_new)):
+        ctx.kv_block_evict(c, seq, 100, ctx.upload(table), 2, ctx.alloc(8), 10, 4)
+    ctx.synchronize()
+    for part, own in zip(parts, (near.d_codes, near.d_scales, near.d_sums)):
+        assert np.array_equal(part.download(np.uint8), own.download(np.uint8))
+    vocabulary, pitch = 5000, stride // 2
+    logits = rng.standard_normal((total, vocabulary)).astype(np.float32)
+    for r in range(total):
+        pkg.DeviceBuffer(ctx, wide.offset(r * pitch * 4), vocabulary * 4).upload(logits[r])
+    results = []
+    for buf, step in ((ctx.upload(logits), 0), (wide, pitch)):
+        ids, tops, entropy = ctx.alloc(total * 12), ctx.alloc(total * 12), ctx.alloc(total * 4)
+        ctx.token_logprobs(buf, pkg.F32, total, vocabulary, None, 3, None, entropy, ids, tops, step)
+        ctx.synchronize()
+        results.append((ids.download(np.int32), tops.download(np.float32), entropy.download(np.float32)))
+    assert all(np.array_equal(a, b) for a, b in zip(*results))
+    for b in big + [wide] + dense:
+        b.free()
