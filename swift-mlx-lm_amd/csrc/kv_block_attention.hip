@@ -47,10 +47,15 @@ struct AttentionArgs {
     // and what each of `sum_parts` shares of the rows adds, [share][sequence * kv_heads + head][sum_stride]
     float* sums;
     uint32_t sum_parts, sum_stride;
+    // many rows in spans (null: a workgroup takes one tile): for [head][sequence][tile] the workgroup that begins the tile
+    // and the number of parts it is in, workgroups of a head, and the smallest span in units of one block
+    int2* spans;
+    uint32_t span_count, span_least;
 };
 
 constexpr float kLowest = -3.402823466e38f;
-constexpr uint32_t kFewParts = 4;
+constexpr uint32_t kFewParts = 8;
+constexpr uint32_t kLeastSpan = 6;                    // blocks of a workgroup's span at least
 constexpr uint32_t kMostParts = 128;                  // parts that the visible blocks of a row tile are split into
 constexpr float kRaise = 8.0f, kHeadroom = 6.0f;      // log2: how far scores may pass m, and p = 2^6 at the maximum
 
@@ -73,6 +78,22 @@ __device__ __forceinline__ RowRange row_range(const AttentionArgs& a, const KvSe
 __device__ __forceinline__ uint32_t part_count(const AttentionArgs& a, const RowRange& g) {
     const uint32_t blocks = (uint32_t)(g.last - g.first);
     return blocks <= a.part_blocks ? 1u : (blocks + a.part_blocks - 1) / a.part_blocks;
+}
+// Where the partial results of a row are: row `at(p)` of part_out and part_ml.
+struct PartRows {
+    uint32_t parts;
+    size_t first, base, stride;
+    __device__ size_t at(uint32_t p) const { return p ? base + p * stride : first; }
+};
+__device__ __forceinline__ PartRows part_rows(const AttentionArgs& a, const KvSequence& s, uint32_t b, uint32_t head, uint32_t r, uint32_t rows, uint32_t tile_rows) {
+    const uint32_t tile = r / tile_rows, r0 = tile * tile_rows;
+    if (a.spans) {                                         // workgroup w leaves what it continues in slot 2 w, what it begins in 2 w + 1
+        const int2 span = a.spans[((size_t)head * a.kv.sequences + b) * a.tiles + tile];
+        const size_t base = (size_t)span.x * 2 * tile_rows + (r - r0);
+        return PartRows{(uint32_t)span.y, base + tile_rows, base, 2 * (size_t)tile_rows};
+    }
+    const size_t base = (((size_t)b * a.kv.kv_heads + head) * a.tiles + tile) * a.parts * tile_rows + (r - r0);
+    return PartRows{part_count(a, row_range(a, s, r0, min(r0 + tile_rows, rows))), base, base, tile_rows};
 }
 // the lowest position that row r's window reaches (any number below the first token without one)
 __device__ __forceinline__ int32_t row_low(const AttentionArgs& a, int32_t position) {
@@ -473,8 +494,92 @@ __device__ __forceinline__ float load_query_tile(const AttentionArgs& a, bool th
 }
 
 constexpr uint32_t kTileRows = 128;
-
+// units (blocks) that a border of a span moves to a tile's end: about what partial results and their joining cost
+template <int HD>
+constexpr uint32_t kSnapUnits = HD == 64 ? 8 : HD == 128 ? 6 : 4;
+// LDS of the blocks (two halves of a block's tokens add up in it: two rows of 64 numbers more)
 template <int HD, int TS>
+constexpr size_t tile_room() {
+    const size_t room = 2 * sizeof(TileLds<HD, 4 * TS>), halves = TS == 1 ? 0 : (size_t)4 * (HD / 2 + 2) * 256;
+    return room > halves ? room : halves;
+}
+
+// Spans: with few tiles for the chip, or tiles of very different lengths, the blocks of a head's tiles, laid end to end in
+// the order of span_tile(), are dealt out evenly to its workgroups.  A tile also counts as kTileUnits blocks for its rows, its
+// results and the way in and out of the loop.  A border that would fall within `snap` of a tile's ends moves there, so
+// tiles are not split for a few blocks.  Every workgroup finds its span from the sums of the tiles' lengths in LDS.
+constexpr uint32_t kTileUnits = 4, kMostTiles = 2048;
+
+// tiles of short and of long view in turn: their sums then follow the mean closely, and most borders lie near a tile's end
+__device__ __forceinline__ uint32_t span_tile(uint32_t i, uint32_t tiles) { return i & 1 ? tiles - 1 - i / 2 : i / 2; }
+
+struct Spans {
+    const uint32_t* sums;     // units in front of each tile, and of all
+    uint32_t count, each, snap;
+    // the tile in which unit u lies (u below the sum of all)
+    __device__ uint32_t find(uint32_t u) const {
+        uint32_t low = 0, high = count;                    // sums[low] <= u < sums[high]
+        while (high - low > 1) {
+            const uint32_t mid = (low + high) / 2;
+            if (sums[mid] <= u) low = mid;
+            else high = mid;
+        }
+        return (uint32_t)__builtin_amdgcn_readfirstlane((int)low);
+    }
+    __device__ uint32_t border(uint32_t w) const {
+        const uint64_t x = (uint64_t)w * each;
+        if (x >= sums[count]) return sums[count];
+        const uint32_t u = (uint32_t)x, i = find(u), from = sums[i], to = sums[i + 1];
+        return u - from <= snap ? from : to - u <= snap ? to : u;
+    }
+    // parts of the tile of units [from, to): one more than the borders inside it
+    __device__ uint32_t parts(uint32_t from, uint32_t to) const {
+        const uint32_t low = (from + snap) / each + 1, high = to > snap ? (to - snap - 1) / each : 0;
+        return high >= low ? high - low + 2 : 1;
+    }
+};
+
+// Units of tile i (of a.tiles for every sequence), 0 if it has no rows.
+__device__ __forceinline__ uint32_t tile_units(const AttentionArgs& a, uint32_t i) {
+    const uint32_t b = i / a.tiles, at = i - b * a.tiles;
+    const KvSequence s = kv_sequence(a.kv, b);
+    const uint32_t rows = (uint32_t)s.rows * a.group, tiles = (rows + kTileRows - 1) / kTileRows;
+    if (at >= tiles) return 0;
+    const uint32_t r0 = span_tile(at, tiles) * kTileRows;
+    const RowRange g = row_range(a, s, r0, min(r0 + kTileRows, rows));
+    return (uint32_t)(g.last - g.first) + kTileUnits;
+}
+
+// Sums of the tiles' units into `sums`, by all threads of the workgroup.
+template <uint32_t THREADS>
+__device__ __forceinline__ void sum_units(const AttentionArgs& a, uint32_t count, uint32_t* sums, uint32_t* wave_sums) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t before = 0;
+    if (threadIdx.x == 0) sums[0] = 0;
+    for (uint32_t first = 0; first < count; first += THREADS) {
+        const uint32_t i = first + threadIdx.x;
+        uint32_t sum = i < count ? tile_units(a, i) : 0;
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) {
+            const uint32_t x = (uint32_t)__shfl_up((int)sum, o);
+            sum += lane >= (uint32_t)o ? x : 0;
+        }
+        __syncthreads();
+        if (lane == 63) wave_sums[wave] = sum;
+        __syncthreads();
+        uint32_t all = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < THREADS / 64; w++) {
+            if (w == wave) sum += before + all;
+            all += wave_sums[w];
+        }
+        if (i < count) sums[i + 1] = sum;
+        before += all;
+    }
+    __syncthreads();
+}
+
+template <int HD, int TS, bool SPANS>
 __global__ __launch_bounds__(256 * TS, 2) void kv_block_attention_tiles_kernel(AttentionArgs a) {
     constexpr int S = HD / 64, DT = HD / 32, WAVES = 4 * TS, TT = 2 / TS;      // TT: 32-token halves of a wavefront
     constexpr uint32_t ROWS = kTileRows;
@@ -482,167 +587,207 @@ __global__ __launch_bounds__(256 * TS, 2) void kv_block_attention_tiles_kernel(A
     TileLds<HD, WAVES>* const lds = (TileLds<HD, WAVES>*)lds_raw;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
     const uint32_t n = lane & 31, h = lane >> 5, group = wave & 3, share = wave >> 2;      // rows, and which half of the tokens
-    // the last rows of a prompt see most: they start first
-    const uint32_t head = blockIdx.x % a.kv.kv_heads, part = blockIdx.x / a.kv.kv_heads, tile = gridDim.y - 1 - blockIdx.y, b = blockIdx.z;
-    const KvSequence s = kv_sequence(a.kv, b);
-    const uint32_t rows = (uint32_t)s.rows * a.group, r0 = tile * ROWS;
-    if (r0 >= rows) return;
-    const uint32_t r1 = min(r0 + ROWS, rows);
-    const RowRange g = row_range(a, s, r0, r1);
-    const uint32_t parts = part_count(a, g);
-    if (part >= parts) return;
-    const int32_t begin = g.first + (int32_t)(part * a.part_blocks), end = min(begin + (int32_t)a.part_blocks, g.last);
-
-    const uint32_t w0 = r0 + group * 32, r = w0 + n, token = r / a.group, out_head = head * a.group + r % a.group;
-    const bool working = w0 < r1;                          // a wavefront without rows only moves blocks
-    const int32_t position = s.first() + (int32_t)token, low = row_low(a, position);
-    const RowRange own = row_range(a, s, w0, working ? min(w0 + 32, r1) : w0 + 1);
-    half8 q[S][2][2];
-    const float factor = load_query_tile<HD>(a, r < r1, r < r1 ? (size_t)(s.row0 + (int32_t)token) * a.q_stride + (size_t)out_head * HD : 0, h, q);
-    float m = kLowest, l = 0.0f;
-    floatx16 o[DT];
-#pragma unroll
-    for (int d = 0; d < DT; d++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
-
-    if (a.operands && part == 0 && working && share == 0) {              // for the weight sums: the rows as they are multiplied
-        const size_t at = ((size_t)b * a.kv.kv_heads + head) * a.operand_tiles + w0 / 32;
-#pragma unroll
-        for (int k = 0; k < HD / 16; k++) a.operands[(at * (HD / 16) + k) * 64 + lane] = __builtin_bit_cast(u32x4, q[k >> 2][(k >> 1) & 1][k & 1]);
-        if (h == 0) a.factors[at * 32 + n] = factor;
+    const uint32_t head = blockIdx.x % a.kv.kv_heads;
+    // the workgroup's units [unit, unit_end), or its one tile
+    Spans spans{};
+    uint32_t unit = 0, unit_end = 1, owner = 0;
+    if constexpr (SPANS) {
+        uint32_t* const sums = (uint32_t*)(lds_raw + tile_room<HD, TS>());
+        const uint32_t w = blockIdx.x / a.kv.kv_heads, count = a.tiles * a.kv.sequences;
+        sum_units<256 * TS>(a, count, sums, (uint32_t*)lds_raw);
+        spans = Spans{sums, count, max((sums[count] + a.span_count - 1) / a.span_count, a.span_least), 0};
+        spans.snap = max(min(kSnapUnits<HD>, spans.each / 4), kTileUnits);
+        unit = (uint32_t)__builtin_amdgcn_readfirstlane((int)spans.border(w));
+        unit_end = (uint32_t)__builtin_amdgcn_readfirstlane((int)spans.border(w + 1));
+        owner = head * a.span_count + w;
+        if (unit == unit_end) return;
     }
-    TileLoader<HD, WAVES> raw;
-    BlockScales scales[2] = {};
-    int32_t id[2] = {-1, -1};
-    auto fetch = [&](int32_t j, int slot) {                // (a block that is absent loads block 0 and is masked)
-        id[slot] = scalar_block_id(a.kv, s.table, j);
-        raw.load(a, id[slot] < 0 ? 0 : id[slot], head, tid);
-        scales[slot] = scalar_scales(a.kv, id[slot], head);
-    };
-    if (begin < end) {
-        fetch(begin, 0);
-        raw.store(lds[0], tid);
-        if (begin + 1 < end) fetch(begin + 1, 1);
-    }
-    __syncthreads();
-    auto step = [&](int32_t j, auto slot_) {
-        constexpr int slot = decltype(slot_)::value;
-        const TileLds<HD, WAVES>& cur = lds[slot];
-        const BlockScales now = scales[slot];
-        const int32_t id_now = id[slot];
-        const int32_t base = j * (int32_t)kKvTokens;
-        const bool visible = working && id_now >= 0 && j >= own.first && j < own.last;
-        floatx16 x[TT];
-        const uint32_t key_lane = share * (HD / 16) * 64 + lane, value_lane = share * 2 * 64 + lane;
-        if (visible) {
-#pragma unroll
-            for (int t = 0; t < TT; t++) {
-#pragma unroll
-                for (int i = 0; i < 16; i++) x[t][i] = 0.0f;
-#pragma unroll
-                for (int k = 0; k < HD / 16; k++)
-                    x[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, cur.key[(t * (HD / 16) + k) * 64 + key_lane]),
-                                                                  q[k >> 2][(k >> 1) & 1][k & 1], x[t], 0, 0, 0);
-            }
+    do {
+        // the last rows of a prompt see most: without spans they start first
+        uint32_t b = blockIdx.z, tile = gridDim.y - 1 - blockIdx.y, from = 0, to = 1;
+        if constexpr (SPANS) {
+            const uint32_t i = spans.find(unit);
+            from = (uint32_t)__builtin_amdgcn_readfirstlane((int)spans.sums[i]);
+            to = (uint32_t)__builtin_amdgcn_readfirstlane((int)spans.sums[i + 1]);
+            b = i / a.tiles;
+            tile = i - b * a.tiles;
         }
-        if (j + 1 < end) raw.store(lds[slot ^ 1], tid);
-        if (j + 2 < end) fetch(j + 2, slot);
-        if (visible) {
-            const float f = fmaxf(factor * now.key, 1e-37f);      // (a masked score times it stays -inf)
-            const float vlog = now.value > 0.0f ? log2f(now.value) : 0.0f, vinv = exp2f(-vlog);
-            if (!(base + 63 <= own.low && (!a.window || base >= row_low(a, own.high)))) {
+        const KvSequence s = kv_sequence(a.kv, b);
+        const uint32_t rows = (uint32_t)s.rows * a.group;
+        if constexpr (SPANS) tile = span_tile(tile, (rows + ROWS - 1) / ROWS);
+        const uint32_t r0 = tile * ROWS;
+        if (r0 >= rows) return;
+        const uint32_t r1 = min(r0 + ROWS, rows);
+        const RowRange g = row_range(a, s, r0, r1);
+        int32_t begin = g.first, end = g.last;
+        bool whole = true, first_part = true;
+        uint32_t slot = 0;
+        if constexpr (SPANS) {
+            first_part = unit == from;
+            const bool last_part = to <= unit_end;
+            if (!first_part) begin = g.first + (int32_t)(unit - from - kTileUnits);
+            if (!last_part) end = g.first + (int32_t)(unit_end - from - kTileUnits);
+            whole = first_part && last_part;
+            slot = 2 * owner + (first_part ? 1u : 0u);
+            if (first_part && tid == 0) a.spans[((size_t)head * a.kv.sequences + b) * a.tiles + tile] = make_int2((int)owner, (int)spans.parts(from, to));
+        }
+
+        const uint32_t w0 = r0 + group * 32, r = w0 + n, token = r / a.group, out_head = head * a.group + r % a.group;
+        const bool working = w0 < r1;                          // a wavefront without rows only moves blocks
+        const int32_t position = s.first() + (int32_t)token, low = row_low(a, position);
+        const RowRange own = row_range(a, s, w0, working ? min(w0 + 32, r1) : w0 + 1);
+        half8 q[S][2][2];
+        const float factor = load_query_tile<HD>(a, r < r1, r < r1 ? (size_t)(s.row0 + (int32_t)token) * a.q_stride + (size_t)out_head * HD : 0, h, q);
+        float m = kLowest, l = 0.0f;
+        floatx16 o[DT];
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+
+        if (a.operands && first_part && working && share == 0) {             // for the weight sums: the rows as they are multiplied
+            const size_t at = ((size_t)b * a.kv.kv_heads + head) * a.operand_tiles + w0 / 32;
+#pragma unroll
+            for (int k = 0; k < HD / 16; k++) a.operands[(at * (HD / 16) + k) * 64 + lane] = __builtin_bit_cast(u32x4, q[k >> 2][(k >> 1) & 1][k & 1]);
+            if (h == 0) a.factors[at * 32 + n] = factor;
+        }
+        TileLoader<HD, WAVES> raw;
+        BlockScales scales[2] = {};
+        int32_t id[2] = {-1, -1};
+        auto fetch = [&](int32_t j, int slot) {                // (a block that is absent loads block 0 and is masked)
+            id[slot] = scalar_block_id(a.kv, s.table, j);
+            raw.load(a, id[slot] < 0 ? 0 : id[slot], head, tid);
+            scales[slot] = scalar_scales(a.kv, id[slot], head);
+        };
+        if (begin < end) {
+            fetch(begin, 0);
+            raw.store(lds[0], tid);
+            if (begin + 1 < end) fetch(begin + 1, 1);
+        }
+        __syncthreads();
+        auto step = [&](int32_t j, auto slot_) {
+            constexpr int slot = decltype(slot_)::value;
+            const TileLds<HD, WAVES>& cur = lds[slot];
+            const BlockScales now = scales[slot];
+            const int32_t id_now = id[slot];
+            const int32_t base = j * (int32_t)kKvTokens;
+            const bool visible = working && id_now >= 0 && j >= own.first && j < own.last;
+            floatx16 x[TT];
+            const uint32_t key_lane = share * (HD / 16) * 64 + lane, value_lane = share * 2 * 64 + lane;
+            if (visible) {
+#pragma unroll
+                for (int t = 0; t < TT; t++) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) x[t][i] = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < HD / 16; k++)
+                        x[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, cur.key[(t * (HD / 16) + k) * 64 + key_lane]),
+                                                                      q[k >> 2][(k >> 1) & 1][k & 1], x[t], 0, 0, 0);
+                }
+            }
+            if (j + 1 < end) raw.store(lds[slot ^ 1], tid);
+            if (j + 2 < end) fetch(j + 2, slot);
+            if (visible) {
+                const float f = fmaxf(factor * now.key, 1e-37f);      // (a masked score times it stays -inf)
+                const float vlog = now.value > 0.0f ? log2f(now.value) : 0.0f, vinv = exp2f(-vlog);
+                if (!(base + 63 <= own.low && (!a.window || base >= row_low(a, own.high)))) {
+#pragma unroll
+                    for (int t = 0; t < TT; t++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const int32_t at = base + (int32_t)(t + share) * 32 + (i >> 2) * 8 + (int32_t)h * 4 + (i & 3);
+                            x[t][i] = at >= low && at <= position ? x[t][i] : -INFINITY;
+                        }
+                }
+                float top = x[0][0];
+#pragma unroll
+                for (int i = 1; i < 16 * TT; i++) top = fmaxf(top, x[i >> 4][i & 15]);
+                top = top * f + (vlog - kHeadroom);
+                if (__ballot(top > m + kRaise)) {
+                    const float raised = fmaxf(m, fmaxf(top, lane_xor<32>(top)));
+                    const float shrink = exp2f(m - raised);
+                    l *= shrink;
+#pragma unroll
+                    for (int d = 0; d < DT; d++) o[d] *= shrink;
+                    m = raised;
+                }
+                const float shift = vlog - m;
+                float sum = 0.0f;
+                half8 p[TT][2];
 #pragma unroll
                 for (int t = 0; t < TT; t++)
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        const int32_t at = base + (int32_t)(t + share) * 32 + (i >> 2) * 8 + (int32_t)h * 4 + (i & 3);
-                        x[t][i] = at >= low && at <= position ? x[t][i] : -INFINITY;
+                        const float w = __builtin_amdgcn_exp2f(fmaf(x[t][i], f, shift));
+                        sum += w;
+                        p[t][(i >> 2) & 1][(i >> 3) * 4 + (i & 3)] = (_Float16)w;
                     }
+                l += sum * vinv;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int k = 0; k < 2 * TT; k++)
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, cur.value[(d * 4 + k) * 64 + value_lane]),
+                                                                      p[k >> 1][k & 1], o[d], 0, 0, 0);
             }
-            float top = x[0][0];
-#pragma unroll
-            for (int i = 1; i < 16 * TT; i++) top = fmaxf(top, x[i >> 4][i & 15]);
-            top = top * f + (vlog - kHeadroom);
-            if (__ballot(top > m + kRaise)) {
-                const float raised = fmaxf(m, fmaxf(top, lane_xor<32>(top)));
-                const float shrink = exp2f(m - raised);
-                l *= shrink;
-#pragma unroll
-                for (int d = 0; d < DT; d++) o[d] *= shrink;
-                m = raised;
-            }
-            const float shift = vlog - m;
-            float sum = 0.0f;
-            half8 p[TT][2];
-#pragma unroll
-            for (int t = 0; t < TT; t++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const float w = __builtin_amdgcn_exp2f(fmaf(x[t][i], f, shift));
-                    sum += w;
-                    p[t][(i >> 2) & 1][(i >> 3) * 4 + (i & 3)] = (_Float16)w;
-                }
-            l += sum * vinv;
-#pragma unroll
-            for (int d = 0; d < DT; d++)
-#pragma unroll
-                for (int k = 0; k < 2 * TT; k++)
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, cur.value[(d * 4 + k) * 64 + value_lane]),
-                                                                  p[k >> 1][k & 1], o[d], 0, 0, 0);
+            __syncthreads();
+        };
+        for (int32_t j = begin; j < end; j += 2) {
+            step(j, std::integral_constant<int, 0>{});
+            if (j + 1 < end) step(j + 1, std::integral_constant<int, 1>{});
         }
-        __syncthreads();
-    };
-    for (int32_t j = begin; j < end; j += 2) {
-        step(j, std::integral_constant<int, 0>{});
-        if (j + 1 < end) step(j + 1, std::integral_constant<int, 1>{});
-    }
 
-    l += lane_xor<32>(l);
-    if constexpr (TS == 2) {                               // the second half's results to the first, over the blocks' LDS
-        float* const other = (float*)lds_raw + group * (DT * 16 + 2) * 64;
-        if (share) {
+        l += lane_xor<32>(l);
+        if constexpr (TS == 2) {                               // the second half's results to the first, over the blocks' LDS
+            float* const other = (float*)lds_raw + group * (DT * 16 + 2) * 64;
+            if (share) {
 #pragma unroll
-            for (int d = 0; d < DT; d++)
+                for (int d = 0; d < DT; d++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) other[(d * 16 + i) * 64 + lane] = o[d][i];
-            other[DT * 16 * 64 + lane] = m;
-            other[(DT * 16 + 1) * 64 + lane] = l;
+                    for (int i = 0; i < 16; i++) other[(d * 16 + i) * 64 + lane] = o[d][i];
+                other[DT * 16 * 64 + lane] = m;
+                other[(DT * 16 + 1) * 64 + lane] = l;
+            }
+            __syncthreads();
+            if (!share) {
+                const float om = other[DT * 16 * 64 + lane], top = fmaxf(m, om), f0 = exp2f(m - top), f1 = exp2f(om - top);
+                l = l * f0 + other[(DT * 16 + 1) * 64 + lane] * f1;
+                m = top;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) o[d][i] = o[d][i] * f0 + other[(d * 16 + i) * 64 + lane] * f1;
+            }
         }
-        __syncthreads();
-        if (share) return;
-        const float om = other[DT * 16 * 64 + lane], top = fmaxf(m, om), f0 = exp2f(m - top), f1 = exp2f(om - top);
-        l = l * f0 + other[(DT * 16 + 1) * 64 + lane] * f1;
-        m = top;
+        if (r < r1 && !share) {
+            if (whole) {
+                const size_t row = (size_t)(s.row0 + (int32_t)token);
+                const float f = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-        for (int d = 0; d < DT; d++)
+                for (int d = 0; d < DT; d++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) o[d][i] = o[d][i] * f0 + other[(d * 16 + i) * 64 + lane] * f1;
-    }
-    if (r >= r1) return;
-    if (parts > 1) {
-        const size_t slot = ((((size_t)b * a.kv.kv_heads + head) * a.tiles + tile) * a.parts + part) * ROWS + (r - r0);
+                    for (int i = 0; i < 4; i++)
+                        store_row4(a, row * a.out_stride + (size_t)out_head * HD + d * 32 + i * 8 + h * 4,
+                                   floatx4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]}, f);
+                if (h == 0) {
+                    const float lse2 = l == 0.0f ? -INFINITY : m + log2f(l);
+                    if (a.lse) a.lse[row * a.heads + out_head] = lse2 * 0.6931471805599453f;
+                    if (a.lse2) a.lse2[((size_t)b * a.kv.kv_heads + head) * a.score_rows + r] = lse2;
+                }
+            } else {
+                const size_t at = (size_t)slot * ROWS + (r - r0);
 #pragma unroll
-        for (int d = 0; d < DT; d++)
+                for (int d = 0; d < DT; d++)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                *(floatx4*)(a.part_out + slot * HD + d * 32 + i * 8 + h * 4) = floatx4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-        if (h == 0) a.part_ml[slot] = make_float2(m, l);
-        return;
-    }
-    const size_t row = (size_t)(s.row0 + (int32_t)token);
-    const float f = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-    for (int d = 0; d < DT; d++)
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            store_row4(a, row * a.out_stride + (size_t)out_head * HD + d * 32 + i * 8 + h * 4,
-                       floatx4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]}, f);
-    if (h == 0) {
-        const float lse2 = l == 0.0f ? -INFINITY : m + log2f(l);
-        if (a.lse) a.lse[row * a.heads + out_head] = lse2 * 0.6931471805599453f;
-        if (a.lse2) a.lse2[((size_t)b * a.kv.kv_heads + head) * a.score_rows + r] = lse2;
-    }
+                    for (int i = 0; i < 4; i++)
+                        *(floatx4*)(a.part_out + at * HD + d * 32 + i * 8 + h * 4) = floatx4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+                if (h == 0) a.part_ml[at] = make_float2(m, l);
+            }
+        }
+        if constexpr (!SPANS) return;
+        unit = min(to, unit_end);
+        __syncthreads();                                   // the next tile's blocks go where this one's results may still be read
+    } while (unit < unit_end);
 }
 
 // Weight sums of many rows: the scores are computed again, tokens against all rows that see them.  A wavefront holds the
@@ -755,64 +900,14 @@ __global__ __launch_bounds__(256) void kv_block_weights_add_kernel(AttentionArgs
     kv_sums(a.kv, id, head)[t % (int32_t)kKvTokens] += sum;
 }
 
-// Joins few parts (kFewParts at most) of a row: one wavefront per row, added in order.
-template <int HD>
-__global__ __launch_bounds__(256) void kv_block_attention_join_few_kernel(AttentionArgs a, uint32_t tile_rows) {
-    constexpr int E = HD / 64;
-    const uint32_t lane = threadIdx.x & 63, head = blockIdx.y, b = blockIdx.z;
-    const uint32_t r = (uint32_t)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
-    const KvSequence s = kv_sequence(a.kv, b);
-    const uint32_t rows = (uint32_t)s.rows * a.group;
-    if (r >= rows) return;
-    const uint32_t tile = r / tile_rows, r0 = tile * tile_rows;
-    const uint32_t parts = part_count(a, row_range(a, s, r0, min(r0 + tile_rows, rows)));
-    if (parts == 1) return;
-    const size_t slot = (((size_t)b * a.kv.kv_heads + head) * a.tiles + tile) * a.parts * tile_rows + (r - r0);
-    float2 ml[kFewParts];
-    float x[kFewParts][E], top = kLowest;
-#pragma unroll
-    for (uint32_t p = 0; p < kFewParts; p++) {
-        const size_t at = slot + (size_t)(p < parts ? p : 0) * tile_rows;
-        ml[p] = a.part_ml[at];
-        if (p >= parts) ml[p] = make_float2(kLowest, 0.0f);
-#pragma unroll
-        for (int e = 0; e < E; e++) x[p][e] = a.part_out[at * HD + e * 64 + lane];
-        top = fmaxf(top, ml[p].x);
-    }
-    float l = 0.0f, o[E];
-#pragma unroll
-    for (int e = 0; e < E; e++) o[e] = 0.0f;
-#pragma unroll
-    for (uint32_t p = 0; p < kFewParts; p++) {
-        const float f = p < parts ? exp2f(ml[p].x - top) : 0.0f;
-        l += ml[p].y * f;
-#pragma unroll
-        for (int e = 0; e < E; e++) o[e] += x[p][e] * f;
-    }
-    const uint32_t token = r / a.group, h = head * a.group + r % a.group;
-    const size_t row = (size_t)(s.row0 + (int32_t)token);
-    const float f = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        const size_t at = row * a.out_stride + (size_t)h * HD + e * 64 + lane;
-        if (a.out_dtype == MI355Q_BF16) ((uint16_t*)a.out)[at] = f32_to_bf16_rne(o[e] * f);
-        else ((uint16_t*)a.out)[at] = f32_to_f16_rne(o[e] * f);
-    }
-    if (lane == 0) {
-        const float lse2 = l == 0.0f ? -INFINITY : top + log2f(l);
-        if (a.lse) a.lse[row * a.heads + h] = lse2 * 0.6931471805599453f;
-        if (a.lse2) a.lse2[((size_t)b * a.kv.kv_heads + head) * a.score_rows + r] = lse2;
-    }
-}
-
 // The common maximum and the sum of a row's parts, by a wavefront: (m, l) of the row at the same units, and each part's
 // factor 2^(m_part - m) for the lanes' parts.
-__device__ __forceinline__ float2 join_sums(const float2* ml_at, uint32_t parts, uint32_t tile_rows, uint32_t lane, float (&f)[kMostParts / 64]) {
+__device__ __forceinline__ float2 join_sums(const float2* part_ml, const PartRows& part, uint32_t lane, float (&f)[kMostParts / 64]) {
     float2 ml[kMostParts / 64];
     float top = kLowest;
 #pragma unroll
     for (uint32_t i = 0; i < kMostParts / 64; i++) {
-        ml[i] = i * 64 + lane < parts ? ml_at[(size_t)(i * 64 + lane) * tile_rows] : make_float2(kLowest, 0.0f);
+        ml[i] = i * 64 + lane < part.parts ? part_ml[part.at(i * 64 + lane)] : make_float2(kLowest, 0.0f);
         top = fmaxf(top, ml[i].x);
     }
     top = max_across(top, lane);
@@ -826,6 +921,60 @@ __device__ __forceinline__ float2 join_sums(const float2* ml_at, uint32_t parts,
     return make_float2(top, wave_reduce_sum(l));
 }
 
+// Joins the parts of rows, a wavefront per R rows of one tile, kFewParts parts at a time, added in order.
+template <int HD, int R>
+__global__ __launch_bounds__(256) void kv_block_attention_join_few_kernel(AttentionArgs a, uint32_t tile_rows) {
+    constexpr int E = HD / 64;
+    const uint32_t lane = threadIdx.x & 63, head = blockIdx.y, b = blockIdx.z;
+    const uint32_t r0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)((blockIdx.x * 4 + (threadIdx.x >> 6)) * R));
+    const KvSequence s = kv_sequence(a.kv, b);
+    const uint32_t rows = (uint32_t)s.rows * a.group;
+    if (r0 >= rows) return;
+    PartRows part = part_rows(a, s, b, head, r0, rows, tile_rows);
+    if (part.parts == 1) return;
+    const uint32_t end = min(r0 + R, rows);
+    for (uint32_t r = r0; r < end; r++, part.first++, part.base++) {
+        float x[kFewParts][E], f[kMostParts / 64], o[E];
+        auto load = [&](uint32_t first) {
+#pragma unroll
+            for (uint32_t p = 0; p < kFewParts; p++)
+                if (first + p < part.parts) {
+                    const size_t at = part.at(first + p) * HD + lane;
+#pragma unroll
+                    for (int e = 0; e < E; e++) x[p][e] = a.part_out[at + e * 64];
+                }
+        };
+        load(0);
+        const float2 ml = join_sums(a.part_ml, part, lane, f);
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] = 0.0f;
+        for (uint32_t first = 0; first < part.parts; first += kFewParts) {
+            if (first) load(first);
+#pragma unroll
+            for (uint32_t p = 0; p < kFewParts; p++)
+                if (first + p < part.parts) {
+                    const float w = __shfl(first < 64 ? f[0] : f[1], (int)((first + p) & 63));
+#pragma unroll
+                    for (int e = 0; e < E; e++) o[e] += x[p][e] * w;
+                }
+        }
+        const uint32_t token = r / a.group, h = head * a.group + r % a.group;
+        const size_t row = (size_t)(s.row0 + (int32_t)token);
+        const float scale = ml.y == 0.0f ? 0.0f : 1.0f / ml.y;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const size_t at = row * a.out_stride + (size_t)h * HD + e * 64 + lane;
+            if (a.out_dtype == MI355Q_BF16) ((uint16_t*)a.out)[at] = f32_to_bf16_rne(o[e] * scale);
+            else ((uint16_t*)a.out)[at] = f32_to_f16_rne(o[e] * scale);
+        }
+        if (lane == 0) {
+            const float lse2 = ml.y == 0.0f ? -INFINITY : ml.x + log2f(ml.y);
+            if (a.lse) a.lse[row * a.heads + h] = lse2 * 0.6931471805599453f;
+            if (a.lse2) a.lse2[((size_t)b * a.kv.kv_heads + head) * a.score_rows + r] = lse2;
+        }
+    }
+}
+
 // Joins the parts of a row: one workgroup per row, 1024 / HD parts at a time, added in a fixed order.
 template <int HD>
 __device__ __forceinline__ void join_row(const AttentionArgs& a, uint32_t tile_rows, uint32_t r, uint32_t head, uint32_t b, floatx4* lds_out, float* lds_f) {
@@ -834,12 +983,10 @@ __device__ __forceinline__ void join_row(const AttentionArgs& a, uint32_t tile_r
     const KvSequence s = kv_sequence(a.kv, b);
     const uint32_t rows = (uint32_t)s.rows * a.group;
     if (r >= rows) return;
-    const uint32_t tile = r / tile_rows, r0 = tile * tile_rows;
-    const uint32_t parts = part_count(a, row_range(a, s, r0, min(r0 + tile_rows, rows)));
-    if (parts == 1) return;
-    const size_t slot = (((size_t)b * a.kv.kv_heads + head) * a.tiles + tile) * a.parts * tile_rows + (r - r0);
+    const PartRows part = part_rows(a, s, b, head, r, rows, tile_rows);
+    if (part.parts == 1) return;
     float f[kMostParts / 64];
-    const float2 ml = join_sums(a.part_ml + slot, parts, tile_rows, lane, f);
+    const float2 ml = join_sums(a.part_ml, part, lane, f);
 #pragma unroll
     for (uint32_t i = 0; i < kMostParts / 64; i++)
         if (tid < 64) lds_f[i * 64 + lane] = f[i];
@@ -847,8 +994,8 @@ __device__ __forceinline__ void join_row(const AttentionArgs& a, uint32_t tile_r
     floatx4 o = {0, 0, 0, 0};
     const uint32_t d = tid % LANES * 4;
 #pragma unroll 4
-    for (uint32_t p = tid / LANES; p < parts; p += AT_ONCE)
-        o += *(const floatx4*)(a.part_out + (slot + (size_t)p * tile_rows) * HD + d) * lds_f[p];
+    for (uint32_t p = tid / LANES; p < part.parts; p += AT_ONCE)
+        o += *(const floatx4*)(a.part_out + part.at(p) * HD + d) * lds_f[p];
     lds_out[tid] = o;
     __syncthreads();
     if (tid >= LANES) return;
@@ -883,7 +1030,7 @@ __device__ __forceinline__ void weigh_tokens(const AttentionArgs& a, uint32_t ti
             lse2 = scalar_load(a.lse2 + slot * a.score_rows + r);
         } else {
             float f[kMostParts / 64];
-            const float2 ml = join_sums(a.part_ml + slot * a.parts * tile_rows + r, parts, tile_rows, lane, f);
+            const float2 ml = join_sums(a.part_ml, part_rows(a, s, b, head, r, rows, tile_rows), lane, f);
             lse2 = ml.y == 0.0f ? -INFINITY : ml.x + log2f(ml.y);
         }
         if (lane == 0) lds_lse[r] = lse2 == -INFINITY ? INFINITY : lse2;      // a row that sees nothing
@@ -934,27 +1081,30 @@ void choose_parts(AttentionArgs* a, uint64_t blocks, uint64_t groups, uint32_t w
     a->parts = (uint32_t)((blocks + a->part_blocks - 1) / a->part_blocks);
 }
 
-// The tiles kernel fills the chip with 512 workgroups.  Below that the blocks are split where it pays: a workgroup takes
-// about 1.1, 1.8 or 3.4 us a block (heads of 64, 128, 256), parts cost a launch (4 us) and their partial results in and
-// out at 4 TB/s.  (Prompts of 512, 1024 and 1500 rows, 32 heads of 128 on 8: one part 20, 33 and 46 us, as many as fill
-// the chip 25, 48 and 70; 200 rows on 5000 tokens: one part 150 us, nine 54.)
-void choose_tile_parts(AttentionArgs* a, int hd, uint64_t blocks, uint64_t groups) {
-    const double block_us = hd == 64 ? 1.1 : hd == 128 ? 1.8 : 3.4, part_us = (double)groups * kTileRows * hd * 8 / 4e6;
-    const uint64_t most = std::max<uint64_t>(1, std::min<uint64_t>({512 / groups, blocks, kMostParts}));
-    uint64_t parts = 1;
-    double best = (double)blocks * block_us;
-    for (uint64_t p = 2; p <= most; p++) {
-        const double us = (double)((blocks + p - 1) / p) * block_us + 4.0 + (double)p * part_us;
-        if (us < best) { best = us; parts = p; }
-    }
-    a->part_blocks = (uint32_t)((blocks + parts - 1) / parts);
-    a->parts = (uint32_t)((blocks + a->part_blocks - 1) / a->part_blocks);
+// Workgroups of a head among which the tiles kernel deals the blocks, 0: a tile each.  `slots` workgroups fill the chip.  A
+// block takes a workgroup about 1.1, 1.8 or 3.2 us (heads of 64, 128, 256) on a full chip and 0.7 of that on an empty one;
+// splitting costs about 12 us and joining 20 more if all workgroups leave partial results.  Only the longest sequence is
+// known here; those of a batch are taken to be three quarters of it.
+uint32_t span_workgroups(const AttentionArgs& a, int hd, uint32_t slots) {
+    const uint64_t count = (uint64_t)a.tiles * a.kv.sequences, most = (a.kv.max_length + kKvTokens - 1) / kKvTokens + 1;
+    if (count > kMostTiles || count * (most + kTileUnits) >= (1u << 31)) return 0;
+    const double us = hd == 64 ? 1.1 : hd == 128 ? 1.8 : 3.2;
+    const double tiles = ((double)a.kv.row_count * a.group / kTileRows + a.kv.sequences) * a.kv.kv_heads / slots;
+    const double longest = (double)visible_blocks(a, kTileRows), rows = std::min(a.kv.max_rows, a.kv.max_length);
+    const double mean = std::min(longest, (a.kv.max_length - rows / 2) / kKvTokens + 1);
+    const double whole = us * std::max(longest * (0.7 + 0.3 * std::min(1.0, tiles)), tiles * mean);
+    const double each = tiles * mean * (a.kv.sequences == 1 ? 1.0 : 0.75);
+    const double spans = us * std::max(each, (double)kLeastSpan) + 12.0 + 20.0 * std::min(1.0, each / kLeastSpan);
+    return spans < whole ? std::max(1u, slots / a.kv.kv_heads) : 0;
 }
 
 template <int HD>
 mi355q_status launch_join(hipStream_t s, const AttentionArgs& a, uint32_t rows, uint32_t tile_rows) {
-    if (a.parts <= kFewParts)
-        kv_block_attention_join_few_kernel<HD><<<dim3((rows + 3) / 4, a.kv.kv_heads, a.kv.sequences), 256, 0, s>>>(a, tile_rows);
+    // (four rows a wavefront where there are many: launching the wavefronts is what it costs then)
+    if (a.spans && rows >= 1024)
+        kv_block_attention_join_few_kernel<HD, 4><<<dim3((rows + 15) / 16, a.kv.kv_heads, a.kv.sequences), 256, 0, s>>>(a, tile_rows);
+    else if (a.spans || a.parts <= kFewParts)
+        kv_block_attention_join_few_kernel<HD, 1><<<dim3((rows + 3) / 4, a.kv.kv_heads, a.kv.sequences), 256, 0, s>>>(a, tile_rows);
     else
         kv_block_attention_join_kernel<HD><<<dim3(rows, a.kv.kv_heads, a.kv.sequences), 256, 0, s>>>(a, tile_rows, rows);
     MI355Q_HIP(hipGetLastError());
@@ -967,13 +1117,13 @@ mi355q_status launch_tiles(mi355q_context* ctx, hipStream_t s, AttentionArgs a, 
     constexpr uint32_t ROWS = kTileRows;
     const uint32_t rows = a.kv.max_rows * a.group;
     a.tiles = (rows + ROWS - 1) / ROWS;
-    const uint64_t groups = (uint64_t)a.kv.kv_heads * a.tiles * a.kv.sequences;
-    choose_tile_parts(&a, HD, visible_blocks(a, ROWS), groups);
     a.score_rows = rows;
-    // (two halves of a block's tokens add up in the room of the blocks: two rows of 64 numbers more)
-    constexpr size_t room = 2 * sizeof(TileLds<HD, 4 * TS>), lds = TS == 1 ? room : std::max(room, (size_t)4 * (HD / 2 + 2) * 256);
-    if (record)
-        describe_step(record, "kv_block_attention", "kv_block_attention_tiles", a.kv.kv_heads * a.parts, a.tiles, a.kv.sequences, 256 * TS, (uint32_t)lds);
+    a.span_count = span_workgroups(a, HD, TS == 2 ? 256 : 512);
+    a.span_least = std::max(kLeastSpan, (a.kv.max_length / kKvTokens + 1) / (kMostParts - 2) + 1);
+    const uint32_t count = a.tiles * a.kv.sequences;
+    const size_t lds = tile_room<HD, TS>() + (a.span_count ? (count + 1) * 4 : 0);
+    const dim3 grid = a.span_count ? dim3(a.kv.kv_heads * a.span_count) : dim3(a.kv.kv_heads, a.tiles, a.kv.sequences);
+    if (record) describe_step(record, "kv_block_attention", "kv_block_attention_tiles", grid.x, grid.y, grid.z, 256 * TS, (uint32_t)lds);
     if (!run) return MI355Q_OK;
     MI355Q_HIP(hipSetDevice(ctx->device));
     // shares of the rows for the weight sums: about three workgroups a CU, each with eight tiles of 32 rows at least
@@ -983,9 +1133,11 @@ mi355q_status launch_tiles(mi355q_context* ctx, hipStream_t s, AttentionArgs a, 
     a.sum_parts = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({(768 + owners - 1) / owners, (rows + 255) / 256, 64}));
     for (int pass = 0; pass < 2; pass++) {
         Buffers buf{pass ? (char*)ctx->workspace : nullptr, 0};
-        if (a.parts > 1) {
-            a.part_out = buf.take<float>(groups * a.parts * ROWS * HD);
-            a.part_ml = buf.take<float2>(groups * a.parts * ROWS);
+        if (a.span_count) {
+            const size_t slots = (size_t)2 * a.kv.kv_heads * a.span_count;
+            a.part_out = buf.take<float>(slots * ROWS * HD);
+            a.part_ml = buf.take<float2>(slots * ROWS);
+            a.spans = buf.take<int2>((size_t)a.kv.kv_heads * count);
         }
         if (weights) {
             const size_t slots = (size_t)a.kv.sequences * a.kv.kv_heads;
@@ -998,10 +1150,11 @@ mi355q_status launch_tiles(mi355q_context* ctx, hipStream_t s, AttentionArgs a, 
         if (!pass && buf.used)
             if (mi355q_status st = ensure_workspace(ctx, buf.used)) return st;
     }
-    if (mi355q_status st = raise_lds_limit((const void*)kv_block_attention_tiles_kernel<HD, TS>, lds)) return st;
-    kv_block_attention_tiles_kernel<HD, TS><<<dim3(a.kv.kv_heads * a.parts, a.tiles, a.kv.sequences), 256 * TS, lds, s>>>(a);
+    auto* const kernel = a.spans ? kv_block_attention_tiles_kernel<HD, TS, true> : kv_block_attention_tiles_kernel<HD, TS, false>;
+    if (mi355q_status st = raise_lds_limit((const void*)kernel, tile_room<HD, TS>() + (kMostTiles + 1) * 4)) return st;
+    kernel<<<grid, 256 * TS, lds, s>>>(a);
     MI355Q_HIP(hipGetLastError());
-    if (a.parts > 1) {
+    if (a.spans) {
         if (mi355q_status st = launch_join<HD>(s, a, rows, ROWS)) return st;
     }
     if (weights) {

@@ -249,3 +249,46 @@ def test_refusals(pkg, ctx):
         with pytest.raises(pkg.MI355QError) as e:
             ctx.kv_block_attention(*args, **kw)
         assert e.value.status_name == status, (args, str(e.value))
+
+
+SPANS = [
+    # (head dimension, KV heads, group, lengths, rows, window): tiles of 128 rows whose blocks are dealt to the workgroups
+    (128, 1, 4, [6000], [70], 0),                              # many parts of a tile
+    (128, 2, 3, [4000, 70, 0, 1500, 300], [60, 90, 5, 1, 200], 0),      # rows in front of the first token, an empty sequence
+    (64, 3, 5, [5000, 64, 2000], [30, 64, 129], 0),
+    (256, 1, 4, [3000, 129], [40, 129], 0),
+    (256, 2, 2, [2600, 2600, 2600], [9, 30, 12], 2000),
+    (128, 1, 2, [6000, 500], [100, 20], 3000),
+]
+
+
+@pytest.mark.parametrize("hd,heads,group,lengths,rows,window", SPANS)
+def test_attention_in_spans(pkg, ctx, hd, heads, group, lengths, rows, window):
+    rng = np.random.default_rng(hd + sum(lengths) + group)
+    tables, _, blocks = deal(rng, lengths, spare=1)
+    tables[0][len(tables[0]) // 2] = -1                        # an absent block in the middle of the longest sequence
+    cache = Cache(pkg, ctx, heads, hd, blocks, rng)
+    q = (rng.standard_normal((sum(rows), heads * group, hd)) * 0.5).astype(np.float32)
+    check(pkg, ctx, cache, tables, lengths, rows, q, pkg.BF16, pkg.F16, window)
+
+
+def test_as_many_parts_as_there_can_be(pkg, ctx):
+    """One tile of a single head over 200 000 tokens: 125 parts."""
+    rng = np.random.default_rng(12)
+    hd, length, rows = 64, 200_000, 40
+    tables, _, blocks = deal(rng, [length])
+    cache = Cache(pkg, ctx, 1, hd, blocks, rng)
+    q = act_rounded((rng.standard_normal((rows, 1, hd)) * 0.5).astype(np.float32), pkg.F16, pkg)
+    seq = sequences(pkg, ctx, tables, [length], [rows])
+    out, lse = run(pkg, ctx, cache, seq, q, pkg.F16, pkg.F16, hd ** -0.5, weights=False)
+    numbers = cache.codes[tables[0], 0].astype(np.float64) * cache.scales[tables[0], 0][:, :, None, None]
+    k, v = numbers.transpose(1, 0, 2, 3).reshape(2, -1, hd)[:, :length]
+    s = q[:, 0].astype(np.float64) @ k.T * hd ** -0.5
+    s[np.arange(length)[None] > np.arange(length - rows, length)[:, None]] = -np.inf
+    m = s.max(1, keepdims=True)
+    e = np.exp(s - m)
+    total = e.sum(1, keepdims=True)
+    want = e @ v / total
+    top = 127 * cache.scales[..., 1].max()
+    assert np.all(np.abs(out[:, 0] - want) <= 2.0 ** -11 * top + 2.0 ** -11 * np.abs(want) + 1e-6)
+    assert np.all(np.abs(lse - (m + np.log(total))) <= 2e-4)
