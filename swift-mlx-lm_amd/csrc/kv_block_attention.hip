@@ -1022,15 +1022,15 @@ __device__ __forceinline__ void weigh_tokens(const AttentionArgs& a, uint32_t ti
     const RowRange g = row_range(a, s, 0, rows);
     const int32_t t = (int32_t)(chunk * 1024 + threadIdx.x * 4), j = t / (int32_t)kKvTokens;
     if ((int32_t)(chunk * 16) >= g.last || (int32_t)(chunk * 16 + 15) < g.first) return;
-    const uint32_t parts = part_count(a, g);
+    const PartRows part = part_rows(a, s, b, head, 0, rows, tile_rows);
     const size_t slot = (size_t)b * a.kv.kv_heads + head;
     for (uint32_t r = wave; r < rows; r += 4) {
         float lse2;
-        if (parts == 1) {
+        if (part.parts == 1) {
             lse2 = scalar_load(a.lse2 + slot * a.score_rows + r);
         } else {
             float f[kMostParts / 64];
-            const float2 ml = join_sums(a.part_ml, part_rows(a, s, b, head, r, rows, tile_rows), lane, f);
+            const float2 ml = join_sums(a.part_ml + r, part, lane, f);
             lse2 = ml.y == 0.0f ? -INFINITY : ml.x + log2f(ml.y);
         }
         if (lane == 0) lds_lse[r] = lse2 == -INFINITY ? INFINITY : lse2;      // a row that sees nothing
