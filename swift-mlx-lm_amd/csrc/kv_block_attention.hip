@@ -1066,7 +1066,11 @@ __global__ __launch_bounds__(256) void kv_block_attention_join_kernel(AttentionA
 namespace {
 
 // Blocks that the rows of a tile can see, and the parts they are split into so that the launch has about `wanted`
-// workgroups; a part is a multiple of `unit` blocks, one for each wavefront.
+// workgroups: as many as the chip holds at once, two a CU, or one with heads of 256.  A part is a multiple of `unit` blocks,
+// one for each wavefront.  (256 / 512 / 1024 wanted, heads of 128, 8 KV heads: 32 sequences of 2394 to 8192 tokens 69 / 61 / 63 us;
+// 64 of up to 2000 33 / 33 / 38; 16 of up to 16000 with 8 rows each 87 / 70 / 79; 131071 and 38295 tokens 67 / 69 / 62.  16 of up
+// to 16000, 4 KV heads of 256: 64 / 72 / 84.  Equal spans as for many rows, found on the device, were no faster than 512 on
+// batches of such lengths and cost 3 us where that counts.)
 uint64_t visible_blocks(const AttentionArgs& a, uint32_t tile_rows) {
     const uint64_t blocks = (a.kv.max_length + kKvTokens - 1) / kKvTokens;
     if (!a.window) return blocks;
@@ -1173,7 +1177,7 @@ mi355q_status launch_rows(mi355q_context* ctx, hipStream_t s, AttentionArgs a, b
     const uint32_t rows = a.kv.max_rows * a.group;
     a.tiles = 1;
     const uint64_t groups = (uint64_t)a.kv.kv_heads * a.kv.sequences;
-    choose_parts(&a, visible_blocks(a, 16 * RT), groups, 1024, 4);
+    choose_parts(&a, visible_blocks(a, 16 * RT), groups, HD == 256 ? 256 : 512, 4);
     if (record)
         describe_step(record, "kv_block_attention", "kv_block_attention_rows", a.kv.kv_heads * a.parts, 1, a.kv.sequences, 256, 2 * 16 * RT * HD * 4);
     if (!run) return MI355Q_OK;
