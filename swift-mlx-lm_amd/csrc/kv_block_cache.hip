@@ -12,10 +12,20 @@ namespace mi355q {
 // decided by the last bit of the scale).
 constexpr float kInverseSteps = (float)(1.0 / 127.49);
 
-// x / scale to the nearest code, half to even.  fmin and fmax drop a NaN, so it is sorted out first.
-__device__ __forceinline__ int kv_code(float x, float scale) {
-    const float q = rintf(__fdiv_rn(x, scale));
-    return x != x ? 0 : (int)fminf(fmaxf(q, -127.0f), 127.0f);
+// x / scale to the nearest code, half to even.  The quotient is the correctly rounded one, without a division for each
+// element: from `inverse`, the correctly rounded 1 / scale, one step of Newton's method on q = x inverse gives x / scale as a
+// division would round it (Markstein 1990), unless the remainder loses bits below the smallest normal number, which scales
+// under kSmallScale could bring about; those divide.  An infinite x keeps its sign through the bounds.
+constexpr float kSmallScale = 7.888609052e-31f;      // 2^-100
+__device__ __forceinline__ int kv_code(float x, float scale, float inverse) {
+    float q;
+    if (scale >= kSmallScale) {                          // the same for a whole workgroup
+        q = __builtin_amdgcn_fmed3f(x * inverse, -128.0f, 128.0f);
+        q = fmaf(fmaf(-q, scale, x), inverse, q);
+    } else {
+        q = __fdiv_rn(x, scale);
+    }
+    return x != x ? 0 : (int)__builtin_amdgcn_fmed3f(rintf(q), -127.0f, 127.0f);
 }
 
 // four codes of a word times `ratio` (at most one), each to the nearest code
@@ -100,11 +110,18 @@ __global__ __launch_bounds__(2 * HD) void kv_block_append_kernel(KvBlockArgs a, 
             const size_t row = (size_t)(s.row0 + (base + (int32_t)t - s.first()));
             load8<D>(src, row * row_stride + (size_t)head * HD + d8 * 8, vec, x[i]);
 #pragma unroll
-            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[i][e]) <= 3.402823466e38f ? fabsf(x[i][e]) : 0.0f);
+            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[i][e]));      // (drops a NaN)
         } else {
 #pragma unroll
             for (int e = 0; e < 8; e++) x[i][e] = 0.0f;
         }
+    }
+    if (__ballot(top == INFINITY)) {                       // infinities do not count
+        top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[i][e]) < INFINITY ? fabsf(x[i][e]) : 0.0f);
     }
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
@@ -115,7 +132,7 @@ __global__ __launch_bounds__(2 * HD) void kv_block_append_kernel(KvBlockArgs a, 
     for (int w = 0; w < 2 * HD / 64; w++) top = fmaxf(top, wave_top[w]);
     const float scale = fmaxf(old, top * kInverseSteps);
     int8_t* const codes = kv_codes<HD>(a, block, head, part);
-    const float divisor = scale > 0.0f ? scale : 1.0f;
+    const float divisor = scale > 0.0f ? scale : 1.0f, inverse = __fdiv_rn(1.0f, divisor);
     uint32_t c[4][2];                                      // codes of token i: dimensions 0..3, 4..7
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -123,7 +140,7 @@ __global__ __launch_bounds__(2 * HD) void kv_block_append_kernel(KvBlockArgs a, 
         for (int h = 0; h < 2; h++) {
             c[i][h] = 0;
 #pragma unroll
-            for (int e = 0; e < 4; e++) c[i][h] |= ((uint32_t)kv_code(x[i][4 * h + e], divisor) & 0xFFu) << (8 * e);
+            for (int e = 0; e < 4; e++) c[i][h] |= ((uint32_t)kv_code(x[i][4 * h + e], divisor, inverse) & 0xFFu) << (8 * e);
         }
     if (part == 0 && a.sums && tid < kKvTokens && tid >= lo && tid < hi) kv_sums(a, block, head)[tid] = 0.0f;
     if (tid == 0) *scale_at = scale;

@@ -437,3 +437,21 @@ def test_refusals(pkg, ctx):
     refused("SHAPE", ctx.kv_block_evict, cache.c, seq, 0, table, 1, lengths)
     refused("SHAPE", ctx.kv_block_evict, cache.c, seq, 65, table, 1, lengths)
     refused("SHAPE", ctx.kv_block_evict, cache.c, seq, 64, table, 1, lengths, recent=60, sinks=5)
+
+
+@pytest.mark.parametrize("size", [1e-38, 1e-36, 1e-28, 1e-4, 1.0, 1e20, 3e38])
+def test_codes_near_the_middle_of_two(pkg, ctx, size):
+    """Numbers around the middles between codes, at scales from subnormal ones to the largest: the codes of a division."""
+    rng = np.random.default_rng(8)
+    hd, length = 128, 128
+    tables, _, blocks = deal(rng, [length])
+    cache = Cache(pkg, ctx, 1, hd, blocks)
+    scale = np.float32(np.float32(size) * INVERSE)
+    x = ((rng.integers(-126, 127, (2, length, 1, hd)) + rng.choice([0.0, 0.5, 0.49], (2, length, 1, hd))) * np.float64(scale)).astype(np.float32)
+    step = rng.integers(-1, 2, x.shape)
+    x = np.where(step > 0, np.nextafter(x, np.float32(np.inf)), np.where(step < 0, np.nextafter(x, np.float32(-np.inf)), x))
+    x[:, ::64, 0, 0] = np.float32(size)                      # the largest of each block
+    k, v = (ctx.upload(np.ascontiguousarray(x[i].reshape(length, hd))) for i in range(2))
+    ctx.kv_block_append(cache.c, sequences(pkg, ctx, tables, [length], [length]), k, v, pkg.F32)
+    cache.append(tables[0], 0, x)
+    check_tokens(cache, tables, [length])
