@@ -195,7 +195,11 @@ __device__ __forceinline__ void store_row4(const AttentionArgs& a, size_t at, co
 
 // ---- few rows: decode steps and short verifications --------------------------------------------------------------------
 // A workgroup takes one KV head, 16 RT rows and one part of the visible blocks; its four wavefronts take blocks in turn,
-// each with accumulators of its own, which are added at the end.  HBM-bound.
+// each with accumulators of its own, which are added at the end.  HBM-bound: codes go from memory to registers in the order
+// the matrix cores take them, a block ahead, and every row of the group uses them.  (32 sequences of 8192 tokens, 32 heads of 128
+// on 8: 88 us, 6.1 TB/s, where a kernel that only reads reaches 7.1; of 2394 to 8192 tokens 61 us, 5.4 TB/s; 16 of up to 16000
+// tokens, 16 heads of 256 on 4, 64 us.  One sequence of 517 tokens: 6.5 us and 3 for joining, latency.)  Storing the scores for
+// the weight sums costs the second of these 14 us for 21 MB.
 template <int HD, int RT>
 __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void kv_block_attention_rows_kernel(AttentionArgs a) {
     constexpr int S = HD / 64, DT = HD / 16;
@@ -427,9 +431,12 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void kv_block_attention_row
 // block's codes are read once per workgroup, 16 bytes a lane, become f16 on the way into LDS, and lie there as the
 // fragments of 32 x 32 x 16 products, so that an operand is one conflict-free 16-byte read a lane: the loads of block
 // j + 2 and the conversion of block j + 1 overlap the products of block j.  Two wavefronts a SIMD take turns on the matrix
-// cores and the vector unit, which need about the same time.  With heads of 256 the accumulators and rows of 32 rows fill
+// cores and the vector unit, at the clock the card holds under this load (a prompt of 8192 rows, 32 heads of 128 on 8: 630 us,
+// 870 TFLOP/s of the 1130 that a product of 8192 x 8192 f16 matrices reaches here; 5001 rows: 232 us, 1.84 GHz, matrix cores busy
+// 0.43 of the cycles and the vector unit 0.6.  Scores of block j + 1 computed ahead of the softmax of block j spilt registers
+// and took longer; wave priorities for either phase changed nothing).  With heads of 256 the accumulators and rows of 32 rows fill
 // half of the register file and the blocks the LDS of a CU: there two wavefronts share their rows, each taking half of a
-// block's tokens (TS = 2), and add up their results at the end.
+// block's tokens (TS = 2), and add up their results at the end (a prompt of 4096 rows of 16 heads: 251 us without, 171 with).
 template <int HD, int WAVES>
 struct TileLds {
     u32x4 key[2 * (HD / 16) * 64];      // fragment (32-token half, sixteen dimensions)
@@ -507,7 +514,9 @@ constexpr size_t tile_room() {
 // Spans: with few tiles for the chip, or tiles of very different lengths, the blocks of a head's tiles, laid end to end in
 // the order of span_tile(), are dealt out evenly to its workgroups.  A tile also counts as kTileUnits blocks for its rows, its
 // results and the way in and out of the loop.  A border that would fall within `snap` of a tile's ends moves there, so
-// tiles are not split for a few blocks.  Every workgroup finds its span from the sums of the tiles' lengths in LDS.
+// tiles are not split for a few blocks.  Every workgroup finds its span from the sums of the tiles' lengths in LDS.  (8 chunks
+// of 75 to 300 rows on 2250 to 9000 tokens, 32 heads of 128 on 8: 217 us with tiles cut into equal numbers of parts, 155 in
+// spans; chunks of 509, 274 and 295 rows on 6309, 1968 and 2238 tokens, 16 heads of 256: 160 + 9 for joining, 115 + 13.)
 constexpr uint32_t kTileUnits = 4, kMostTiles = 2048;
 
 // tiles of short and of long view in turn: their sums then follow the mean closely, and most borders lie near a tile's end
@@ -793,8 +802,10 @@ __global__ __launch_bounds__(256 * TS, 2) void kv_block_attention_tiles_kernel(A
 // Weight sums of many rows: the scores are computed again, tokens against all rows that see them.  A wavefront holds the
 // keys of 32 tokens as operands and adds up 2^(x - lse2) over the rows, whose operands the tiles kernel left in memory and
 // which pass through LDS 32 at a time, 32 more on their way meanwhile; the sums of its lanes, which hold different rows,
-// are added at the end, so every sum is made in one fixed order.  Where there are few tokens and heads, the rows are dealt
-// to several workgroups, whose sums another launch adds in order.
+// are added at the end, so every sum is made in one fixed order.  Bound by the matrix cores with heads of 256 and by the
+// exponentials, a vector instruction of four times the length for each score, with heads of 64 (the three chunks of 256: 50 us).
+// A wavefront with 64 tokens reads half as much from LDS and took as long.  Where there are few tokens and heads, the rows
+// are dealt to several workgroups, whose sums another launch adds in order.
 constexpr uint32_t kWeightWaves = 4;
 template <int HD>
 __global__ __launch_bounds__(64 * kWeightWaves, 2) void kv_block_weights_tiles_kernel(AttentionArgs a) {
@@ -1130,7 +1141,8 @@ mi355q_status launch_tiles(mi355q_context* ctx, hipStream_t s, AttentionArgs a, 
     if (record) describe_step(record, "kv_block_attention", "kv_block_attention_tiles", grid.x, grid.y, grid.z, 256 * TS, (uint32_t)lds);
     if (!run) return MI355Q_OK;
     MI355Q_HIP(hipSetDevice(ctx->device));
-    // shares of the rows for the weight sums: about three workgroups a CU, each with eight tiles of 32 rows at least
+    // shares of the rows for the weight sums: about three workgroups a CU, each with eight tiles of 32 rows at least (attention
+    // with sums, one share / shares: 1024 rows of 32 heads of 128 on 8 128 / 54 us, 1534 rows of 16 heads of 256 on 2 424 / 125)
     const uint32_t tokens = kWeightWaves * 32, chunks = (a.kv.max_length + tokens - 1) / tokens;
     const uint64_t owners = (uint64_t)chunks * a.kv.kv_heads * a.kv.sequences;
     a.sum_stride = chunks * tokens;
@@ -1240,6 +1252,9 @@ mi355q_status dispatch_kv_block_attention(mi355q_context* ctx, hipStream_t s, co
     return kv_with_head_dimension(cache->head_dimension, [&](auto hd) -> mi355q_status {
         constexpr int HD = decltype(hd)::value;
         const uint32_t rows = a.kv.max_rows * a.group;
+        // 16 rows fill a product of the rows kernel, 32 two of them.  17 to 32 rows on the rows and the tiles kernel: 32 sequences
+        // of 8192 tokens, 32 rows a head, 100 and 154 us; 8 of up to 2000, 24 rows, 21 and 25; one of 30000 29 and 39.  With heads
+        // of 256 two products' accumulators and rows do not fit the registers.
         if (rows <= 16) return launch_rows<HD, 1>(ctx, s, a, weights, run, record);
         if (HD < 256 && rows <= 32) return launch_rows<HD < 256 ? HD : 64, 2>(ctx, s, a, weights, run, record);
         return launch_tiles<HD>(ctx, s, a, weights, run, record);

@@ -2,7 +2,9 @@
 //
 // With z = x - m and m the largest logit seen, a lane carries l = sum e^z and t = sum e^z z, which move to a larger
 // maximum m' by e^(m - m') and t' = e^(m - m') (t + (m - m') l).  Then log softmax(x)_i = x_i - m - log l and the entropy
-// is log l - t / l.  HBM-bound: a logit is read once; about ten vector instructions each, one of them an exponential.
+// is log l - t / l.  A logit is read once and takes about ten vector instructions, one of them an exponential: with 16-bit
+// logits that is two thirds of the time of their bytes, and the two overlap in part (777 rows of 100003 bf16 logits, 20
+// alternatives: 42 us and 5 for joining, 155 MB; fp32 logits of 2 x the bytes 69; one row of 65536: 6 + 5).
 //
 // Alternatives: logits are ordered by 64-bit keys (ordered value, ~index), all distinct, so equal logits need no rule of
 // their own.  The pass itself only notes, for every lane, the largest logit of each of its steps of sixteen (one LDS
@@ -351,8 +353,9 @@ __global__ __launch_bounds__(64) void token_logprobs_join_kernel(LogprobArgs a) 
 
 namespace {
 
-// Slices of a row: whole steps, few enough that a slice is worth its own partial result, and enough workgroups that
-// every CU has several.
+// Slices of a row: whole steps, few enough that a slice is worth its own partial result, and enough workgroups that every CU
+// has several.  (768, 1024 or 2048 workgroups: within 3 % of each other, but 2048 lose 3 of 19 us on 64 rows of 128000 with 20
+// alternatives.  Slices of up to 16 steps; with 8 the 777 rows above take 53 us instead of 47: twice the ends.)
 void logprob_slices(LogprobArgs* a) {
     const uint32_t span = a->vocabulary + 8, steps = (span + kLogprobStep - 1) / kLogprobStep;
     uint64_t slices = (1024 + a->rows - 1) / a->rows;
