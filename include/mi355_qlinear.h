@@ -748,7 +748,9 @@ typedef struct mi355q_kv_block_cache {
  * row_starts_dev: int32 [sequence_count + 1]: rows [row_starts[b], row_starts[b + 1]) of the call's row tensors are the
  *   LAST tokens of sequence b, so row i of n stands at position length - n + i.
  * row_count, maximum_rows, maximum_length: bounds of row_starts[sequence_count], of the rows of a sequence and of its
- *   length, known on the host: launches are sized by them.
+ *   length, known on the host: launches are sized by them, and so is the scratch of the context (attention that
+ *   accumulates weights for up to 32 rows of a KV head: 4 bytes per row, head and token up to maximum_length; eviction
+ *   beyond 32768 tokens: 4 bytes per head and token), so they are best kept near the truth.
  * The tables are read on the device only and are not errors there: lengths are cut to [0, maximum_length] and to the
  * table's width, rows to [0, row_count] and to maximum_rows, and a token whose block id lies outside [0, block_count) is
  * absent: nothing is written for it, it reads as zeros, and attention does not see it. */
@@ -805,7 +807,7 @@ MI355Q_API mi355q_status mi355q_kv_block_evict(mi355q_context* ctx, void* stream
  * in order with their log probabilities ([row_count, top_count]; equal logits: the lowest index first).  A NaN logit
  * counts as -inf (a masked token), +inf as the largest finite number.  Masked tokens are no alternatives: places that
  * nothing fills hold -1 and -inf.  A row that is masked throughout has entropy 0 and log probability -inf; so has a token
- * id outside the vocabulary.  token_ids_dev and logprob_dev go together and may be NULL both, entropy_dev may be NULL.
+ * id outside the vocabulary.  Fewer than 2^24 rows.  token_ids_dev and logprob_dev go together and may be NULL both, entropy_dev may be NULL.
  * Partial results live in the context's scratch. */
 MI355Q_API mi355q_status mi355q_token_logprobs(mi355q_context* ctx, void* stream, const void* logits_dev,
                                                mi355q_dtype dtype, uint32_t row_count, uint32_t vocabulary_size,

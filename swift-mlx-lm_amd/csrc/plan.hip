@@ -3,6 +3,7 @@
 // (Sources/MetalCompiler/Execution/MetalDecodePlan.swift:6-140, MetalDecodeEncoder.swift:18-36).
 #include <functional>
 #include <new>
+#include <utility>
 #include <string>
 #include <vector>
 
@@ -75,19 +76,23 @@ mi355q_status encode_range(mi355q_plan* plan, hipStream_t s, uint32_t first, uin
 }
 
 // A step that is no projection: checked now, run at every replay.
-mi355q_status add_call(mi355q_plan* plan, int32_t layer_index, const char* tensor_name, uint32_t rows,
-                       std::function<mi355q_status(hipStream_t, bool, mi355q_step*)> call) {
+template <typename F>
+mi355q_status add_call(mi355q_plan* plan, int32_t layer_index, const char* tensor_name, uint32_t rows, F&& call) {
     if (plan->graph_exec) return fail(MI355Q_ERR_INVALID_ARGUMENT, "plan is frozen: its graph has been built");
-    PlanStep st{};
-    st.kind = kCall;
-    if (mi355q_status rc = call(nullptr, false, &st.record)) return rc;
-    st.m = rows;
-    st.record.path = rows <= 8 ? MI355Q_PATH_DECODE_PROJECTION : MI355Q_PATH_PREFILL_PROJECTION;
-    st.record.sequence_length = rows;
-    st.layer_index = layer_index;
-    if (tensor_name) st.tensor_name = tensor_name;
-    st.call = std::move(call);
-    plan->steps.push_back(std::move(st));
+    try {
+        PlanStep st{};
+        st.kind = kCall;
+        if (mi355q_status rc = call(nullptr, false, &st.record)) return rc;
+        st.m = rows;
+        st.record.path = rows <= 8 ? MI355Q_PATH_DECODE_PROJECTION : MI355Q_PATH_PREFILL_PROJECTION;
+        st.record.sequence_length = rows;
+        st.layer_index = layer_index;
+        if (tensor_name) st.tensor_name = tensor_name;
+        st.call = std::forward<F>(call);
+        plan->steps.push_back(std::move(st));
+    } catch (const std::bad_alloc&) {
+        return fail(MI355Q_ERR_OUT_OF_MEMORY, "host allocation failed");
+    }
     return MI355Q_OK;
 }
 
