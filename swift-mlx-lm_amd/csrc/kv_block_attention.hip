@@ -35,8 +35,8 @@ struct AttentionArgs {
     uint32_t tiles, parts, part_blocks;
     float* part_out;          // [slot row][HD], in units of 2^m
     float2* part_ml;          // [slot row] (m, l)
-    // weights wanted: scores in units of log2, [sequence * kv_heads + head][score_blocks][score_rows][64], and each row's
-    // log2 of the sum
+    // weights wanted: scores in units of log2, [sequence * kv_heads + head][score_blocks][sixteen tokens]
+    // [score_rows][16], and each row's log2 of the sum
     float* scores;
     float* lse2;
     uint32_t score_rows, score_blocks;
@@ -200,7 +200,8 @@ __device__ __forceinline__ void store_row4(const AttentionArgs& a, size_t at, co
 // on 8: 88 us, 6.1 TB/s, where a kernel that only reads reaches 7.1; of 2394 to 8192 tokens 61 us, 5.4 TB/s; 16 of up to 16000
 // tokens, 16 heads of 256 on 4, 64 us.  One sequence of 517 tokens: 6.5 us and 3 for joining, latency.)  Storing the scores for
 // the weight sums costs the second of these 14 us for 21 MB.
-template <int HD, int RT>
+// SCORES: they are stored for the weight sums (apart, since their addresses cost registers that 32 rows do not have to spare).
+template <int HD, int RT, bool SCORES>
 __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void kv_block_attention_rows_kernel(AttentionArgs a) {
     constexpr int S = HD / 64, DT = HD / 16;
     __shared__ __align__(16) float lds_out[2][16 * RT * HD];
@@ -324,10 +325,10 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void kv_block_attention_row
             for (int k = 0; k < 4; k++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) top = fmaxf(top, x[t][k][i]);
-            if (a.scores && t * 16 + n < rows) {
-                float* const at = a.scores + ((((size_t)b * a.kv.kv_heads + head) * a.score_blocks + j) * a.score_rows + t * 16 + n) * kKvTokens + c * 4;
+            if (SCORES && t * 16 + n < rows) {
+                float* const at = a.scores + (((size_t)b * a.kv.kv_heads + head) * a.score_blocks + j) * a.score_rows * kKvTokens + (t * 16 + n) * 16 + c * 4;
 #pragma unroll
-                for (int k = 0; k < 4; k++) *(floatx4*)(at + k * 16) = x[t][k];
+                for (int k = 0; k < 4; k++) *(floatx4*)(at + k * 16 * a.score_rows) = x[t][k];      // (rows side by side: whole lines)
             }
             top += vlog - kHeadroom;
             if (__ballot(top > m[t] + kRaise)) {
@@ -421,7 +422,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void kv_block_attention_row
         if (c == 0) {
             const float lse2 = l[t] == 0.0f ? -INFINITY : m[t] + log2f(l[t]);
             if (a.lse) a.lse[row * a.heads + h] = lse2 * 0.6931471805599453f;
-            if (a.scores) a.lse2[((size_t)b * a.kv.kv_heads + head) * a.score_rows + r] = lse2;
+            if (SCORES) a.lse2[((size_t)b * a.kv.kv_heads + head) * a.score_rows + r] = lse2;
         }
     }
 }
@@ -1049,11 +1050,11 @@ __device__ __forceinline__ void weigh_tokens(const AttentionArgs& a, uint32_t ti
     __syncthreads();
     if (j < g.first || j >= g.last) return;
     const int32_t block = kv_block_id(a.kv, s.table, j);
-    const floatx4* const scores = (const floatx4*)(a.scores + (slot * a.score_blocks + j) * a.score_rows * kKvTokens + t % (int32_t)kKvTokens);
+    const floatx4* const scores = (const floatx4*)(a.scores + ((slot * a.score_blocks + j) * 4 + t % (int32_t)kKvTokens / 16) * a.score_rows * 16 + t % 16);
     floatx4 sum = {0, 0, 0, 0};
 #pragma unroll 4
     for (uint32_t r = 0; r < rows; r++) {
-        const floatx4 x = scores[r * (kKvTokens / 4)];
+        const floatx4 x = scores[r * 4];
         const float lse2 = lds_lse[r];
 #pragma unroll
         for (int i = 0; i < 4; i++) sum[i] += __builtin_amdgcn_exp2f(x[i] - lse2);
@@ -1209,7 +1210,9 @@ mi355q_status launch_rows(mi355q_context* ctx, hipStream_t s, AttentionArgs a, b
         if (!pass && buf.used)
             if (mi355q_status st = ensure_workspace(ctx, buf.used)) return st;
     }
-    kv_block_attention_rows_kernel<HD, RT><<<dim3(a.kv.kv_heads * a.parts, 1, a.kv.sequences), 256, 0, s>>>(a);
+    const dim3 grid(a.kv.kv_heads * a.parts, 1, a.kv.sequences);
+    if (weights) kv_block_attention_rows_kernel<HD, RT, true><<<grid, 256, 0, s>>>(a);
+    else kv_block_attention_rows_kernel<HD, RT, false><<<grid, 256, 0, s>>>(a);
     MI355Q_HIP(hipGetLastError());
     if (weights) {
         const uint32_t join_rows = a.parts > 1 ? rows : 0, chunks = (a.kv.max_length + 1023) / 1024;
