@@ -810,8 +810,9 @@ __global__ __launch_bounds__(256 * TS, 2) void kv_block_attention_tiles_kernel(A
 constexpr uint32_t kWeightWaves = 4;
 template <int HD>
 __global__ __launch_bounds__(64 * kWeightWaves, 2) void kv_block_weights_tiles_kernel(AttentionArgs a) {
-    constexpr int S = HD / 64, PER = HD / 16 / kWeightWaves;      // operands of 64 lanes that a wavefront moves
-    __shared__ u32x4 lds_q[2][(HD / 16) * 64];
+    constexpr int S = HD / 64, TILES = HD == 256 ? 1 : 2, PER = TILES * HD / 16 / kWeightWaves;      // operands of 64 lanes that a wavefront moves
+    constexpr uint32_t STEP = 32 * TILES;
+    __shared__ u32x4 lds_q[2][TILES * (HD / 16) * 64];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
     const uint32_t n = lane & 31, h = lane >> 5;
     const uint32_t head = blockIdx.x % a.kv.kv_heads, chunk = blockIdx.x / a.kv.kv_heads, b = blockIdx.z;
@@ -826,7 +827,7 @@ __global__ __launch_bounds__(64 * kWeightWaves, 2) void kv_block_weights_tiles_k
     uint32_t r_last = (uint32_t)max((int64_t)0, min((int64_t)s.rows, behind)) * a.group;
     const uint32_t share = blockIdx.y;
     if (a.sum_parts > 1 && r_first < r_last) {
-        const uint32_t each = ((r_last - r_first + 31) / 32 + a.sum_parts - 1) / a.sum_parts * 32;
+        const uint32_t each = ((r_last - r_first + STEP - 1) / STEP + a.sum_parts - 1) / a.sum_parts * STEP;
         r_first += min(share * each, r_last - r_first);
         r_last = min(r_first + each, r_last);
     }
@@ -848,33 +849,52 @@ __global__ __launch_bounds__(64 * kWeightWaves, 2) void kv_block_weights_tiles_k
 #pragma unroll
     for (int i = 0; i < 16; i++) sum[i] = 0.0f;
     const size_t slot = (size_t)b * a.kv.kv_heads + head;
+    // of the 32 rows from row `first` on, some see the wavefront's tokens if first + 31 >= seen_from and first < seen_to, and
+    // all see all of them if first >= whole_from and first + 31 < whole_to
+    auto row_at = [&](int64_t position) { return (int32_t)max((int64_t)-(1 << 30), min((position - s.first()) * (int64_t)a.group, (int64_t)1 << 30)); };
+    const int32_t seen_from = row_at(base), whole_from = row_at(base + 31);
+    const int32_t seen_to = a.window ? row_at((int64_t)base + 31 + a.window) : 1 << 30, whole_to = a.window ? row_at((int64_t)base + a.window) : 1 << 30;
     u32x4 next[PER];
-    float next_factor = 0.0f, next_lse = INFINITY;
-    auto fetch = [&](uint32_t first) {
-        const size_t at = slot * a.operand_tiles + first / 32;
+    float next_factor[TILES], next_lse[TILES];
+    auto fetch = [&](uint32_t first) {                     // (a tile behind the last one is the last one, and is not used)
+        const size_t base = slot * a.operand_tiles;
+        const uint32_t last = a.operand_tiles - 1;
 #pragma unroll
-        for (int i = 0; i < PER; i++) next[i] = a.operands[(at * (HD / 16) + wave * PER + i) * 64 + lane];
-        next_factor = a.factors[at * 32 + n];
-        next_lse = first + n < rows ? a.lse2[slot * a.score_rows + first + n] : INFINITY;
+        for (int i = 0; i < PER; i++) {
+            const uint32_t f = wave * PER + i, tile = min(first / 32 + f / (HD / 16), last);
+            next[i] = a.operands[((base + tile) * (HD / 16) + f % (HD / 16)) * 64 + lane];
+        }
+#pragma unroll
+        for (int u = 0; u < TILES; u++) {
+            next_factor[u] = a.factors[(base + min(first / 32 + u, last)) * 32 + n];
+            next_lse[u] = first + u * 32 + n < rows ? a.lse2[slot * a.score_rows + first + u * 32 + n] : INFINITY;
+        }
     };
     if (r_first < r_last) fetch(r_first);
     int buffer = 0;
-    for (uint32_t first = r_first; first < r_last; first += 32, buffer ^= 1) {
+    for (uint32_t step = r_first; step < r_last; step += STEP, buffer ^= 1) {
 #pragma unroll
         for (int i = 0; i < PER; i++) lds_q[buffer][(wave * PER + i) * 64 + lane] = next[i];
-        const float f = fmaxf(next_factor * ks, 1e-37f), lse2 = next_lse == -INFINITY ? INFINITY : next_lse;
+        float factor[TILES], lse[TILES];
+#pragma unroll
+        for (int u = 0; u < TILES; u++) {
+            factor[u] = fmaxf(next_factor[u] * ks, 1e-37f);
+            lse[u] = next_lse[u] == -INFINITY ? INFINITY : next_lse[u];
+        }
         __syncthreads();                                   // (the other buffer's readers are all past the barrier before)
-        if (first + 32 < r_last) fetch(first + 32);
-        const int32_t position = s.first() + (int32_t)((first + n) / a.group), low = row_low(a, position);
-        const int32_t p_low = s.first() + (int32_t)(first / a.group), p_high = s.first() + (int32_t)((first + 31) / a.group);
-        if (id >= 0 && p_high >= base && base + 31 >= row_low(a, p_low)) {
+        if (step + STEP < r_last) fetch(step + STEP);
+#pragma unroll
+        for (int u = 0; u < TILES; u++) {
+            const uint32_t first = step + u * 32;
+            if (id < 0 || first >= r_last || (int32_t)first + 31 < seen_from || (int32_t)first >= seen_to) continue;
             floatx16 x;
 #pragma unroll
             for (int i = 0; i < 16; i++) x[i] = 0.0f;
 #pragma unroll
             for (int i = 0; i < HD / 16; i++)
-                x = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i], __builtin_bit_cast(half8, lds_q[buffer][i * 64 + lane]), x, 0, 0, 0);
-            if (!(base + 31 <= p_low && base >= row_low(a, p_high))) {
+                x = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i], __builtin_bit_cast(half8, lds_q[buffer][(u * (HD / 16) + i) * 64 + lane]), x, 0, 0, 0);
+            if ((int32_t)first < whole_from || (int32_t)first + 31 >= whole_to) {
+                const int32_t position = s.first() + (int32_t)((first + n) / a.group), low = row_low(a, position);
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const int32_t at = base + (i >> 2) * 8 + (int32_t)h * 4 + (i & 3);
@@ -882,7 +902,7 @@ __global__ __launch_bounds__(64 * kWeightWaves, 2) void kv_block_weights_tiles_k
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 16; i++) sum[i] += __builtin_amdgcn_exp2f(fmaf(x[i], f, -lse2));
+            for (int i = 0; i < 16; i++) sum[i] += __builtin_amdgcn_exp2f(fmaf(x[i], factor[u], -lse[u]));
         }
     }
     float* const at = a.sum_parts > 1 ? a.sums + (share * (size_t)a.kv.sequences * a.kv.kv_heads + slot) * a.sum_stride + base
