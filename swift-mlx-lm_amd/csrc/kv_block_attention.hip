@@ -199,7 +199,8 @@ __device__ __forceinline__ void store_row4(const AttentionArgs& a, size_t at, co
 // the matrix cores take them, a block ahead, and every row of the group uses them.  (32 sequences of 8192 tokens, 32 heads of 128
 // on 8: 88 us, 6.1 TB/s, where a kernel that only reads reaches 7.1; of 2394 to 8192 tokens 61 us, 5.4 TB/s; 16 of up to 16000
 // tokens, 16 heads of 256 on 4, 64 us.  One sequence of 517 tokens: 6.5 us and 3 for joining, latency.)  Storing the scores for
-// the weight sums costs the second of these 14 us for 21 MB.
+// the weight sums costs the second of these 9 us for 21 MB; rows side by side in sixteens of tokens make whole lines of them
+// (rows behind blocks of 64 tokens: 16).
 // SCORES: they are stored for the weight sums (apart, since their addresses cost registers that 32 rows do not have to spare).
 template <int HD, int RT, bool SCORES>
 __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void kv_block_attention_rows_kernel(AttentionArgs a) {
@@ -802,9 +803,10 @@ __global__ __launch_bounds__(256 * TS, 2) void kv_block_attention_tiles_kernel(A
 
 // Weight sums of many rows: the scores are computed again, tokens against all rows that see them.  A wavefront holds the
 // keys of 32 tokens as operands and adds up 2^(x - lse2) over the rows, whose operands the tiles kernel left in memory and
-// which pass through LDS 32 at a time, 32 more on their way meanwhile; the sums of its lanes, which hold different rows,
-// are added at the end, so every sum is made in one fixed order.  Bound by the matrix cores with heads of 256 and by the
-// exponentials, a vector instruction of four times the length for each score, with heads of 64 (the three chunks of 256: 50 us).
+// which pass through LDS 64 at a time (32 with heads of 256), as many more on their way; the sums of its lanes, which hold
+// different rows, are added at the end, so every sum is made in one fixed order.  Bound by the matrix cores with heads of 256 and by the
+// exponentials, a vector instruction of four times the length for each score, with heads of 64 (the three chunks of 256: 48 us;
+// 4 chunks of 512 rows on 5000 tokens, 32 heads of 128: 113).
 // A wavefront with 64 tokens reads half as much from LDS and took as long.  Where there are few tokens and heads, the rows
 // are dealt to several workgroups, whose sums another launch adds in order.
 constexpr uint32_t kWeightWaves = 4;
