@@ -396,7 +396,7 @@ __device__ __forceinline__ void write_kept(const SelectTask& s, uint32_t first, 
         uint2 all;
         const uint2 before = scan_counts(make_uint2((uint32_t)__popcll(keep), (uint32_t)__popcll(tie)), totals, s.lane, s.wave, &all);
         const uint32_t ties_before = ties + before.y;
-        uint32_t place = written + before.x + min(ties_before, need) - min(ties, need);
+        const uint32_t place = written + before.x + min(ties_before, need) - min(ties, need);
         // the block's ties that are kept are its first: drop the last set bits until they fit
         uint32_t fit = ties_before < need ? need - ties_before : 0;
         if ((uint32_t)__popcll(tie) > fit) {
@@ -407,7 +407,13 @@ __device__ __forceinline__ void write_kept(const SelectTask& s, uint32_t first, 
             }
             tie = chosen;
         }
-        for (keep |= tie; keep; keep &= keep - 1) s.out[place++] = (int32_t)((from + threadIdx.x) * kKvTokens + (uint32_t)__builtin_ctzll(keep));
+        // the masks become those of the tokens kept and the places of their first; then a wavefront writes a block's at once
+        if (mine) { masks->keep[threadIdx.x] = keep | tie; masks->tie[threadIdx.x] = place; }
+        __syncthreads();
+        for (uint32_t j = s.wave; j < to - from; j += kSelectWaves) {
+            const uint64_t kept = masks->keep[j];
+            if (kept >> s.lane & 1) s.out[(uint32_t)masks->tie[j] + (uint32_t)__popcll(kept & ((1ull << s.lane) - 1))] = (int32_t)((from + j) * kKvTokens + s.lane);
+        }
         written += all.x + min(ties + all.y, need) - min(ties, need);
         ties += all.y;
     }
