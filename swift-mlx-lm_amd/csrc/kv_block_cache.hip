@@ -423,7 +423,7 @@ __device__ __forceinline__ void write_kept(const SelectTask& s, uint32_t first, 
 // Latency-bound (a workgroup has one sequence's few tens of kilobytes): the sums are read once, eight blocks of a wavefront
 // in flight, and their keys held in LDS; the key of the last token kept is found in three digits of 11, 11 and 10 bits from
 // histograms; then every block's kept tokens and ties become bit masks, whose counts give each block its place in the list
-// (8 sequences of 8192 tokens, 8 heads: 17 us).
+// (8 sequences of 8192 tokens, 8 heads: 15.5 us).
 // Ties with the last key are kept from the lowest position on.
 __global__ __launch_bounds__(kSelectThreads) void kv_block_select_kernel(KvBlockArgs a, EvictArgs e) {
     extern __shared__ uint32_t lds_keys[];
@@ -490,7 +490,7 @@ __global__ __launch_bounds__(kSelectThreads) void kv_block_select_kernel(KvBlock
 // `list`: with the histograms of all chunks every workgroup finds the first digit, counts its chunk's tokens that are kept
 // for sure and lists the keys that begin with it.  `write`: from the lists of all chunks every workgroup finds the other
 // digits and its chunk's place, and writes its positions.  What a workgroup does alike with the others of its sequence
-// and head are a few thousand numbers.  Latency-bound like the kernel above: 60001 tokens of 4 heads take 5 + 10 + 14 us, one
+// and head are a few thousand numbers.  Latency-bound like the kernel above: 60001 tokens of 4 heads take 5 + 10 + 12 us, one
 // workgroup a head took 64 (60 tokens a thread: bound by instructions).
 struct SelectChunks {
     uint32_t chunks, blocks;      // chunks of a sequence, blocks of a chunk
@@ -640,17 +640,19 @@ __global__ __launch_bounds__(kSelectThreads) void kv_block_select_write_kernel(K
     write_kept(s, first, last, true, prefix, need, written + min(ties, need), ties, &masks, totals, read);
 }
 
-// One workgroup per new block, head and sequence: keys and values of its 64 kept tokens, gathered piece by piece (keys)
-// and code by code (values, whose pieces hold sixteen tokens), brought to the largest of their scales.  Bound by the
-// requests of the values: a lane's load brings one code, and a line of 128 bytes holds eight dimensions of sixteen tokens, so
-// lines are asked for many times over (8 sequences of 8192 tokens, 8 heads of 128, to 2048: 83 of the old blocks' 134 MB read
-// and 34 written in 38 us).  Passing the old blocks' values through LDS in whole, and picking the codes there, took 47 us: a
-// workgroup then waits for its blocks behind two barriers more.
+// One workgroup per new block, head and sequence: keys and values of its 64 kept tokens, brought to the largest of their
+// scales.  Keys are gathered by pieces of 16 dimensions of a token.  A value piece holds sixteen tokens of one dimension, and
+// the kept tokens come in order: a thread has one dimension and reads all 64 codes of each old block once, a block ahead, and
+// picks the kept ones.  HBM-bound where many are kept, latency-bound where they are few (8 sequences of 8192 tokens, 8 heads of
+// 128, to 2048: 83 MB read and 34 written in 28.6 us; to 6000 of spread tokens 85 -> 64 with the selection, against a load for
+// each code, which asked for every line many times over: 38 us for the first).  Passing the old blocks' values through LDS in
+// whole, and picking the codes there, took 47 us.
 template <int HD>
 __global__ __launch_bounds__(2 * HD) void kv_block_gather_kernel(KvBlockArgs a, EvictArgs e) {
     __shared__ int32_t block_of[kKvTokens];               // source block of each kept token, -1: none
     __shared__ uint32_t token_of[kKvTokens];
     __shared__ float ratio[2][kKvTokens];
+    __shared__ __align__(16) uint8_t picked[kKvTokens * HD];
     const uint32_t j = blockIdx.x, head = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
     const uint32_t length = (uint32_t)kv_length(a, b), kept = min(length, e.budget);
     const int32_t target = e.new_table[(size_t)b * e.new_stride + j];
@@ -699,24 +701,47 @@ __global__ __launch_bounds__(2 * HD) void kv_block_gather_kernel(KvBlockArgs a, 
         }
         *(uint4*)(keys + piece * 16) = w;
     }
+    // values: a thread per dimension and half of the kept tokens, which come in order, so that their old blocks come in runs: of
+    // each it reads the dimension's 64 codes, a run ahead, and picks the kept ones
+    const uint32_t d = tid % HD, lane = tid & 63;
+    const uint32_t half = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid / HD));
+    const int32_t own_block = block_of[lane], own_token = (int32_t)token_of[lane];
+    const int32_t own_ratio = __float_as_int(ratio[1][lane]);
+    const uint64_t starts = __ballot(lane % 32 == 0 || own_block != __shfl_up(own_block, 1));
+    auto load = [&](uint32_t o, u32x4 (&w)[4]) {
+        const int32_t block = __builtin_amdgcn_readlane(own_block, (int)o);
+        const int8_t* const from = kv_codes<HD>(a, block < 0 ? 0 : block, head, 1) + (d >> 4) * 1024 + (d & 15) * 16;
+#pragma unroll
+        for (int c = 0; c < 4; c++) w[c] = block < 0 ? u32x4{} : *(const u32x4*)(from + c * 256);
+    };
+    uint32_t o = half * 32, word = 0;
+    const uint32_t end = o + 32;
+    u32x4 next[4];
+    load(o, next);
+    while (o < end) {
+        const uint64_t behind = o == 63 ? 0 : starts >> (o + 1);
+        const uint32_t stop = behind ? min(o + 1 + (uint32_t)__builtin_ctzll(behind), end) : end;
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) w[i] = next[i >> 2][i & 3];
+        if (stop < end) load(stop, next);
+        for (; o < stop; o++) {
+            const uint32_t u = (uint32_t)__builtin_amdgcn_readlane(own_token, (int)o);
+            const float f = __int_as_float(__builtin_amdgcn_readlane(own_ratio, (int)o));
+            const uint32_t codes = w[(u >> 2 & 3) * 4 + (u >> 4)];
+            word |= ((uint32_t)(int)rintf((float)(int8_t)(codes >> (8 * (u & 3))) * f) & 0xFFu) << (8 * (o & 3));
+            if ((o & 3) == 3) {
+                *(uint32_t*)(picked + kv_value_byte<HD>(o & ~3u, d)) = word;
+                word = 0;
+            }
+        }
+    }
+    __syncthreads();
     int8_t* const values = kv_codes<HD>(a, target, head, 1);
 #pragma unroll
     for (int r = 0; r < 2; r++) {
-        const uint32_t piece = r * 2 * HD + tid;           // dimension piece / 64 * 16 + piece % 16, lane group piece / 16 % 4
-        const uint32_t d = piece / 64 * 16 + piece % 16, c = piece / 16 % 4;
-        uint32_t w[4];
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-            w[q] = 0;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint32_t t = (uint32_t)q * 16 + c * 4 + i;
-                if (block_of[t] < 0) continue;
-                const float code = (float)kv_codes<HD>(a, block_of[t], head, 1)[kv_value_byte<HD>(token_of[t], d)];
-                w[q] |= ((uint32_t)(int)rintf(code * ratio[1][t]) & 0xFFu) << (8 * i);
-            }
-        }
-        *(uint4*)(values + piece * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+        const uint32_t byte = (r * 2 * HD + tid) * 16;
+        *(uint4*)(values + byte) = *(const uint4*)(picked + byte);
     }
 }
 
