@@ -707,7 +707,8 @@ __global__ __launch_bounds__(2 * HD) void kv_block_gather_kernel(KvBlockArgs a, 
     const uint32_t half = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid / HD));
     const int32_t own_block = block_of[lane], own_token = (int32_t)token_of[lane];
     const int32_t own_ratio = __float_as_int(ratio[1][lane]);
-    const uint64_t starts = __ballot(lane % 32 == 0 || own_block != __shfl_up(own_block, 1));
+    const int32_t in_front = __shfl_up(own_block, 1);      // (by all lanes: one that is switched off gives 0)
+    const uint64_t starts = __ballot(lane % 32 == 0 || own_block != in_front);
     auto load = [&](uint32_t o, u32x4 (&w)[4]) {
         const int32_t block = __builtin_amdgcn_readlane(own_block, (int)o);
         const int8_t* const from = kv_codes<HD>(a, block < 0 ? 0 : block, head, 1) + (d >> 4) * 1024 + (d & 15) * 16;

@@ -455,3 +455,19 @@ def test_codes_near_the_middle_of_two(pkg, ctx, size):
     ctx.kv_block_append(cache.c, sequences(pkg, ctx, tables, [length], [length]), k, v, pkg.F32)
     cache.append(tables[0], 0, x)
     check_tokens(cache, tables, [length])
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("sinks", [1, 2, 31, 32, 33, 63])
+def test_evict_across_the_first_block_of_the_pool(pkg, ctx, hd, sinks):
+    """`sinks` tokens of a block and the others from block 0, which the second lane of a half meets first."""
+    rng = np.random.default_rng(sinks)
+    cache = Cache(pkg, ctx, 2, hd, 4, rng)
+    table, new_table, budget = [2, 0], [1], 64
+    seq = sequences(pkg, ctx, [table], [128], [1])
+    ctx.kv_block_evict(cache.c, seq, budget, ctx.upload(np.array([new_table], np.int32)), 1, ctx.alloc(4), budget - sinks, sinks)
+    codes, scales, sums = cache.download()
+    for target, want_codes, want_scales, want_sums in plain_evict(cache, table, 128, budget, budget - sinks, sinks, new_table):
+        if target is not None:
+            assert np.array_equal(codes[target], want_codes) and np.array_equal(scales[target], want_scales)
+            assert np.array_equal(sums[target], want_sums)
