@@ -437,8 +437,8 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void kv_block_attention_row
 // 870 TFLOP/s of the 1130 that a product of 8192 x 8192 f16 matrices reaches here; 5001 rows: 232 us, 1.84 GHz, matrix cores busy
 // 0.43 of the cycles and the vector unit 0.6.  Scores of block j + 1 computed ahead of the softmax of block j spilt registers
 // and took longer; wave priorities for either phase changed nothing).  With heads of 256 the accumulators and rows of 32 rows fill
-// half of the register file and the blocks the LDS of a CU: there two wavefronts share their rows, each taking half of a
-// block's tokens (TS = 2), and add up their results at the end (a prompt of 4096 rows of 16 heads: 251 us without, 171 with).
+// half of the register file and the blocks the LDS of a CU: there, and where tiles are few, two wavefronts share their rows, each
+// taking half of a block's tokens (TS = 2), and add up their results at the end (a prompt of 4096 rows of 16 heads: 251 us without, 171 with).
 template <int HD, int WAVES>
 struct TileLds {
     u32x4 key[2 * (HD / 16) * 64];      // fragment (32-token half, sixteen dimensions)
@@ -447,34 +447,47 @@ struct TileLds {
 
 template <int HD, int WAVES>
 struct TileLoader {
-    static constexpr int PIECES = 4 * HD / (64 * WAVES);      // 16-byte pieces of a thread, keys and values each
+    // 16-byte pieces of a block: 4 HD of keys, 4 HD of values behind them.  A thread has some of each, or, where the threads are as
+    // many as all of them, one: the first half of the wavefronts keys, the others values
+    static constexpr uint32_t ALL = 4 * HD, THREADS = 64 * WAVES;
+    static constexpr int PIECES = ALL < THREADS ? 1 : ALL / THREADS;
+    static constexpr bool ONE = ALL < THREADS;
+    static_assert(ONE ? 2 * ALL == THREADS : ALL % THREADS == 0);
     u32x4 key[PIECES], value[PIECES];
     __device__ __forceinline__ void load(const AttentionArgs& a, int32_t block, uint32_t head, uint32_t tid) {
-        const u32x4* const kp = (const u32x4*)kv_codes<HD>(a.kv, block, head, 0) + tid;
-        const u32x4* const vp = (const u32x4*)kv_codes<HD>(a.kv, block, head, 1) + tid;
+        const u32x4* const p = (const u32x4*)kv_codes<HD>(a.kv, block, head, 0) + tid;
 #pragma unroll
-        for (int i = 0; i < PIECES; i++) key[i] = kp[i * 64 * WAVES];
+        for (int i = 0; i < PIECES; i++) key[i] = p[i * THREADS];
+        if constexpr (!ONE) {
 #pragma unroll
-        for (int i = 0; i < PIECES; i++) value[i] = vp[i * 64 * WAVES];
+            for (int i = 0; i < PIECES; i++) value[i] = p[ALL + i * THREADS];
+        }
+    }
+    static __device__ __forceinline__ void store_key(TileLds<HD, WAVES>& lds, uint32_t p, u32x4 piece) {
+        constexpr uint32_t S = HD / 64;
+        const uint32_t t = p & 15, kq = (p >> 4) & 3, seg = (p >> 6) % S, tile = (p >> 6) / S;
+        const uint32_t fragment = (tile >> 1) * (HD / 16) + seg * 4 + (kq >> 1) * 2, slot = (kq & 1) * 32 + (tile & 1) * 16 + t;
+        const u32x4 w = biased(piece);
+        lds.key[fragment * 64 + slot] = __builtin_bit_cast(u32x4, codes_f16(w.x, w.y));
+        lds.key[(fragment + 1) * 64 + slot] = __builtin_bit_cast(u32x4, codes_f16(w.z, w.w));
+    }
+    static __device__ __forceinline__ void store_value(TileLds<HD, WAVES>& lds, uint32_t p, u32x4 piece) {
+        const uint32_t d = p & 15, kq = (p >> 4) & 3, tile = p >> 6;
+        const uint32_t fragment = (tile >> 1) * 4 + (kq >> 1), slot = (kq & 1) * 32 + (tile & 1) * 16 + d;
+        const u32x4 w = biased(piece);
+        lds.value[fragment * 64 + slot] = __builtin_bit_cast(u32x4, codes_f16(w.x, w.y));
+        lds.value[(fragment + 2) * 64 + slot] = __builtin_bit_cast(u32x4, codes_f16(w.z, w.w));
     }
     __device__ __forceinline__ void store(TileLds<HD, WAVES>& lds, uint32_t tid) const {
-        constexpr uint32_t S = HD / 64;
-#pragma unroll
-        for (int i = 0; i < PIECES; i++) {
-            const uint32_t p = i * 64 * WAVES + tid, t = p & 15, kq = (p >> 4) & 3, seg = (p >> 6) % S, tile = (p >> 6) / S;
-            const uint32_t fragment = (tile >> 1) * (HD / 16) + seg * 4 + (kq >> 1) * 2, slot = (kq & 1) * 32 + (tile & 1) * 16 + t;
-            const u32x4 w = biased(key[i]);
-            lds.key[fragment * 64 + slot] = __builtin_bit_cast(u32x4, codes_f16(w.x, w.y));
-            lds.key[(fragment + 1) * 64 + slot] = __builtin_bit_cast(u32x4, codes_f16(w.z, w.w));
+        if constexpr (ONE) {
+            if (__builtin_amdgcn_readfirstlane((int)(tid / ALL)) == 0) store_key(lds, tid, key[0]);
+            else store_value(lds, tid - ALL, key[0]);
+            return;
         }
 #pragma unroll
-        for (int i = 0; i < PIECES; i++) {
-            const uint32_t p = i * 64 * WAVES + tid, d = p & 15, kq = (p >> 4) & 3, tile = p >> 6;
-            const uint32_t fragment = (tile >> 1) * 4 + (kq >> 1), slot = (kq & 1) * 32 + (tile & 1) * 16 + d;
-            const u32x4 w = biased(value[i]);
-            lds.value[fragment * 64 + slot] = __builtin_bit_cast(u32x4, codes_f16(w.x, w.y));
-            lds.value[(fragment + 2) * 64 + slot] = __builtin_bit_cast(u32x4, codes_f16(w.z, w.w));
-        }
+        for (int i = 0; i < PIECES; i++) store_key(lds, i * THREADS + tid, key[i]);
+#pragma unroll
+        for (int i = 0; i < PIECES; i++) store_value(lds, i * THREADS + tid, value[i]);
     }
 };
 
@@ -1123,11 +1136,12 @@ void choose_parts(AttentionArgs* a, uint64_t blocks, uint64_t groups, uint32_t w
 // block takes a workgroup about 1.1, 1.8 or 3.2 us (heads of 64, 128, 256) on a full chip and 0.7 of that on an empty one;
 // splitting costs about 12 us and joining 20 more if all workgroups leave partial results.  Only the longest sequence is
 // known here; those of a batch are taken to be three quarters of it.
+double expected_tiles(const AttentionArgs& a) { return ((double)a.kv.row_count * a.group / kTileRows + a.kv.sequences) * a.kv.kv_heads; }
 uint32_t span_workgroups(const AttentionArgs& a, int hd, uint32_t slots) {
     const uint64_t count = (uint64_t)a.tiles * a.kv.sequences, most = (a.kv.max_length + kKvTokens - 1) / kKvTokens + 1;
     if (count > kMostTiles || count * (most + kTileUnits) >= (1u << 31)) return 0;
     const double us = hd == 64 ? 1.1 : hd == 128 ? 1.8 : 3.2;
-    const double tiles = ((double)a.kv.row_count * a.group / kTileRows + a.kv.sequences) * a.kv.kv_heads / slots;
+    const double tiles = expected_tiles(a) / slots;
     const double longest = (double)visible_blocks(a, kTileRows), rows = std::min(a.kv.max_rows, a.kv.max_length);
     const double mean = std::min(longest, (a.kv.max_length - rows / 2) / kKvTokens + 1);
     const double whole = us * std::max(longest * (0.7 + 0.3 * std::min(1.0, tiles)), tiles * mean);
@@ -1149,14 +1163,11 @@ mi355q_status launch_join(hipStream_t s, const AttentionArgs& a, uint32_t rows, 
     return MI355Q_OK;
 }
 
-template <int HD>
+template <int HD, int TS>
 mi355q_status launch_tiles(mi355q_context* ctx, hipStream_t s, AttentionArgs a, bool weights, bool run, mi355q_step* record) {
-    constexpr int TS = HD == 256 ? 2 : 1;
     constexpr uint32_t ROWS = kTileRows;
     const uint32_t rows = a.kv.max_rows * a.group;
-    a.tiles = (rows + ROWS - 1) / ROWS;
     a.score_rows = rows;
-    a.span_count = span_workgroups(a, HD, TS == 2 ? 256 : 512);
     a.span_least = std::max(kLeastSpan, (a.kv.max_length / kKvTokens + 1) / (kMostParts - 2) + 1);
     const uint32_t count = a.tiles * a.kv.sequences;
     const size_t lds = tile_room<HD, TS>() + (a.span_count ? (count + 1) * 4 : 0);
@@ -1282,7 +1293,15 @@ mi355q_status dispatch_kv_block_attention(mi355q_context* ctx, hipStream_t s, co
         // of 256 two products' accumulators and rows do not fit the registers.
         if (rows <= 16) return launch_rows<HD, 1>(ctx, s, a, weights, run, record);
         if (HD < 256 && rows <= 32) return launch_rows<HD < 256 ? HD : 64, 2>(ctx, s, a, weights, run, record);
-        return launch_tiles<HD>(ctx, s, a, weights, run, record);
+        a.tiles = (rows + kTileRows - 1) / kTileRows;
+        // Four wavefronts a tile, two workgroups a CU; eight, sharing the blocks' tokens, with heads of 256 and where the tiles
+        // leave the second workgroup's place empty.  (Prompts of 700, 1024, 1300 and 1700 rows, 32 heads of 128 on 8, which are 176 to
+        // 425 tiles: four 24.7, 34.1, 42.1 and 55.2 us, eight 23.2, 30.6, 37.4 and 51.2; 8192 rows 590 and 685; of 1300 and 8192 rows
+        // with heads of 64 28.9 and 375, 26 and 439; 8 prompts of 300 rows, 480 equal tiles, 21 and 29.)
+        a.span_count = span_workgroups(a, HD, HD == 256 ? 256 : 512);
+        if (HD < 256 && (a.span_count || expected_tiles(a) > 384))
+            return launch_tiles<HD, HD < 256 ? 1 : 2>(ctx, s, a, weights, run, record);
+        return launch_tiles<HD, 2>(ctx, s, a, weights, run, record);
     });
 }
 }  // namespace mi355q

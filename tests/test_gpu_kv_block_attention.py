@@ -292,3 +292,39 @@ def test_as_many_parts_as_there_can_be(pkg, ctx):
     top = 127 * cache.scales[..., 1].max()
     assert np.all(np.abs(out[:, 0] - want) <= 2.0 ** -11 * top + 2.0 ** -11 * np.abs(want) + 1e-6)
     assert np.all(np.abs(lse - (m + np.log(total))) <= 2e-4)
+
+
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_more_tiles_than_the_chip_holds(pkg, ctx, hd, window):
+    """Forty short prompts of ten heads: a workgroup a tile, with the wavefronts' other shape."""
+    rng = np.random.default_rng(hd + window)
+    lengths = rng.integers(30, 150, 40).tolist()
+    rows = [33 if i % 7 else 34 for i in range(40)]
+    tables, _, blocks = deal(rng, lengths)
+    cache = Cache(pkg, ctx, 10, hd, blocks, rng)
+    q = (rng.standard_normal((sum(rows), 10, hd)) * 0.5).astype(np.float32)
+    check(pkg, ctx, cache, tables, lengths, rows, q, pkg.BF16, pkg.F16, window)
+
+
+def test_long_prompt_with_all_tiles_whole(pkg, ctx):
+    """A prompt of 1500 rows of 40 heads on 40: 480 tiles of up to 24 blocks, one of them absent; a sample of rows and heads
+    against the definition."""
+    rng = np.random.default_rng(21)
+    hd, heads, length = 64, 40, 1500
+    tables, _, blocks = deal(rng, [length])
+    tables[0][5] = blocks + 3
+    cache = Cache(pkg, ctx, heads, hd, blocks, rng)
+    q = act_rounded((rng.standard_normal((length, heads, hd)) * 0.5).astype(np.float32), pkg.BF16, pkg)
+    out, lse = run(pkg, ctx, cache, sequences(pkg, ctx, tables, [length], [length]), q, pkg.BF16, pkg.BF16, hd ** -0.5, weights=False)
+    k, v = cache.numbers(tables[0], length).astype(np.float64)
+    there = np.array([0 <= tables[0][t // TOKENS] < blocks for t in range(length)])
+    top = 127 * cache.scales[..., 1].max()
+    for r in list(range(0, 140)) + list(rng.integers(140, length, 200)) + [length - 1]:
+        for h in rng.integers(0, heads, 3):
+            seen = there & (np.arange(length) <= r)
+            s = k[seen, h] @ q[r, h].astype(np.float64) * hd ** -0.5
+            e = np.exp(s - s.max())
+            want = e @ v[seen, h] / e.sum()
+            assert np.all(np.abs(out[r, h] - want) <= 2.0 ** -11 * top + 2.0 ** -8 * np.abs(want) + 1e-6)
+            assert abs(lse[r, h] - (s.max() + np.log(e.sum()))) <= 2e-4
