@@ -63,6 +63,8 @@ struct mi355q_context {
     // fused output head: one packed (ordered value, ~row) key per workgroup of the projection launch
     // (kArgmaxPartialCapacity entries), then kArgmaxStandaloneKeys entries for the stand-alone argmax
     unsigned long long* argmax_partials;
+    // arrivals of the workgroups that share a result (kArrivals counters, 0 between launches): the last one joins
+    uint32_t* arrivals;
     // fp32 partial results (split-K of the prefill GEMM, K parts of the tile kernel): grown on demand, never shrunk;
     // outgrown buffers are kept until the context goes, because captured graphs hold their addresses
     void* workspace;
@@ -89,6 +91,7 @@ struct mi355q_context {
     bool scratch_pending, scratch_touched, scratch_marked;
 };
 constexpr int kRetiredWorkspaces = 96;
+constexpr uint32_t kArrivals = 16384;
 
 struct mi355q_weight {
     mi355q_context* ctx;

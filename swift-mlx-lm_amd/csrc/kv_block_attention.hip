@@ -35,6 +35,7 @@ struct AttentionArgs {
     uint32_t tiles, parts, part_blocks;
     float* part_out;          // [slot row][HD], in units of 2^m
     float2* part_ml;          // [slot row] (m, l)
+    uint32_t* arrivals;       // of the parts of each sequence and head; null: a launch of its own joins them
     // weights wanted: scores in units of log2, [sequence * kv_heads + head][score_blocks][sixteen tokens]
     // [score_rows][16], and each row's log2 of the sum
     float* scores;
@@ -193,6 +194,75 @@ __device__ __forceinline__ void store_row4(const AttentionArgs& a, size_t at, co
     else store4<MI355Q_F16>(a.out, at, v, f);
 }
 
+// ---- joining parts -----------------------------------------------------------------------------------------------------
+// The common maximum and the sum of a row's parts, by a wavefront: (m, l) of the row at the same units, and each part's
+// factor 2^(m_part - m) for the lanes' parts.
+template <bool SHARED = false>
+__device__ __forceinline__ float2 join_sums(const float2* part_ml, const PartRows& part, uint32_t lane, float (&f)[kMostParts / 64]) {
+    float2 ml[kMostParts / 64];
+    float top = kLowest;
+#pragma unroll
+    for (uint32_t i = 0; i < kMostParts / 64; i++) {
+        ml[i] = make_float2(kLowest, 0.0f);
+        if (i * 64 + lane < part.parts) ml[i] = SHARED ? share_load2((const float*)(part_ml + part.at(i * 64 + lane))) : part_ml[part.at(i * 64 + lane)];
+        top = fmaxf(top, ml[i].x);
+    }
+    top = max_across(top, lane);
+    top = fmaxf(top, lane_xor<1>(top)); top = fmaxf(top, lane_xor<2>(top)); top = fmaxf(top, lane_xor<4>(top)); top = fmaxf(top, lane_xor<8>(top));
+    float l = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < kMostParts / 64; i++) {
+        f[i] = exp2f(ml[i].x - top);
+        l += ml[i].y * f[i];
+    }
+    return make_float2(top, wave_reduce_sum(l));
+}
+
+// Joins the parts of a row, by a wavefront, kFewParts parts at a time, added in order.  SHARED: they come from the launch that
+// runs.
+template <int HD, bool SHARED>
+__device__ __forceinline__ void join_parts(const AttentionArgs& a, const KvSequence& s, uint32_t b, uint32_t head, uint32_t r, const PartRows& part, uint32_t lane) {
+    constexpr int E = HD / 64;
+    float x[kFewParts][E], f[kMostParts / 64], o[E];
+    auto load = [&](uint32_t first) {
+#pragma unroll
+        for (uint32_t p = 0; p < kFewParts; p++)
+            if (first + p < part.parts) {
+                const size_t at = part.at(first + p) * HD + lane;
+#pragma unroll
+                for (int e = 0; e < E; e++) x[p][e] = SHARED ? share_load(a.part_out + at + e * 64) : a.part_out[at + e * 64];
+            }
+    };
+    load(0);
+    const float2 ml = join_sums<SHARED>(a.part_ml, part, lane, f);
+#pragma unroll
+    for (int e = 0; e < E; e++) o[e] = 0.0f;
+    for (uint32_t first = 0; first < part.parts; first += kFewParts) {
+        if (first) load(first);
+#pragma unroll
+        for (uint32_t p = 0; p < kFewParts; p++)
+            if (first + p < part.parts) {
+                const float w = __shfl(first < 64 ? f[0] : f[1], (int)((first + p) & 63));
+#pragma unroll
+                for (int e = 0; e < E; e++) o[e] += x[p][e] * w;
+            }
+    }
+    const uint32_t token = r / a.group, h = head * a.group + r % a.group;
+    const size_t row = (size_t)(s.row0 + (int32_t)token);
+    const float scale = ml.y == 0.0f ? 0.0f : 1.0f / ml.y;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const size_t at = row * a.out_stride + (size_t)h * HD + e * 64 + lane;
+        if (a.out_dtype == MI355Q_BF16) ((uint16_t*)a.out)[at] = f32_to_bf16_rne(o[e] * scale);
+        else ((uint16_t*)a.out)[at] = f32_to_f16_rne(o[e] * scale);
+    }
+    if (lane == 0) {
+        const float lse2 = ml.y == 0.0f ? -INFINITY : ml.x + log2f(ml.y);
+        if (a.lse) a.lse[row * a.heads + h] = lse2 * 0.6931471805599453f;
+        if (a.lse2) a.lse2[((size_t)b * a.kv.kv_heads + head) * a.score_rows + r] = lse2;
+    }
+}
+
 // ---- few rows: decode steps and short verifications --------------------------------------------------------------------
 // A workgroup takes one KV head, 16 RT rows and one part of the visible blocks; its four wavefronts take blocks in turn,
 // each with accumulators of its own, which are added at the end.  HBM-bound: codes go from memory to registers in the order
@@ -207,6 +277,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void kv_block_attention_row
     constexpr int S = HD / 64, DT = HD / 16;
     __shared__ __align__(16) float lds_out[2][16 * RT * HD];
     __shared__ float2 lds_ml[4][16 * RT];
+    __shared__ bool last;
     const uint32_t lane = threadIdx.x & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t n = lane & 15, c = lane >> 4;
     const uint32_t head = blockIdx.x % a.kv.kv_heads, part = blockIdx.x / a.kv.kv_heads, b = blockIdx.z;
@@ -403,16 +474,26 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void kv_block_attention_row
         }
         __syncthreads();
     }
-    if (wave) return;
+    const bool joins = RT == 1 && parts > 1 && a.arrivals;
+    if (wave && !joins) return;
 #pragma unroll
     for (int t = 0; t < RT; t++) {
         const uint32_t r = t * 16 + n;
-        if (r >= rows) continue;
+        if (wave || r >= rows) continue;
         if (parts > 1) {
             const size_t slot = (((size_t)b * a.kv.kv_heads + head) * a.parts + part) * (16 * RT) + t * 16 + n;
 #pragma unroll
-            for (int d = 0; d < DT; d++) *(floatx4*)(a.part_out + slot * HD + d * 16 + c * 4) = o[t][d];
-            if (c == 0) a.part_ml[slot] = make_float2(m[t], l[t]);
+            for (int d = 0; d < DT; d++) {
+                float* const at = a.part_out + slot * HD + d * 16 + c * 4;
+                if (joins) {
+                    share_store(at, o[t][d].x, o[t][d].y);
+                    share_store(at + 2, o[t][d].z, o[t][d].w);
+                } else {
+                    *(floatx4*)at = o[t][d];
+                }
+            }
+            if (c == 0 && joins) share_store((float*)(a.part_ml + slot), m[t], l[t]);
+            else if (c == 0) a.part_ml[slot] = make_float2(m[t], l[t]);
             continue;
         }
         const uint32_t token = r / a.group, h = head * a.group + r % a.group;
@@ -426,6 +507,14 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void kv_block_attention_row
             if (SCORES) a.lse2[((size_t)b * a.kv.kv_heads + head) * a.score_rows + r] = lse2;
         }
     }
+    if (!joins) return;
+    if (!wave) {
+        const bool own = arrive_last(a.arrivals + (size_t)b * a.kv.kv_heads + head, parts);
+        if (lane == 0) last = own;
+    }
+    __syncthreads();
+    if (!last) return;
+    if (wave < rows) join_parts<HD, true>(a, s, b, head, wave, part_rows(a, s, b, head, wave, rows, 16 * RT), lane);      // (four rows at most)
 }
 
 // ---- many rows: prompts and prompt chunks ------------------------------------------------------------------------------
@@ -947,31 +1036,9 @@ __global__ __launch_bounds__(256) void kv_block_weights_add_kernel(AttentionArgs
     kv_sums(a.kv, id, head)[t % (int32_t)kKvTokens] += sum;
 }
 
-// The common maximum and the sum of a row's parts, by a wavefront: (m, l) of the row at the same units, and each part's
-// factor 2^(m_part - m) for the lanes' parts.
-__device__ __forceinline__ float2 join_sums(const float2* part_ml, const PartRows& part, uint32_t lane, float (&f)[kMostParts / 64]) {
-    float2 ml[kMostParts / 64];
-    float top = kLowest;
-#pragma unroll
-    for (uint32_t i = 0; i < kMostParts / 64; i++) {
-        ml[i] = i * 64 + lane < part.parts ? part_ml[part.at(i * 64 + lane)] : make_float2(kLowest, 0.0f);
-        top = fmaxf(top, ml[i].x);
-    }
-    top = max_across(top, lane);
-    top = fmaxf(top, lane_xor<1>(top)); top = fmaxf(top, lane_xor<2>(top)); top = fmaxf(top, lane_xor<4>(top)); top = fmaxf(top, lane_xor<8>(top));
-    float l = 0.0f;
-#pragma unroll
-    for (uint32_t i = 0; i < kMostParts / 64; i++) {
-        f[i] = exp2f(ml[i].x - top);
-        l += ml[i].y * f[i];
-    }
-    return make_float2(top, wave_reduce_sum(l));
-}
-
-// Joins the parts of rows, a wavefront per R rows of one tile, kFewParts parts at a time, added in order.
+// Joins the parts of rows, a wavefront per R rows of one tile.
 template <int HD, int R>
 __global__ __launch_bounds__(256) void kv_block_attention_join_few_kernel(AttentionArgs a, uint32_t tile_rows) {
-    constexpr int E = HD / 64;
     const uint32_t lane = threadIdx.x & 63, head = blockIdx.y, b = blockIdx.z;
     const uint32_t r0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)((blockIdx.x * 4 + (threadIdx.x >> 6)) * R));
     const KvSequence s = kv_sequence(a.kv, b);
@@ -980,46 +1047,7 @@ __global__ __launch_bounds__(256) void kv_block_attention_join_few_kernel(Attent
     PartRows part = part_rows(a, s, b, head, r0, rows, tile_rows);
     if (part.parts == 1) return;
     const uint32_t end = min(r0 + R, rows);
-    for (uint32_t r = r0; r < end; r++, part.first++, part.base++) {
-        float x[kFewParts][E], f[kMostParts / 64], o[E];
-        auto load = [&](uint32_t first) {
-#pragma unroll
-            for (uint32_t p = 0; p < kFewParts; p++)
-                if (first + p < part.parts) {
-                    const size_t at = part.at(first + p) * HD + lane;
-#pragma unroll
-                    for (int e = 0; e < E; e++) x[p][e] = a.part_out[at + e * 64];
-                }
-        };
-        load(0);
-        const float2 ml = join_sums(a.part_ml, part, lane, f);
-#pragma unroll
-        for (int e = 0; e < E; e++) o[e] = 0.0f;
-        for (uint32_t first = 0; first < part.parts; first += kFewParts) {
-            if (first) load(first);
-#pragma unroll
-            for (uint32_t p = 0; p < kFewParts; p++)
-                if (first + p < part.parts) {
-                    const float w = __shfl(first < 64 ? f[0] : f[1], (int)((first + p) & 63));
-#pragma unroll
-                    for (int e = 0; e < E; e++) o[e] += x[p][e] * w;
-                }
-        }
-        const uint32_t token = r / a.group, h = head * a.group + r % a.group;
-        const size_t row = (size_t)(s.row0 + (int32_t)token);
-        const float scale = ml.y == 0.0f ? 0.0f : 1.0f / ml.y;
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            const size_t at = row * a.out_stride + (size_t)h * HD + e * 64 + lane;
-            if (a.out_dtype == MI355Q_BF16) ((uint16_t*)a.out)[at] = f32_to_bf16_rne(o[e] * scale);
-            else ((uint16_t*)a.out)[at] = f32_to_f16_rne(o[e] * scale);
-        }
-        if (lane == 0) {
-            const float lse2 = ml.y == 0.0f ? -INFINITY : ml.x + log2f(ml.y);
-            if (a.lse) a.lse[row * a.heads + h] = lse2 * 0.6931471805599453f;
-            if (a.lse2) a.lse2[((size_t)b * a.kv.kv_heads + head) * a.score_rows + r] = lse2;
-        }
-    }
+    for (uint32_t r = r0; r < end; r++, part.first++, part.base++) join_parts<HD, false>(a, s, b, head, r, part, lane);
 }
 
 // Joins the parts of a row: one workgroup per row, 1024 / HD parts at a time, added in a fixed order.
@@ -1244,6 +1272,10 @@ mi355q_status launch_rows(mi355q_context* ctx, hipStream_t s, AttentionArgs a, b
             if (mi355q_status st = ensure_workspace(ctx, buf.used)) return st;
     }
     const dim3 grid(a.kv.kv_heads * a.parts, 1, a.kv.sequences);
+    // Few parts of at most four rows, one for each wavefront, are joined by the last of their workgroups (one sequence of 517
+    // tokens, 4 rows of 8 heads: 9.2 us, with a launch of its own 12.2; 8 of up to 2000 11.8 and 12.8; 16 rows 15.8 and 14.3)
+    static_assert(512 <= kArrivals);                       // (sequences and heads that are split are fewer)
+    if (!weights && rows <= 4 && a.parts > 1 && a.parts <= kFewParts) a.arrivals = ctx->arrivals;
     if (weights) kv_block_attention_rows_kernel<HD, RT, true><<<grid, 256, 0, s>>>(a);
     else kv_block_attention_rows_kernel<HD, RT, false><<<grid, 256, 0, s>>>(a);
     MI355Q_HIP(hipGetLastError());
@@ -1253,7 +1285,7 @@ mi355q_status launch_rows(mi355q_context* ctx, hipStream_t s, AttentionArgs a, b
         MI355Q_HIP(hipGetLastError());
         return MI355Q_OK;
     }
-    return a.parts > 1 ? launch_join<HD>(s, a, rows, 16 * RT) : MI355Q_OK;
+    return a.parts > 1 && !a.arrivals ? launch_join<HD>(s, a, rows, 16 * RT) : MI355Q_OK;
 }
 
 }  // namespace

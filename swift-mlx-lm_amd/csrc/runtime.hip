@@ -362,8 +362,11 @@ mi355q_status mi355q_context_create(int device_index, mi355q_context** out) {
     e = hipMalloc((void**)&ctx->argmax_scratch, 256);
     if (e == hipSuccess) e = hipMemset(ctx->argmax_scratch, 0, 256);
     if (e == hipSuccess) e = hipMalloc((void**)&ctx->argmax_partials, (size_t)(kArgmaxPartialCapacity + kArgmaxStandaloneKeys) * 8);
+    if (e == hipSuccess) e = hipMalloc((void**)&ctx->arrivals, kArrivals * sizeof(uint32_t));
+    if (e == hipSuccess) e = hipMemset(ctx->arrivals, 0, kArrivals * sizeof(uint32_t));
     if (e == hipSuccess) e = hipEventCreateWithFlags(&ctx->scratch_event, hipEventDisableTiming);
     if (e != hipSuccess) {
+        if (ctx->arrivals) (void)hipFree(ctx->arrivals);
         if (ctx->scratch_event) (void)hipEventDestroy(ctx->scratch_event);
         if (ctx->argmax_scratch) (void)hipFree(ctx->argmax_scratch);
         if (ctx->argmax_partials) (void)hipFree(ctx->argmax_partials);
@@ -397,6 +400,7 @@ mi355q_status mi355q_context_destroy(mi355q_context* ctx) {
     mi355q::dense_library_release(ctx);
     if (ctx->scratch_event) (void)hipEventDestroy(ctx->scratch_event);
     if (ctx->argmax_scratch) (void)hipFree(ctx->argmax_scratch);
+    if (ctx->arrivals) (void)hipFree(ctx->arrivals);
     if (ctx->argmax_partials) (void)hipFree(ctx->argmax_partials);
     if (ctx->workspace) (void)hipFree(ctx->workspace);
     if (ctx->split_buffer) (void)hipFree(ctx->split_buffer);

@@ -34,6 +34,7 @@ struct LogprobArgs {
     // partial results of a slice: (m, l, t, unused), then `top` keys, largest first (0: none)
     float4* parts;
     unsigned long long* part_keys;
+    uint32_t* arrivals;       // of each row's slices; null: a launch of its own joins them
 };
 
 __device__ __forceinline__ unsigned long long logit_key(float v, uint32_t index) {
@@ -167,6 +168,54 @@ __device__ void write_row(const LogprobArgs& a, uint32_t row, const LogSum& s, c
 template <int D>
 __device__ __forceinline__ float logit_at(const LogprobArgs& a, size_t row_at, uint32_t lead, uint32_t at) {
     return at >= lead && at < a.vocabulary + lead ? load_act<D>(a.logits, row_at + (at - lead)) : kMasked;
+}
+
+// Joins the slices of a row, by one wavefront; `room` is LDS of its own.
+template <int D>
+__device__ void join_slices(const LogprobArgs& a, uint32_t row, uint32_t lane, unsigned long long* room) {
+    LogSum s{kMasked, 0.0f, 0.0f};
+    for (uint32_t i = lane; i < a.slices; i += 64) {
+        const float* const p = (const float*)(a.parts + (size_t)row * a.slices + i);
+        const float2 ml = share_load2(p);
+        s.join(ml.x, ml.y, share_load(p + 2));
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        const float om = __shfl_xor(s.m, o), ol = __shfl_xor(s.l, o), ot = __shfl_xor(s.t, o);
+        s.join(om, ol, ot);
+    }
+    if (a.top) {
+        TopKeys keys{room, kMaskedKey, 0, a.top, lane};
+        const size_t base = (size_t)row * a.slices * a.top;
+        const uint32_t all = a.slices * a.top;
+        if (all > 64) {
+            // a limit that `top` keys reach: the slices' keys are in order, so if n of their q-th keys reach it, n q do
+            const uint32_t lists = a.slices < 64 ? a.slices : 64, q = (a.top + lists - 1) / lists, n = (a.top + q - 1) / q;
+            const unsigned long long own = lane < lists ? share_load(a.part_keys + base + (size_t)lane * a.top + q - 1) : 0;
+            room[lane] = own;
+            wave_lds_order();
+            uint32_t above = 0;
+#pragma unroll 8
+            for (uint32_t k = 0; k < 64; k++) above += room[k] > own || (room[k] == own && k < lane) ? 1u : 0u;
+            const int holder = (int)__builtin_ctzll(__ballot(above == n - 1));
+            const unsigned long long limit = ((unsigned long long)(uint32_t)__shfl((int)(own >> 32), holder) << 32) |
+                                             (uint32_t)__shfl((int)(uint32_t)own, holder);
+            wave_lds_order();
+            if (limit > keys.threshold) keys.threshold = limit - 1;
+        }
+        for (uint32_t i = 0; i < all; i += 64) keys.push(i + lane < all ? share_load(a.part_keys + base + i + lane) : 0);
+        keys.cut();
+        if (lane >= keys.count && lane < a.top) room[lane] = 0;
+        wave_lds_order();
+    }
+    write_row<D>(a, row, s, room, lane);
+}
+
+// One wavefront per row joins its slices, where the rows are more than the counters of the last arrivals.
+template <int D>
+__global__ __launch_bounds__(64) void token_logprobs_join_kernel(LogprobArgs a) {
+    __shared__ unsigned long long room[kTopRoom];
+    join_slices<D>(a, blockIdx.x, threadIdx.x, room);
 }
 
 // One workgroup per slice of a row; its wavefronts take steps of 1024 logits in turn.
@@ -305,50 +354,14 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(LogprobArgs a) {
         write_row<D>(a, row, s, room[0], lane);
         return;
     }
-    if (lane == 0) a.parts[blockIdx.x] = make_float4(s.m, s.l, s.t, 0.0f);
-    if (lane < a.top) a.part_keys[(size_t)blockIdx.x * a.top + lane] = room[0][lane];
-}
-
-// One wavefront per row joins its slices.
-template <int D>
-__global__ __launch_bounds__(64) void token_logprobs_join_kernel(LogprobArgs a) {
-    __shared__ unsigned long long room[kTopRoom];
-    const uint32_t row = blockIdx.x, lane = threadIdx.x;
-    LogSum s{kMasked, 0.0f, 0.0f};
-    for (uint32_t i = lane; i < a.slices; i += 64) {
-        const float4 p = a.parts[(size_t)row * a.slices + i];
-        s.join(p.x, p.y, p.z);
+    if (lane == 0) {
+        float* const p = (float*)(a.parts + blockIdx.x);
+        share_store(p, s.m, s.l);
+        share_store(p + 2, s.t);
     }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-        const float om = __shfl_xor(s.m, o), ol = __shfl_xor(s.l, o), ot = __shfl_xor(s.t, o);
-        s.join(om, ol, ot);
-    }
-    if (a.top) {
-        TopKeys keys{room, kMaskedKey, 0, a.top, lane};
-        const size_t base = (size_t)row * a.slices * a.top;
-        const uint32_t all = a.slices * a.top;
-        if (all > 64) {
-            // a limit that `top` keys reach: the slices' keys are in order, so if n of their q-th keys reach it, n q do
-            const uint32_t lists = a.slices < 64 ? a.slices : 64, q = (a.top + lists - 1) / lists, n = (a.top + q - 1) / q;
-            const unsigned long long own = lane < lists ? a.part_keys[base + (size_t)lane * a.top + q - 1] : 0;
-            room[lane] = own;
-            wave_lds_order();
-            uint32_t above = 0;
-#pragma unroll 8
-            for (uint32_t k = 0; k < 64; k++) above += room[k] > own || (room[k] == own && k < lane) ? 1u : 0u;
-            const int holder = (int)__builtin_ctzll(__ballot(above == n - 1));
-            const unsigned long long limit = ((unsigned long long)(uint32_t)__shfl((int)(own >> 32), holder) << 32) |
-                                             (uint32_t)__shfl((int)(uint32_t)own, holder);
-            wave_lds_order();
-            if (limit > keys.threshold) keys.threshold = limit - 1;
-        }
-        for (uint32_t i = 0; i < all; i += 64) keys.push(i + lane < all ? a.part_keys[base + i + lane] : 0);
-        keys.cut();
-        if (lane >= keys.count && lane < a.top) room[lane] = 0;
-        wave_lds_order();
-    }
-    write_row<D>(a, row, s, room, lane);
+    if (lane < a.top) share_store(a.part_keys + (size_t)blockIdx.x * a.top + lane, room[0][lane]);
+    // the last of the row's workgroups joins its slices
+    if (a.arrivals && arrive_last(a.arrivals + row, a.slices)) join_slices<D>(a, row, lane, room[0]);
 }
 
 namespace {
@@ -371,7 +384,7 @@ template <int D>
 mi355q_status launch_logprobs(hipStream_t s, const LogprobArgs& a) {
     token_logprobs_kernel<D><<<dim3(a.rows * a.slices), 256, 0, s>>>(a);
     MI355Q_HIP(hipGetLastError());
-    if (a.slices > 1) {
+    if (a.slices > 1 && !a.arrivals) {
         token_logprobs_join_kernel<D><<<dim3(a.rows), 64, 0, s>>>(a);
         MI355Q_HIP(hipGetLastError());
     }
@@ -401,7 +414,7 @@ mi355q_status dispatch_token_logprobs(mi355q_context* ctx, hipStream_t s, const 
         (uintptr_t)entropy % 4 || (uintptr_t)top_ids % 4 || (uintptr_t)top_logprobs % 4)
         return fail(MI355Q_ERR_INVALID_ARGUMENT, "misaligned pointer");
     LogprobArgs a{logits, tokens, logprob, entropy, top_ids, top_logprobs,
-                  rows, vocabulary, row_stride, top, 1, 0, nullptr, nullptr};
+                  rows, vocabulary, row_stride, top, 1, 0, nullptr, nullptr, nullptr};
     logprob_slices(&a);
     if ((uint64_t)a.rows * a.slices >= (1u << 24))
         return fail(MI355Q_ERR_SHAPE, "%u rows of %u logits: too many for one launch", rows, vocabulary);
@@ -413,6 +426,7 @@ mi355q_status dispatch_token_logprobs(mi355q_context* ctx, hipStream_t s, const 
         if (mi355q_status st = ensure_workspace(ctx, parts * (sizeof(float4) + a.top * 8))) return st;
         a.parts = (float4*)ctx->workspace;
         a.part_keys = (unsigned long long*)(a.parts + parts);
+        a.arrivals = a.rows <= kArrivals ? ctx->arrivals : nullptr;
     }
     if (dtype == MI355Q_F32) return launch_logprobs<MI355Q_F32>(s, a);
     if (dtype == MI355Q_BF16) return launch_logprobs<MI355Q_BF16>(s, a);
