@@ -268,7 +268,7 @@ __device__ __forceinline__ void join_parts(const AttentionArgs& a, const KvSeque
 // each with accumulators of its own, which are added at the end.  HBM-bound: codes go from memory to registers in the order
 // the matrix cores take them, a block ahead, and every row of the group uses them.  (32 sequences of 8192 tokens, 32 heads of 128
 // on 8: 88 us, 6.1 TB/s, where a kernel that only reads reaches 7.1; of 2394 to 8192 tokens 61 us, 5.4 TB/s; 16 of up to 16000
-// tokens, 16 heads of 256 on 4, 64 us.  One sequence of 517 tokens: 6.5 us and 3 for joining, latency.)  Storing the scores for
+// tokens, 16 heads of 256 on 4, 64 us.  One sequence of 517 tokens: 8.9 us, joined, latency.)  Storing the scores for
 // the weight sums costs the second of these 9 us for 21 MB; rows side by side in sixteens of tokens make whole lines of them
 // (rows behind blocks of 64 tokens: 16).
 // SCORES: they are stored for the weight sums (apart, since their addresses cost registers that 32 rows do not have to spare).
